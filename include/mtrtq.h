@@ -504,6 +504,110 @@ int mtrtq_argmax_rows(const float* logits, int64_t rows, int64_t V, int64_t ldl,
 int mtrtq_decode_next(unsigned long long* best, int64_t rows, int32_t* tok, int32_t* history,
                       int64_t history_len, int32_t* pos, void* stream);
 
+/* ---- serving many requests from one paged cache ---------------------------------
+ * The reference decodes one sequence over contiguous caches (KVDecoder,
+ * tools/run_gpt2.cpp:88-191). These calls serve requests of different lengths
+ * together: prompts packed one after another, a key/value cache in pages, and beam
+ * search over it. Everything that changes from step to step (lengths, page numbers,
+ * scores) is read from device memory, so a step can be captured in a CUDA graph.
+ *
+ * Attention, for a row of query head h and position i of its request, over the keys j
+ * the row sees (those of its request with j <= i; head h reads key/value head
+ * h / (heads / kv_heads)):
+ *   s_j = scale * sum_d q_d k_jd,  p_j = exp(s_j - max s) / sum exp(s - max s),
+ *   out_d = sum_j p_j v_jd;
+ * a row that sees no key gives zeros. Keys outside a row's view have no effect on it,
+ * whatever they hold (infinities and NaN included).
+ *
+ * Element types: x_dtype of q, k and v; dtype of the cache and of out. Both f32: every
+ * product and sum in fp32. dtype bf16 (x_dtype f32 or bf16): k and v are rounded to
+ * bf16 as they are stored, q and the weights p are rounded to bf16 for the tensor
+ * cores' products, the maximum, the sum and the output are held in fp32 and out is
+ * rounded once. x_dtype bf16 with dtype f32 is refused.
+ *
+ * The packed rows are given by cu_rows: request b owns rows cu_rows[b] ..
+ * cu_rows[b+1] - 1 of q, k, v and out (non-decreasing; a request may own none; values
+ * are clamped to [0, rows]). Rows outside every request are left as they are.
+ * Strides are in elements: row r, head h, dimension d is at r * row + h * head + d.
+ * head_dim is a multiple of 8 up to 128, heads / kv_heads is whole and at most 128,
+ * batch is at most 1024; pointers are 16-byte aligned and strides multiples of 16
+ * bytes (else MTRTQ_ERR_ALIGNMENT); scale is positive and finite.
+ *
+ * Paged cache: page n holds page_size (16, 32, 64 or 128) tokens of every key/value
+ * head, [kv_heads, page_size, head_dim] contiguous, page_stride elements after page
+ * n - 1. Token i of request b is in page table[b * table_ld + i / page_size]. kv_len[b]
+ * counts the request's tokens after this call; its new tokens (its rows) are the last
+ * of them, so a row t of m sits at position kv_len[b] - m + t. Page numbers outside
+ * [0, num_pages), and positions past table_width pages, are not touched; keys there
+ * read as unseen. */
+#define MTRTQ_MAX_BATCH 1024
+typedef struct mtrtq_attention_args {
+  const void *q, *k, *v; /* device; paged: k and v may both be NULL (the pages already hold the new tokens) */
+  void* out;             /* device; [rows, heads, head_dim] by its strides */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  int64_t rows, batch;
+  int heads, kv_heads, head_dim;
+  int x_dtype, dtype; /* MTRTQ_DTYPE_* */
+  float scale;
+  const int32_t* cu_rows; /* device [batch + 1] */
+  /* paged only */
+  void *k_pages, *v_pages;
+  int64_t page_stride, num_pages;
+  int page_size;
+  const int32_t* table; /* device [batch, table_ld] */
+  int64_t table_ld, table_width;
+  const int32_t* kv_len; /* device [batch] */
+} mtrtq_attention_args;
+
+/* Workspace of either call for these arguments (paged: k_pages is set); depends on
+ * the sizes and types alone. 256-byte aligned, zero-filled once after allocation
+ * (calls leave its counters at zero; after a MTRTQ_ERR_TIMEOUT fill it again); calls
+ * that share it must be ordered. Returns -1 for arguments the calls would refuse. */
+int64_t mtrtq_attention_workspace_bytes(const mtrtq_attention_args* a);
+/* Causal attention of whole packed prompts (the reference attends one position at a
+ * time, tools/run_gpt2.cpp:146-172). */
+int mtrtq_prompt_attention(const mtrtq_attention_args* a, void* workspace, size_t workspace_bytes,
+                           void* stream);
+/* The new tokens' keys and values go into the pages, then their rows attend to all
+ * their request has cached: one token for each request (decoding), chunks of a
+ * prompt, or both in one call. */
+int mtrtq_paged_attention(const mtrtq_attention_args* a, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* One step of beam search for `requests` requests of `beams` beams each (1..32):
+ * candidate (w, t) of a request has the score scores[w] + log_softmax(logits[w])[t],
+ * and a beam that is done the single candidate (w, eos) with its own score; the best
+ * `beams` candidates, by score and then by lowest w * vocab + t, become the beams:
+ * out_scores, parent (their w), token (their t) and out_done (the parent's, or token ==
+ * eos), best first. logits [requests * beams, ldl] f32; scores, done (0 or 1), parent,
+ * token, out_scores, out_done [requests, beams]. NaN logits count as -infinity, so do
+ * candidates whose score is NaN; a beam not in use has the score -infinity. eos may be
+ * -1 (none ends; done must then be 0). outputs must not overlap inputs.
+ * beams * vocab is below 2^31. The greedy step is mtrtq_argmax_rows
+ * (tools/run_gpt2.cpp:42-47). */
+#define MTRTQ_MAX_BEAMS 32
+int64_t mtrtq_beam_workspace_bytes(int64_t requests, int64_t beams, int64_t vocab);
+int mtrtq_beam_select(const float* logits, int64_t ldl, const float* scores, const uint8_t* done, int32_t eos,
+                      int64_t requests, int64_t beams, int64_t vocab, float* out_scores, int32_t* parent,
+                      int32_t* token, uint8_t* out_done, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The cached states follow their beams: beam i of a request continues beam parent[i].
+ * Row r = request * beams + i of `owned` [requests * beams, owned_ld] lists the pages
+ * that only beam i writes, row r of `table` [.., table_ld] those it reads; both have
+ * `width` columns. With n = kv_len[request] cached tokens, the n / page_size full pages
+ * are never written again and are shared: the columns before that one are taken from
+ * the parent's row of the table. The n % page_size tokens of the page that is still
+ * being filled are copied from the parent's owned page to the beam's own (in place
+ * over all beams of the request at once, in every layer), and that column and the
+ * later ones are the owned pages. Pages as in mtrtq_attention_args, `layers` of them
+ * layer_stride elements apart. A parent outside [0, beams) counts as the beam itself;
+ * page numbers outside [0, num_pages) are not touched. No two rows own the same page
+ * in a column from n / page_size on. */
+int mtrtq_beam_reorder(const int32_t* parent, int64_t requests, int64_t beams, int32_t* table, int64_t table_ld,
+                       const int32_t* owned, int64_t owned_ld, int64_t width, const int32_t* kv_len,
+                       void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride, int64_t page_stride,
+                       int64_t num_pages, int kv_heads, int page_size, int head_dim, int dtype, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -114,6 +114,30 @@ SIGNATURES["mtrtq_gemv_group_workspace_bytes"] = (_i64, [_vp, _int])
 SIGNATURES["mtrtq_gemv_group"] = (_int, [_vp, _int, _int, _int, _vp, _sz, _vp])
 SIGNATURES["mtrtq_gemv_group_allgather"] = (_int, [_vp, _int, _int, _int, _vp, _sz, _vp, ctypes.c_uint, _vp])
 
+MAX_BATCH = 1024
+MAX_BEAMS = 32
+
+
+class AttentionArgs(ctypes.Structure):
+    """mtrtq_attention_args (include/mtrtq.h)."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("q_row", _i64), ("q_head", _i64),
+                ("k_row", _i64), ("k_head", _i64), ("v_row", _i64), ("v_head", _i64), ("out_row", _i64),
+                ("out_head", _i64), ("rows", _i64), ("batch", _i64), ("heads", _int), ("kv_heads", _int),
+                ("head_dim", _int), ("x_dtype", _int), ("dtype", _int), ("scale", ctypes.c_float),
+                ("cu_rows", _vp), ("k_pages", _vp), ("v_pages", _vp), ("page_stride", _i64),
+                ("num_pages", _i64), ("page_size", _int), ("table", _vp), ("table_ld", _i64),
+                ("table_width", _i64), ("kv_len", _vp)]
+
+
+SIGNATURES["mtrtq_attention_workspace_bytes"] = (_i64, [_vp])
+SIGNATURES["mtrtq_prompt_attention"] = (_int, [_vp, _vp, _sz, _vp])
+SIGNATURES["mtrtq_paged_attention"] = (_int, [_vp, _vp, _sz, _vp])
+SIGNATURES["mtrtq_beam_workspace_bytes"] = (_i64, [_i64, _i64, _i64])
+SIGNATURES["mtrtq_beam_select"] = (_int, [_vp, _i64, _vp, _vp, ctypes.c_int32, _i64, _i64, _i64, _vp, _vp, _vp,
+                                          _vp, _vp, _sz, _vp])
+SIGNATURES["mtrtq_beam_reorder"] = (_int, [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64,
+                                           _i64, _i64, _int, _int, _int, _int, _vp])
+
 
 class MtrtqError(RuntimeError):
     """A non-zero status from the C ABI."""
