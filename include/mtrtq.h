@@ -538,8 +538,8 @@ int mtrtq_decode_next(unsigned long long* best, int64_t rows, int32_t* tok, int3
  * n - 1. Token i of request b is in page table[b * table_ld + i / page_size]. kv_len[b]
  * counts the request's tokens after this call; its new tokens (its rows) are the last
  * of them, so a row t of m sits at position kv_len[b] - m + t. Page numbers outside
- * [0, num_pages), and positions past table_width pages, are not touched; keys there
- * read as unseen. */
+ * [0, num_pages) are never touched: tokens there are not stored and read as zeros.
+ * Positions past table_width pages are not stored and not seen. */
 #define MTRTQ_MAX_BATCH 1024
 typedef struct mtrtq_attention_args {
   const void *q, *k, *v; /* device; paged: k and v may both be NULL (the pages already hold the new tokens) */

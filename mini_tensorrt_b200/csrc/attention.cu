@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include "../../include/mtrtq.h"
+#include "attention.h"
 #include "q8_common.cuh"
 
 namespace mtrtq {
@@ -44,7 +45,8 @@ __device__ int64_t request_of(const Args& a, int64_t r) {
   return r >= r0 && r < r1 ? lo : -1;
 }
 
-// Where token i of request b lies in the pages of head g (elements), or -1.
+// Where token i of request b lies in the pages of head g (elements); -1 if its page
+// number is out of range.
 __device__ __forceinline__ int64_t page_offset(const Args& a, int64_t b, int64_t i, int64_t g) {
   const int64_t c = i / a.page_size;
   if (i < 0 || c >= a.table_width) return -1;
@@ -54,10 +56,19 @@ __device__ __forceinline__ int64_t page_offset(const Args& a, int64_t b, int64_t
 }
 
 // One block per new row: its k and v go to its position's page, rounded to the
-// cache's type.
+// cache's type; q_rows (if not null) gets q in that type, [rows, heads, head_dim].
 template <typename TX, typename TC>
-__global__ void append_kernel(const __grid_constant__ Args a) {
+__global__ void append_kernel(const __grid_constant__ Args a, TC* q_rows) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t r = blockIdx.x;
+  if (q_rows) {
+    for (int e = threadIdx.x; e < a.heads * a.head_dim; e += blockDim.x) {
+      const int h = e / a.head_dim, d = e - h * a.head_dim;
+      q_rows[r * a.heads * a.head_dim + e] =
+          from_f32<TC>(to_f32(static_cast<const TX*>(a.q)[r * a.q_row + h * a.q_head + d]));
+    }
+  }
+  if (!a.k) return;
   const int64_t b = request_of(a, r);
   if (b < 0) return;
   int64_t r0, r1;
@@ -71,6 +82,21 @@ __global__ void append_kernel(const __grid_constant__ Args a) {
         from_f32<TC>(to_f32(static_cast<const TX*>(a.k)[r * a.k_row + g * a.k_head + d]));
     static_cast<TC*>(a.v_pages)[at + d] =
         from_f32<TC>(to_f32(static_cast<const TX*>(a.v)[r * a.v_row + g * a.v_head + d]));
+  }
+}
+
+// Rows of q, k and v in bf16, [rows, heads + 2 kv_heads, head_dim].
+template <typename TX>
+__global__ void cast_kernel(const __grid_constant__ Args a, __nv_bfloat16* rows) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t r = blockIdx.x;
+  const int hq = a.heads, hk = a.kv_heads, all = hq + 2 * hk;
+  for (int e = threadIdx.x; e < all * a.head_dim; e += blockDim.x) {
+    const int h = e / a.head_dim, d = e - h * a.head_dim;
+    const TX* src = h < hq        ? static_cast<const TX*>(a.q) + r * a.q_row + h * a.q_head
+                    : h < hq + hk ? static_cast<const TX*>(a.k) + r * a.k_row + (h - hq) * a.k_head
+                                  : static_cast<const TX*>(a.v) + r * a.v_row + (h - hq - hk) * a.v_head;
+    rows[r * all * a.head_dim + e] = from_f32<__nv_bfloat16>(to_f32(src[d]));
   }
 }
 
@@ -97,14 +123,13 @@ __global__ void __launch_bounds__(32) rows_kernel(const __grid_constant__ Args a
   float m = -INFINITY, l = 0.0f;
   for (int64_t j = 0; j <= last; ++j) {
     const int64_t at = PAGED ? page_offset(a, b, j, g) : 0;
-    if (at < 0) continue;
     float s = 0.0f, v[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int d = c * 32 + lane;
       float k = 0.0f;
       v[c] = 0.0f;
-      if (d < a.head_dim) {
+      if (d < a.head_dim && at >= 0) {
         if (PAGED) {
           k = to_f32(static_cast<const TC*>(a.k_pages)[at + d]);
           v[c] = to_f32(static_cast<const TC*>(a.v_pages)[at + d]);
@@ -181,22 +206,162 @@ int check_args(const Args* a, bool paged) {
   return MTRTQ_OK;
 }
 
-template <typename TX, typename TC>
-int launch(const Args& a, bool paged, cudaStream_t st) {
-  if (paged) {
-    if (a.k) append_kernel<TX, TC><<<(unsigned)a.rows, 128, 0, st>>>(a);
-    rows_kernel<TX, TC, true><<<dim3((unsigned)a.rows, a.heads), 32, 0, st>>>(a);
-  } else {
-    rows_kernel<TX, TC, false><<<dim3((unsigned)a.rows, a.heads), 32, 0, st>>>(a);
+int cuda_status(cudaError_t e, const char* what) {
+  return e == cudaSuccess ? MTRTQ_OK : report_cuda_error(e, what);
+}
+
+size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+
+// Workspace of the tensor-core path: tickets | cast rows | partials of cut tiles.
+struct TcLayout {
+  int grid, slot_tokens, part_rows;
+  bool cast;
+  size_t off_rows, off_ml, off_part, total;
+};
+
+// TMA reads rows of the kernel's own type whose strides are not zero.
+bool needs_cast(const Args& a) {
+  return a.x_dtype == MTRTQ_DTYPE_F32 || a.q_row == 0 || a.q_head == 0 ||
+         (!a.k_pages && (a.k_row == 0 || a.k_head == 0 || a.v_row == 0 || a.v_head == 0));
+}
+
+TcLayout tc_layout(const Args& a, int sm_count) {
+  TcLayout l;
+  l.grid = sm_count;
+  const int group = a.heads / a.kv_heads;
+  l.slot_tokens = 128 / group;
+  l.part_rows = a.rows > l.slot_tokens ? 256 : (int)((a.rows * group + 31) / 32 * 32);
+  l.cast = needs_cast(a);
+  const int dp = a.head_dim <= 64 ? 64 : 128, heads = a.heads + (a.k_pages ? 0 : 2 * a.kv_heads);
+  l.off_rows = round256((size_t)l.grid * sizeof(unsigned));
+  l.off_ml = l.off_rows + (l.cast ? round256((size_t)a.rows * heads * a.head_dim * 2) : 0);
+  l.off_part = l.off_ml + round256((size_t)l.grid * 2 * l.part_rows * sizeof(float2));
+  l.total = l.off_part + (size_t)l.grid * 2 * l.part_rows * dp * sizeof(float);
+  return l;
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// bf16, 128-byte-swizzled boxes of 64 dimensions; strides in elements, of dimension 1 on.
+int make_map(CUtensorMap* map, const void* base, int rank, const int64_t* dims, const int64_t* strides, const int* box) {
+  static const EncodeFn encode = reinterpret_cast<EncodeFn>(tensor_map_encoder());
+  if (!encode) return report_error(MTRTQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], one[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = (cuuint64_t)dims[i];
+    b[i] = (cuuint32_t)box[i];
+    one[i] = 1;
+    if (i) s[i - 1] = (cuuint64_t)strides[i - 1] * 2;
   }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? MTRTQ_OK : report_cuda_error(e, "attention launch");
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s, b, one,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? MTRTQ_OK : report_error(MTRTQ_ERR_CUDA, "tensor map: driver error %d", (int)r);
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
+  }
+  return n;
+}
+
+int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cudaStream_t st) {
+  const TcLayout l = tc_layout(a, sm_count());
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  __nv_bfloat16* rows = reinterpret_cast<__nv_bfloat16*>(ws + l.off_rows);
+  Args x = a;
+  const bool before = l.cast || (paged && a.k);
+  if (before) {
+    if (!paged) {
+      if (a.x_dtype == MTRTQ_DTYPE_F32) cast_kernel<float><<<(unsigned)a.rows, 256, 0, st>>>(a, rows);
+      else cast_kernel<__nv_bfloat16><<<(unsigned)a.rows, 256, 0, st>>>(a, rows);
+    } else if (a.x_dtype == MTRTQ_DTYPE_F32) {
+      append_kernel<float, __nv_bfloat16><<<(unsigned)a.rows, 256, 0, st>>>(a, l.cast ? rows : nullptr);
+    } else {
+      append_kernel<__nv_bfloat16, __nv_bfloat16><<<(unsigned)a.rows, 256, 0, st>>>(a, l.cast ? rows : nullptr);
+    }
+    if (int rc = cuda_status(cudaGetLastError(), "attention rows launch")) return rc;
+  }
+  if (l.cast) {
+    const int64_t row = (int64_t)(a.heads + (paged ? 0 : 2 * a.kv_heads)) * a.head_dim;
+    x.q = rows;
+    x.k = rows + (int64_t)a.heads * a.head_dim;
+    x.v = rows + (int64_t)(a.heads + a.kv_heads) * a.head_dim;
+    x.q_row = x.k_row = x.v_row = row;
+    x.q_head = x.k_head = x.v_head = a.head_dim;
+  }
+  const int group = a.heads / a.kv_heads;
+  CUtensorMap qm, km, vm;
+  {
+    const int64_t dims[4] = {a.head_dim, group, a.kv_heads, a.rows};
+    const int64_t strides[3] = {x.q_head, x.q_head * group, x.q_row};
+    const int box[4] = {64, group, 1, l.slot_tokens};
+    if (int rc = make_map(&qm, x.q, 4, dims, strides, box)) return rc;
+  }
+  for (int i = 0; i < 2; ++i) {
+    int rc;
+    if (paged) {
+      const int64_t dims[3] = {a.head_dim, (int64_t)a.kv_heads * a.page_size, a.num_pages};
+      const int64_t strides[2] = {a.head_dim, a.page_stride};
+      const int box[3] = {64, a.page_size, 1};
+      rc = make_map(i ? &vm : &km, i ? a.v_pages : a.k_pages, 3, dims, strides, box);
+    } else {
+      const int64_t dims[3] = {a.head_dim, a.kv_heads, a.rows};
+      const int64_t strides[2] = {i ? x.v_head : x.k_head, i ? x.v_row : x.k_row};
+      const int box[3] = {64, 1, 128};
+      rc = make_map(i ? &vm : &km, i ? x.v : x.k, 3, dims, strides, box);
+    }
+    if (rc) return rc;
+  }
+  TcAttention p = {};
+  p.cu_rows = a.cu_rows;
+  p.kv_len = paged ? a.kv_len : nullptr;
+  p.table = paged ? a.table : nullptr;
+  p.table_ld = a.table_ld;
+  p.rows = a.rows;
+  p.batch = (int)a.batch;
+  p.kv_heads = a.kv_heads;
+  p.group = group;
+  p.head_dim = a.head_dim;
+  p.page_size = a.page_size;
+  p.slot_tokens = l.slot_tokens;
+  p.max_keys = a.table_width * a.page_size;
+  p.min_steps = 2;
+  p.scale = a.scale;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.out_row = a.out_row;
+  p.out_head = a.out_head;
+  p.v = static_cast<const __nv_bfloat16*>(paged ? a.v_pages : x.v);
+  p.v_row = paged ? a.page_stride : x.v_row;
+  p.v_head = x.v_head;
+  p.counters = reinterpret_cast<unsigned*>(ws);
+  p.partials = reinterpret_cast<float*>(ws + l.off_part);
+  p.part_ml = reinterpret_cast<float2*>(ws + l.off_ml);
+  p.part_rows = l.part_rows;
+  p.status = status;
+  return cuda_status(launch_attention_tc(p, qm, km, vm, l.grid, before, st), "attention launch");
+}
+
+int launch_f32(const Args& a, bool paged, cudaStream_t st) {
+  if (paged) {
+    if (a.k) append_kernel<float, float><<<(unsigned)a.rows, 128, 0, st>>>(a, nullptr);
+    rows_kernel<float, float, true><<<dim3((unsigned)a.rows, a.heads), 32, 0, st>>>(a);
+  } else {
+    rows_kernel<float, float, false><<<dim3((unsigned)a.rows, a.heads), 32, 0, st>>>(a);
+  }
+  return cuda_status(cudaGetLastError(), "attention launch");
 }
 
 int attention(const Args* a, bool paged, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_args(a, paged)) return rc;
   int rc;
-  device_status_address(&rc);
+  unsigned* status = device_status_address(&rc);
   if (rc) return rc;
   if (a->rows == 0) return MTRTQ_OK;
   const int64_t need = mtrtq_attention_workspace_bytes(a);
@@ -205,9 +370,8 @@ int attention(const Args* a, bool paged, void* workspace, size_t workspace_bytes
   if (reinterpret_cast<uintptr_t>(workspace) % 256)
     return report_error(MTRTQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == MTRTQ_DTYPE_F32) return launch<float, float>(*a, paged, st);
-  if (a->x_dtype == MTRTQ_DTYPE_F32) return launch<float, __nv_bfloat16>(*a, paged, st);
-  return launch<__nv_bfloat16, __nv_bfloat16>(*a, paged, st);
+  if (a->dtype == MTRTQ_DTYPE_F32) return launch_f32(*a, paged, st);
+  return launch_tc(*a, paged, workspace, status, st);
 }
 
 }  // namespace
@@ -219,7 +383,7 @@ extern "C" {
 
 int64_t mtrtq_attention_workspace_bytes(const mtrtq_attention_args* a) {
   if (check_args(a, a && a->k_pages)) return -1;
-  return 4096;
+  return a->dtype == MTRTQ_DTYPE_F32 ? 4096 : (int64_t)tc_layout(*a, sm_count()).total;
 }
 
 int mtrtq_prompt_attention(const mtrtq_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {

@@ -946,6 +946,8 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
+void* tensor_map_encoder() { return reinterpret_cast<void*>(get_encode_fn()); }
+
 int make_x_tensor_map(CUtensorMap* map, const void* X, int64_t M, int64_t K, int64_t ldx,
                       int tile_m, bool x_f32) {
   EncodeTiledFn enc = get_encode_fn();

@@ -211,6 +211,9 @@ bool skinny_x_resident(int tile_m, int64_t k_pad);
 int make_x_tensor_map(CUtensorMap* map, const void* X, int64_t M, int64_t K, int64_t ldx,
                       int tile_m, bool x_f32 = false);
 
+// cuTensorMapEncodeTiled, or null.
+void* tensor_map_encoder();
+
 // GEMM tile sizes with a compiled kernel.
 bool gemm_tile_supported(int tile_m);
 
