@@ -560,7 +560,8 @@ typedef struct mtrtq_attention_args {
 } mtrtq_attention_args;
 
 /* Workspace of either call for these arguments (paged: k_pages is set); depends on
- * the sizes and types alone. 256-byte aligned, zero-filled once after allocation
+ * the sizes and types alone. Its first 4 KiB hold tickets, as in mtrtq_matmul's, so one
+ * workspace may serve both and mtrtq_beam_select too. 256-byte aligned, zero-filled once after allocation
  * (calls leave its counters at zero; after a MTRTQ_ERR_TIMEOUT fill it again); calls
  * that share it must be ordered. Returns -1 for arguments the calls would refuse. */
 int64_t mtrtq_attention_workspace_bytes(const mtrtq_attention_args* a);
@@ -574,7 +575,7 @@ int mtrtq_prompt_attention(const mtrtq_attention_args* a, void* workspace, size_
 int mtrtq_paged_attention(const mtrtq_attention_args* a, void* workspace, size_t workspace_bytes,
                           void* stream);
 
-/* One step of beam search for `requests` requests of `beams` beams each (1..32):
+/* One step of beam search for `requests` requests (1..MTRTQ_MAX_BATCH) of `beams` beams each (1..32):
  * candidate (w, t) of a request has the score scores[w] + log_softmax(logits[w])[t],
  * and a beam that is done the single candidate (w, eos) with its own score; the best
  * `beams` candidates, by score and then by lowest w * vocab + t, become the beams:

@@ -212,7 +212,7 @@ int cuda_status(cudaError_t e, const char* what) {
 
 size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-// Workspace of the tensor-core path: tickets | cast rows | partials of cut tiles.
+// Workspace of the tensor-core path: 4 KiB of tickets, as in every call's | cast rows | partials of cut tiles.
 struct TcLayout {
   int grid, slot_tokens, part_rows;
   bool cast;
@@ -227,13 +227,13 @@ bool needs_cast(const Args& a) {
 
 TcLayout tc_layout(const Args& a, int sm_count) {
   TcLayout l;
-  l.grid = sm_count;
+  l.grid = sm_count < 1024 ? sm_count : 1024;  // a ticket each
   const int group = a.heads / a.kv_heads;
   l.slot_tokens = 128 / group;
   l.part_rows = a.rows > l.slot_tokens ? 256 : (int)((a.rows * group + 31) / 32 * 32);
   l.cast = needs_cast(a);
   const int dp = a.head_dim <= 64 ? 64 : 128, heads = a.heads + (a.k_pages ? 0 : 2 * a.kv_heads);
-  l.off_rows = round256((size_t)l.grid * sizeof(unsigned));
+  l.off_rows = 4096;
   l.off_ml = l.off_rows + (l.cast ? round256((size_t)a.rows * heads * a.head_dim * 2) : 0);
   l.off_part = l.off_ml + round256((size_t)l.grid * 2 * l.part_rows * sizeof(float2));
   l.total = l.off_part + (size_t)l.grid * 2 * l.part_rows * dp * sizeof(float);

@@ -30,6 +30,39 @@ __device__ __forceinline__ uint32_t key_index(unsigned long long key) { return ~
 __device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY; }
 
 constexpr int kThreads = 256;
+constexpr int kChunk = 4096;   // logits of one row that a block looks at, 16 per thread
+constexpr int kGroups = 64;    // of 4 threads: their maxima bound a chunk's best from below
+constexpr int kList = 256;     // candidates above that bound which are ranked side by side
+
+// Workspace: a ticket per request, 4 KiB of them | per row and chunk (max, sum of exponentials) | per row
+// and chunk beams + 1 keys (logit, index in the row), best first, 0 where there are fewer.
+struct BeamLayout {
+  int chunks;
+  size_t off_stats, off_keys, total;
+};
+inline BeamLayout beam_layout(int64_t requests, int64_t beams, int64_t vocab) {
+  BeamLayout l;
+  l.chunks = (int)((vocab + 3 + kChunk - 1) / kChunk);  // rows start up to 3 floats past 16 bytes
+  const size_t parts = (size_t)requests * beams * l.chunks;
+  l.off_stats = 4096;
+  l.off_keys = (l.off_stats + parts * sizeof(float2) + 255) & ~(size_t)255;
+  l.total = l.off_keys + parts * (beams + 1) * sizeof(unsigned long long);
+  return l;
+}
+
+struct BeamArgs {
+  const float* logits;
+  int64_t ldl;
+  const float* scores;
+  const uint8_t* done;
+  int eos, beams, vocab, chunks;
+  float* out_scores;
+  int32_t *parent, *token;
+  uint8_t* out_done;
+  unsigned* tickets;
+  float2* stats;
+  unsigned long long* keys;
+};
 
 __device__ float block_max(float v, float* red) {
 #pragma unroll
@@ -38,6 +71,7 @@ __device__ float block_max(float v, float* red) {
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = red[0];
+#pragma unroll
   for (int w = 1; w < kThreads / 32; ++w) v = fmaxf(v, red[w]);
   return v;
 }
@@ -48,61 +82,236 @@ __device__ float block_sum(float v, float* red) {
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = red[0];
+#pragma unroll
   for (int w = 1; w < kThreads / 32; ++w) v += red[w];
   return v;
 }
-
-// One block per row: log sum_t exp(logit_t) = max + log sum exp(logit - max).
-__global__ void __launch_bounds__(kThreads) row_lse_kernel(const float* logits, int64_t ldl, int vocab, float* lse) {
-  __shared__ float red[kThreads / 32];
-  const float* x = logits + blockIdx.x * ldl;
-  float m = -INFINITY;
-  for (int t = threadIdx.x; t < vocab; t += kThreads) m = fmaxf(m, logit(x[t]));
-  m = block_max(m, red);
-  float s = 0.0f;
-  for (int t = threadIdx.x; t < vocab; t += kThreads) s += expf(logit(x[t]) - m);
-  s = block_sum(s, red);
-  if (threadIdx.x == 0) lse[blockIdx.x] = m + logf(s);
+__device__ unsigned long long block_best(unsigned long long k, unsigned long long* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long x = __shfl_xor_sync(0xffffffffu, k, o);
+    k = x > k ? x : k;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = k;
+  __syncthreads();
+  k = red[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 32; ++w) k = red[w] > k ? red[w] : k;
+  return k;
 }
 
-// One block per request: `beams` times the best candidate below the last one.
-__global__ void __launch_bounds__(kThreads)
-    pick_kernel(const float* logits, int64_t ldl, const float* lse, const float* scores, const uint8_t* done,
-                int32_t eos, int beams, int vocab, float* out_scores, int32_t* parent, int32_t* token,
-                uint8_t* out_done) {
-  __shared__ unsigned long long best[kThreads];
-  const int64_t r0 = (int64_t)blockIdx.x * beams;
-  unsigned long long below = ~0ull;
-  for (int i = 0; i < beams; ++i) {
-    unsigned long long k = 0;
-    for (int w = 0; w < beams; ++w) {
-      const float* x = logits + (r0 + w) * ldl;
-      const float base = scores[r0 + w], z = lse[r0 + w];
-      const bool ended = done[r0 + w] != 0;
-      for (int t = threadIdx.x; t < vocab; t += kThreads) {
-        float s = ended ? (t == eos ? base : -INFINITY) : base + (logit(x[t]) - z);
-        if (s != s) s = -INFINITY;
-        const unsigned long long c = candidate_key(s, (uint32_t)w * vocab + t);
-        if (c < below && c > k) k = c;
-      }
+struct Shared {
+  unsigned long long list[kList];
+  unsigned long long red[kThreads / 32];
+  unsigned long long group[kGroups];
+  unsigned long long best[MTRTQ_MAX_BEAMS + 1];
+  float lse[MTRTQ_MAX_BEAMS];
+  int count, flag;
+};
+
+// The `want` largest of the block's keys (distinct, 0 = none), best first, in sh.best; 0
+// where there are fewer. each(f) calls f with every key of the calling thread, in any
+// order, any number of times over. The want-th largest of 64 groups' maxima is at most
+// the want-th largest key, so only keys from it on are ranked (some 1.2 times `want`;
+// when more than kList reach it, as with many equal logits, `want` rounds of a block-wide
+// maximum do it instead).
+template <typename Each>
+__device__ void block_top(int want, Shared& sh, Each each) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  unsigned long long k = 0;
+  each([&](unsigned long long c) { k = c > k ? c : k; });
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    const unsigned long long x = __shfl_xor_sync(0xffffffffu, k, o);
+    k = x > k ? x : k;
+  }
+  __syncthreads();
+  if ((lane & 3) == 0) sh.group[tid >> 2] = k;
+  if (tid == 0) sh.count = 0;
+  if (tid <= MTRTQ_MAX_BEAMS) sh.best[tid] = 0;
+  __syncthreads();
+  if (tid < kGroups) {
+    const unsigned long long mine = sh.group[tid];
+    int above = 0;
+#pragma unroll 8
+    for (int g = 0; g < kGroups; ++g) above += sh.group[g] > mine || (sh.group[g] == mine && g < tid);
+    if (above == want - 1) sh.red[0] = mine;
+  }
+  __syncthreads();
+  const unsigned long long bound = sh.red[0] ? sh.red[0] : 1ull;
+  each([&](unsigned long long c) {
+    if (c >= bound) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kList) sh.list[at] = c;
     }
-    best[threadIdx.x] = k;
-    __syncthreads();
-    for (int n = kThreads / 2; n > 0; n >>= 1) {
-      if (threadIdx.x < n && best[threadIdx.x + n] > best[threadIdx.x]) best[threadIdx.x] = best[threadIdx.x + n];
-      __syncthreads();
+  });
+  __syncthreads();
+  const int have = sh.count;
+  if (have <= kList) {
+    if (tid < have) {
+      const unsigned long long mine = sh.list[tid];
+      int above = 0;
+      for (int x = 0; x < have; ++x) above += sh.list[x] > mine;
+      if (above < want) sh.best[above] = mine;
     }
-    below = best[0];
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const uint32_t at = key_index(below);
-      const int w = at / vocab, t = at % vocab;
-      out_scores[r0 + i] = key_score(below);
-      parent[r0 + i] = w;
-      token[r0 + i] = t;
-      out_done[r0 + i] = done[r0 + w] != 0 || t == eos;
+  } else {
+    unsigned long long below = ~0ull;
+    for (int i = 0; i < want && below; ++i) {
+      k = 0;
+      each([&](unsigned long long c) { k = c < below && c > k ? c : k; });
+      below = block_best(k, sh.red);
+      if (tid == 0) sh.best[i] = below;
     }
   }
+  __syncthreads();
+}
+
+// Candidate (w, t)'s score, with what its row's logits are worth in all.
+__device__ __forceinline__ float row_score(float base, float x, float lse) {
+  const float s = base + (x - lse);
+  return s == s ? s : -INFINITY;
+}
+
+// One block per (chunk, row). It reads its logits once: their maximum and the sum of
+// exponentials below it, and the beams + 1 largest. The last block of a request then
+// joins the rows' sums into log-sums and ranks the rows' candidates by their scores.
+// Bound by memory: 4 bytes of each logit once (rows of beams that are done or not in use
+// are not read).
+//
+// Rounding can give two unequal logits of a row the same score, and the tie then goes to
+// the lower index, perhaps to a logit that its chunk did not pass on. That needs a score
+// of the first one left out, at most that of the last one passed on, no worse than the
+// last beam chosen: where a chunk's (beams + 1)-th does reach it, its logits are looked at
+// again (also when the candidates left are all -infinity).
+__global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ BeamArgs p) {
+  __shared__ Shared sh;
+  __shared__ float red[kThreads / 32];
+  __shared__ unsigned ticket;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int chunk = blockIdx.x, w0 = blockIdx.y, want = p.beams + 1;
+  const int64_t request = blockIdx.z, first_row = request * p.beams, row = first_row + w0;
+  const float* x = p.logits + row * p.ldl;
+  const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) >> 2);
+  const int64_t part = row * p.chunks + chunk;
+  const bool used = p.done[row] == 0 && p.scores[row] > -INFINITY;
+  if (used) {
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // 16-byte loads from the boundary before the row's first logit on
+      const int t = chunk * kChunk + (j * kThreads + tid) * 4 - shift;
+      float4 u = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (t < p.vocab && t + 3 >= 0) u = __ldcs(reinterpret_cast<const float4*>(x + t));
+      v[4 * j] = t >= 0 && t < p.vocab ? logit(u.x) : -INFINITY;
+      v[4 * j + 1] = t + 1 >= 0 && t + 1 < p.vocab ? logit(u.y) : -INFINITY;
+      v[4 * j + 2] = t + 2 >= 0 && t + 2 < p.vocab ? logit(u.z) : -INFINITY;
+      v[4 * j + 3] = t + 3 >= 0 && t + 3 < p.vocab ? logit(u.w) : -INFINITY;
+    }
+    float m = v[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) m = fmaxf(m, v[j]);
+    m = block_max(m, red);
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s += exp2f((v[j] - m) * 1.4426950408889634f);
+    s = block_sum(s, red);
+    if (tid == 0) __stcg(p.stats + part, make_float2(m, m == -INFINITY ? 0.0f : s));
+    block_top(want, sh, [&](auto f) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (v[j] > -INFINITY)
+          f(candidate_key(v[j], (uint32_t)(chunk * kChunk + ((j >> 2) * kThreads + tid) * 4 + (j & 3) - shift)));
+    });
+    if (tid < want) __stcg(p.keys + part * want + tid, sh.best[tid]);
+  }
+  __syncthreads();
+  if (tid == 0) ticket = ticket_acq_rel(p.tickets + request);
+  __syncthreads();
+  if (ticket != (unsigned)(p.beams * p.chunks - 1)) return;
+
+  // ---- the request's last block ----
+  for (int w = warp; w < p.beams; w += kThreads / 32) {
+    const int64_t r = first_row + w;
+    float lse = -INFINITY;  // of a row that passes nothing on
+    if (p.done[r] == 0 && p.scores[r] > -INFINITY) {
+      float m = -INFINITY, s = 0.0f;
+      for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, __ldcg(p.stats + r * p.chunks + c).x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int c = lane; c < p.chunks; c += 32) {
+        const float2 st = __ldcg(p.stats + r * p.chunks + c);
+        s += st.x == m ? st.y : st.y * exp2f((st.x - m) * 1.4426950408889634f);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      lse = m + logf(s);
+    }
+    if (lane == 0) sh.lse[w] = lse;
+  }
+  __syncthreads();
+  const int per_row = p.chunks * want, all = p.beams * per_row;
+  // Keys of what the chunks passed on (candidates of -infinity are left to the second look).
+  auto passed = [&](auto f) {
+    for (int e = tid; e < all; e += kThreads) {
+      const int w = e / per_row;
+      const int64_t r = first_row + w;
+      if (p.done[r] != 0 || !(p.scores[r] > -INFINITY)) continue;
+      const unsigned long long k = __ldcg(p.keys + r * per_row + (e - w * per_row));
+      if (!k) continue;
+      const float s = row_score(p.scores[r], key_score(k), sh.lse[w]);
+      if (s > -INFINITY) f(candidate_key(s, (uint32_t)w * p.vocab + key_index(k)));
+    }
+    if (tid < p.beams && p.done[first_row + tid] != 0 && p.eos >= 0 && p.scores[first_row + tid] > -INFINITY)
+      f(candidate_key(p.scores[first_row + tid], (uint32_t)tid * p.vocab + p.eos));
+  };
+  block_top(p.beams, sh, passed);
+  const unsigned long long kth = sh.best[p.beams - 1];
+  const float least = kth ? key_score(kth) : -INFINITY;
+  // Which chunks may hold more: the last one each passed on reaches the last beam.
+  auto reaches = [&](int w, int c) {
+    const int64_t r = first_row + w;
+    if (p.done[r] != 0 || !(p.scores[r] > -INFINITY)) return least == -INFINITY;
+    const unsigned long long k = __ldcg(p.keys + r * per_row + c * want + want - 1);
+    return k ? row_score(p.scores[r], key_score(k), sh.lse[w]) >= least : least == -INFINITY;
+  };
+  bool again = false;
+  for (int e = tid; e < p.beams * p.chunks; e += kThreads) again |= reaches(e / p.chunks, e % p.chunks);
+  if (__syncthreads_or(again)) {
+    unsigned long long below = ~0ull;
+    for (int i = 0; i < p.beams; ++i) {
+      unsigned long long k = 0;
+      passed([&](unsigned long long c) { k = c < below && c > k ? c : k; });
+      for (int e = 0; e < p.beams * p.chunks; ++e) {
+        const int w = e / p.chunks, c = e % p.chunks;
+        if (!reaches(w, c)) continue;
+        const int64_t r = first_row + w;
+        const float* y = p.logits + r * p.ldl;
+        const int skip = (int)((reinterpret_cast<uintptr_t>(y) & 15) >> 2);
+        const bool ended = p.done[r] != 0;
+        const int t1 = min(p.vocab, (c + 1) * kChunk - skip);
+        for (int t = max(0, c * kChunk - skip) + tid; t < t1; t += kThreads) {
+          const float s = ended ? (t == p.eos ? p.scores[r] : -INFINITY)
+                          : p.scores[r] > -INFINITY ? row_score(p.scores[r], logit(y[t]), sh.lse[w])
+                                                    : -INFINITY;
+          const unsigned long long key = candidate_key(s, (uint32_t)w * p.vocab + t);
+          k = key < below && key > k ? key : k;
+        }
+      }
+      below = block_best(k, sh.red);
+      if (tid == 0) sh.best[i] = below;
+    }
+    __syncthreads();
+  }
+  if (tid < p.beams) {
+    const uint32_t at = key_index(sh.best[tid]);
+    const int w = at / p.vocab, t = at % p.vocab;
+    p.out_scores[first_row + tid] = key_score(sh.best[tid]);
+    p.parent[first_row + tid] = w;
+    p.token[first_row + tid] = t;
+    p.out_done[first_row + tid] = p.done[first_row + w] != 0 || t == p.eos;
+  }
+  if (tid == 0) p.tickets[request] = 0u;
 }
 
 // The partly filled pages' tokens move along with their beams, in place: a thread
@@ -164,9 +373,9 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 int check_beams(int64_t requests, int64_t beams) {
-  if (requests < 1 || requests > 65535 || beams < 1 || beams > MTRTQ_MAX_BEAMS)
-    return report_error(MTRTQ_ERR_INVALID_ARG, "requests (%lld) is 1 to 65535, beams (%lld) 1 to %d",
-                        (long long)requests, (long long)beams, MTRTQ_MAX_BEAMS);
+  if (requests < 1 || requests > MTRTQ_MAX_BATCH || beams < 1 || beams > MTRTQ_MAX_BEAMS)
+    return report_error(MTRTQ_ERR_INVALID_ARG, "requests (%lld) is 1 to %d, beams (%lld) 1 to %d",
+                        (long long)requests, MTRTQ_MAX_BATCH, (long long)beams, MTRTQ_MAX_BEAMS);
   return MTRTQ_OK;
 }
 
@@ -186,7 +395,7 @@ extern "C" {
 
 int64_t mtrtq_beam_workspace_bytes(int64_t requests, int64_t beams, int64_t vocab) {
   if (check_select(requests, beams, vocab)) return -1;
-  return requests * beams * (int64_t)sizeof(float);
+  return (int64_t)beam_layout(requests, beams, vocab).total;
 }
 
 int mtrtq_beam_select(const float* logits, int64_t ldl, const float* scores, const uint8_t* done, int32_t eos,
@@ -204,11 +413,14 @@ int mtrtq_beam_select(const float* logits, int64_t ldl, const float* scores, con
   if (!workspace || (int64_t)workspace_bytes < mtrtq_beam_workspace_bytes(requests, beams, vocab))
     return report_error(MTRTQ_ERR_WORKSPACE, "workspace %zu bytes < %lld", workspace_bytes,
                         (long long)mtrtq_beam_workspace_bytes(requests, beams, vocab));
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  float* lse = static_cast<float*>(workspace);
-  row_lse_kernel<<<(unsigned)(requests * beams), kThreads, 0, st>>>(logits, ldl, (int)vocab, lse);
-  pick_kernel<<<(unsigned)requests, kThreads, 0, st>>>(logits, ldl, lse, scores, done, eos, (int)beams, (int)vocab,
-                                                       out_scores, parent, token, out_done);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 || reinterpret_cast<uintptr_t>(logits) % 4)
+    return report_error(MTRTQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned, logits 4-byte");
+  const BeamLayout l = beam_layout(requests, beams, vocab);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const BeamArgs p = {logits, ldl, scores, done, eos, (int)beams, (int)vocab, l.chunks, out_scores, parent, token,
+                      out_done, reinterpret_cast<unsigned*>(ws), reinterpret_cast<float2*>(ws + l.off_stats),
+                      reinterpret_cast<unsigned long long*>(ws + l.off_keys)};
+  beam_kernel<<<dim3(l.chunks, (unsigned)beams, (unsigned)requests), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MTRTQ_OK : report_cuda_error(e, "beam selection launch");
 }
