@@ -100,64 +100,6 @@ __global__ void cast_kernel(const __grid_constant__ Args a, __nv_bfloat16* rows)
   }
 }
 
-// One warp per (row, head), lanes over the dimensions: the running maximum m, sum l
-// and output o of a softmax over the keys in order.
-template <typename TX, typename TC, bool PAGED>
-__global__ void __launch_bounds__(32) rows_kernel(const __grid_constant__ Args a) {
-  const int64_t r = blockIdx.x;
-  const int h = blockIdx.y, lane = threadIdx.x;
-  const int64_t b = request_of(a, r);
-  if (b < 0) return;
-  int64_t r0, r1;
-  request_rows(a, b, r0, r1);
-  const int g = h / (a.heads / a.kv_heads);
-  int64_t last = PAGED ? (int64_t)a.kv_len[b] - (r1 - r0) + (r - r0) : r - r0;
-  if (PAGED && last >= a.table_width * a.page_size) last = a.table_width * a.page_size - 1;
-  float q[4], o[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int d = c * 32 + lane;
-    q[c] = d < a.head_dim ? to_f32(static_cast<const TX*>(a.q)[r * a.q_row + h * a.q_head + d]) * a.scale : 0.0f;
-    o[c] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t j = 0; j <= last; ++j) {
-    const int64_t at = PAGED ? page_offset(a, b, j, g) : 0;
-    float s = 0.0f, v[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int d = c * 32 + lane;
-      float k = 0.0f;
-      v[c] = 0.0f;
-      if (d < a.head_dim && at >= 0) {
-        if (PAGED) {
-          k = to_f32(static_cast<const TC*>(a.k_pages)[at + d]);
-          v[c] = to_f32(static_cast<const TC*>(a.v_pages)[at + d]);
-        } else {
-          k = to_f32(from_f32<TC>(to_f32(static_cast<const TX*>(a.k)[(r0 + j) * a.k_row + g * a.k_head + d])));
-          v[c] = to_f32(from_f32<TC>(to_f32(static_cast<const TX*>(a.v)[(r0 + j) * a.v_row + g * a.v_head + d])));
-        }
-      }
-      s += q[c] * k;
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float top = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.0f : expf(m - top), p = top == -INFINITY ? 0.0f : expf(s - top);
-    m = top;
-    l = l * keep + p;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] = o[c] * keep + p * v[c];
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int d = c * 32 + lane;
-    if (d < a.head_dim)
-      static_cast<TC*>(a.out)[r * a.out_row + h * a.out_head + d] = from_f32<TC>(l == 0.0f ? 0.0f : o[c] * inv);
-  }
-}
-
 bool on16(const void* p, int64_t s0, int64_t s1, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s0 * size % 16 == 0 && s1 * size % 16 == 0;
 }
@@ -271,6 +213,20 @@ int sm_count() {
   return n;
 }
 
+void fill_list(const Args& a, bool paged, AttentionList& p) {
+  p.cu_rows = a.cu_rows;
+  p.kv_len = paged ? a.kv_len : nullptr;
+  p.table = paged ? a.table : nullptr;
+  p.table_ld = a.table_ld;
+  p.rows = a.rows;
+  p.batch = (int)a.batch;
+  p.kv_heads = a.kv_heads;
+  p.group = a.heads / a.kv_heads;
+  p.head_dim = a.head_dim;
+  p.page_size = a.page_size;
+  p.max_keys = a.table_width * a.page_size;
+}
+
 int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cudaStream_t st) {
   const TcLayout l = tc_layout(a, sm_count());
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -320,18 +276,9 @@ int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cuda
     if (rc) return rc;
   }
   TcAttention p = {};
-  p.cu_rows = a.cu_rows;
-  p.kv_len = paged ? a.kv_len : nullptr;
-  p.table = paged ? a.table : nullptr;
-  p.table_ld = a.table_ld;
-  p.rows = a.rows;
-  p.batch = (int)a.batch;
-  p.kv_heads = a.kv_heads;
-  p.group = group;
-  p.head_dim = a.head_dim;
-  p.page_size = a.page_size;
+  fill_list(a, paged, p);
   p.slot_tokens = l.slot_tokens;
-  p.max_keys = a.table_width * a.page_size;
+  p.tile_tokens = 2 * l.slot_tokens;
   p.min_steps = 2;
   p.scale = a.scale;
   p.out = static_cast<__nv_bfloat16*>(a.out);
@@ -348,14 +295,58 @@ int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cuda
   return cuda_status(launch_attention_tc(p, qm, km, vm, l.grid, before, st), "attention launch");
 }
 
-int launch_f32(const Args& a, bool paged, cudaStream_t st) {
-  if (paged) {
-    if (a.k) append_kernel<float, float><<<(unsigned)a.rows, 128, 0, st>>>(a, nullptr);
-    rows_kernel<float, float, true><<<dim3((unsigned)a.rows, a.heads), 32, 0, st>>>(a);
-  } else {
-    rows_kernel<float, float, false><<<dim3((unsigned)a.rows, a.heads), 32, 0, st>>>(a);
+// The f32 path: tickets | partials of cut tiles. Tiles of 16 rows where requests have few
+// rows each, of 64 and 128 for longer ones (a tile holds whole groups of heads).
+struct F32Layout {
+  int grid, tile_rows;
+  size_t off_ml, off_part, total;
+};
+
+F32Layout f32_layout(const Args& a, int sm_count) {
+  F32Layout l;
+  const int group = a.heads / a.kv_heads, dp = a.head_dim <= 64 ? 64 : 128;
+  const int64_t each = a.rows * group / a.batch;  // rows of a request's tiles, on average
+  l.tile_rows = each <= 16 && group <= 16 ? 16 : each <= 256 && group <= 64 ? 64 : 128;
+  const int ctas = dp == 64 || l.tile_rows == 16 ? 2 : 1;
+  l.grid = sm_count * ctas < 1024 ? sm_count * ctas : 1024;
+  l.off_ml = 4096;
+  l.off_part = l.off_ml + round256((size_t)l.grid * 2 * l.tile_rows * sizeof(float2));
+  l.total = l.off_part + (size_t)l.grid * 2 * l.tile_rows * dp * sizeof(float);
+  return l;
+}
+
+int launch_f32(const Args& a, bool paged, void* workspace, cudaStream_t st) {
+  const F32Layout l = f32_layout(a, sm_count());
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const bool before = paged && a.k;
+  if (before) {
+    append_kernel<float, float><<<(unsigned)a.rows, 256, 0, st>>>(a, nullptr);
+    if (int rc = cuda_status(cudaGetLastError(), "attention rows launch")) return rc;
   }
-  return cuda_status(cudaGetLastError(), "attention launch");
+  F32Attention p = {};
+  fill_list(a, paged, p);
+  p.slot_tokens = 0;
+  p.tile_tokens = l.tile_rows / p.group;
+  p.min_steps = 2;
+  p.scale = a.scale;
+  p.q = static_cast<const float*>(a.q);
+  p.k = static_cast<const float*>(paged ? a.k_pages : a.k);
+  p.v = static_cast<const float*>(paged ? a.v_pages : a.v);
+  p.q_row = a.q_row;
+  p.q_head = a.q_head;
+  p.k_row = paged ? a.page_stride : a.k_row;
+  p.k_head = a.k_head;
+  p.v_row = paged ? a.page_stride : a.v_row;
+  p.v_head = a.v_head;
+  p.num_pages = a.num_pages;
+  p.out = static_cast<float*>(a.out);
+  p.out_row = a.out_row;
+  p.out_head = a.out_head;
+  p.counters = reinterpret_cast<unsigned*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + l.off_ml);
+  p.partials = reinterpret_cast<float*>(ws + l.off_part);
+  p.tile_rows = l.tile_rows;
+  return cuda_status(launch_attention_f32(p, l.grid, before, st), "attention launch");
 }
 
 int attention(const Args* a, bool paged, void* workspace, size_t workspace_bytes, void* stream) {
@@ -370,7 +361,7 @@ int attention(const Args* a, bool paged, void* workspace, size_t workspace_bytes
   if (reinterpret_cast<uintptr_t>(workspace) % 256)
     return report_error(MTRTQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == MTRTQ_DTYPE_F32) return launch_f32(*a, paged, st);
+  if (a->dtype == MTRTQ_DTYPE_F32) return launch_f32(*a, paged, workspace, st);
   return launch_tc(*a, paged, workspace, status, st);
 }
 
@@ -383,7 +374,7 @@ extern "C" {
 
 int64_t mtrtq_attention_workspace_bytes(const mtrtq_attention_args* a) {
   if (check_args(a, a && a->k_pages)) return -1;
-  return a->dtype == MTRTQ_DTYPE_F32 ? 4096 : (int64_t)tc_layout(*a, sm_count()).total;
+  return (int64_t)(a->dtype == MTRTQ_DTYPE_F32 ? f32_layout(*a, sm_count()).total : tc_layout(*a, sm_count()).total);
 }
 
 int mtrtq_prompt_attention(const mtrtq_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {

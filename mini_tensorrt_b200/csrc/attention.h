@@ -9,16 +9,21 @@
 
 namespace mtrtq {
 
-struct TcAttention {
+// What a call's list of steps (attention_sched.cuh) is made from.
+struct AttentionList {
   const int32_t* cu_rows;
   const int32_t* kv_len;  // paged only, like table
   const int32_t* table;
   int64_t table_ld;
   int64_t rows;
   int batch, kv_heads, group, head_dim, page_size;
-  int slot_tokens;   // 128 / group: tokens in a tile slot's 128 rows
-  int64_t max_keys;  // paged: tokens the table's columns hold
-  int64_t min_steps; // fewest steps worth a CTA
+  int slot_tokens;    // tensor cores: 128 / group, the tokens in a slot's 128 rows
+  int tile_tokens;
+  int64_t max_keys;   // paged: tokens the table's columns hold
+  int64_t min_steps;  // fewest steps worth a CTA
+};
+
+struct TcAttention : AttentionList {
   float scale;
   __nv_bfloat16* out;
   int64_t out_row, out_head;
@@ -30,6 +35,22 @@ struct TcAttention {
   int part_rows;           // rows a tile can have, at most 256
   unsigned* status;
 };
+
+// fp32 throughout, on the CUDA cores (attention_f32.cu): tiles of 16, 64 or 128 rows.
+struct F32Attention : AttentionList {
+  float scale;
+  const float *q, *k, *v;  // paged: k and v are the pages, k_row and v_row the page stride
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  float* out;
+  int64_t out_row, out_head;
+  unsigned* counters;  // [grid] tickets, zero
+  int64_t num_pages;
+  float* partials;     // [grid][2][tile_rows][head_dim rounded to 64 or 128]
+  float2* part_ml;     // [grid][2][tile_rows]
+  int tile_rows;
+};
+
+cudaError_t launch_attention_f32(const F32Attention& p, int grid, bool pdl, cudaStream_t st);
 
 cudaError_t launch_attention_tc(const TcAttention& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                                 int grid, bool pdl, cudaStream_t st);

@@ -1,0 +1,360 @@
+// Attention with every product and sum in fp32, on the CUDA cores: packed prompts and new
+// tokens over a paged cache whose rows and pages are f32.
+//
+// The same online softmax as on the tensor cores (attention_tc.cu), over blocks of 64 keys:
+// a CTA of 256 threads holds a tile of 16 RM rows (tokens times the group's heads), thread
+// (ty, tx) the rows ty RM .. and the keys 4 tx .. of the scores, then the same rows and
+// dimensions 4 tx .. of the output. Q and K lie transposed in shared memory, so that one
+// dimension's step is RM + 4 values read for 4 RM products (packed two at a time), and P
+// transposed for the same reason. Bound by the fp32 units for tiles of many rows: one
+// product of each score and output element per lane and clock.
+//
+// V rows past the request's keys are read as zeros; where a block not seen whole by every
+// row holds an infinity or a NaN, its products are formed only for the rows that see them.
+#include <math.h>
+
+#include "../../include/mtrtq.h"
+#include "attention_sched.cuh"
+#include "q8_common.cuh"
+
+namespace mtrtq {
+
+namespace {
+
+constexpr int kKeys = 64;
+constexpr int kThreads = 256;
+
+template <int HD, int RM>
+struct Cfg {
+  static constexpr int BM = 16 * RM;
+  static constexpr int QS = BM + 4;    // row strides, in floats
+  static constexpr int KS = kKeys + 4;
+  static constexpr int OFF_Q = 0;                       // [HD][QS]
+  static constexpr int OFF_K = OFF_Q + HD * QS;         // [HD][KS]
+  static constexpr int OFF_V = OFF_K + HD * KS;         // [kKeys][HD]
+  static constexpr int OFF_P = OFF_V + kKeys * HD;      // [kKeys][QS]
+  static constexpr int FLOATS = OFF_P + kKeys * QS;
+  static constexpr int BYTES = FLOATS * 4 + (MTRTQ_MAX_BATCH + 1) * 8;
+  static constexpr int CTAS = BYTES <= 112 * 1024 ? 2 : 1;
+  static_assert(BYTES <= 226 * 1024 && FLOATS % 2 == 0, "shared memory per CTA");
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ bool broken(float x) { return !(fabsf(x) < INFINITY); }
+
+template <int HD, int RM, bool PAGED>
+__global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
+    attention_f32_kernel(const __grid_constant__ F32Attention p) {
+  using C = Cfg<HD, RM>;
+  constexpr int RP = RM == 1 ? 1 : RM / 2;  // row pairs of a thread
+  constexpr int NC = HD / 64;               // groups of four output columns of a thread
+  extern __shared__ float4 raw4[];
+  float* sm = reinterpret_cast<float*>(raw4);
+  float *qs = sm + C::OFF_Q, *ks = sm + C::OFF_K, *vs = sm + C::OFF_V, *ps = sm + C::OFF_P;
+  int64_t* prefix = reinterpret_cast<int64_t*>(sm + C::FLOATS);
+  __shared__ int start[4];
+  __shared__ unsigned ticket;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, lane = tid & 31, warp = tid >> 5;
+
+  int64_t per;
+  Walk<kKeys> walk = find_run<kKeys, kThreads>(p, prefix, start, per);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const float c2 = p.scale * 1.4426950408889634f;  // scale log2 e
+
+  Segment s;
+  while (walk.next(p, s)) {
+    // Q, transposed; rows past the tile's tokens and dimensions past the head's are zero.
+    __syncthreads();
+    for (int e = tid; e < C::BM * (HD / 4); e += kThreads) {
+      const int row = e % C::BM, d = e / C::BM * 4;
+      const int token = row / p.group, head = row - token * p.group;
+      float4 x = make_float4(0, 0, 0, 0);
+      if (token < s.tile.tokens && d < p.head_dim)
+        x = *reinterpret_cast<const float4*>(p.q + (s.q.r0 + s.tile.t0 + token) * p.q_row +
+                                             (int64_t)(s.h * p.group + head) * p.q_head + d);
+      qs[d * C::QS + row] = x.x;
+      qs[(d + 1) * C::QS + row] = x.y;
+      qs[(d + 2) * C::QS + row] = x.z;
+      qs[(d + 3) * C::QS + row] = x.w;
+    }
+    float m[RM], l[RM], o[RM][4 * NC];
+    int sees[RM];  // keys the row sees
+    int least = 0x7fffffff;
+#pragma unroll
+    for (int r = 0; r < RM; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 4 * NC; ++c) o[r][c] = 0.0f;
+      const int token = (ty * RM + r) / p.group;
+      const int64_t n = s.q.ctx + s.tile.t0 + token + 1;
+      sees[r] = token < s.tile.tokens ? (int)max((int64_t)0, min(n, (int64_t)s.q.keys)) : 0;
+      if (token < s.tile.tokens) least = min(least, sees[r]);
+    }
+    const int64_t first_sees = s.q.ctx + s.tile.t0 + 1;
+    const int64_t all_see = first_sees < s.q.keys ? first_sees : s.q.keys;
+
+    for (int j = s.j0; j < s.j1; ++j) {
+      const int key0 = j * kKeys;
+      __syncthreads();
+      // K transposed: a lane per key; V as it is. Tokens past the keys, and pages out of
+      // range, read as zeros.
+      bool odd = false;
+      {
+        const int key = key0 + (warp & 1) * 32 + lane;
+        const float* src = nullptr;
+        if (key < s.q.keys) {
+          if (PAGED) {
+            const int64_t page = p.table[s.b * p.table_ld + key / p.page_size];
+            if (page >= 0 && page < p.num_pages)
+              src = p.k + page * p.k_row + ((int64_t)s.h * p.page_size + key % p.page_size) * p.head_dim;
+          } else {
+            src = p.k + (s.q.r0 + key) * p.k_row + s.h * p.k_head;
+          }
+        }
+        float* dst = ks + (warp & 1) * 32 + lane;
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+          const int d = (warp >> 1) * (HD / 4) + c * 4;
+          const float4 x = src && d < p.head_dim ? *reinterpret_cast<const float4*>(src + d) : make_float4(0, 0, 0, 0);
+          dst[d * C::KS] = x.x;
+          dst[(d + 1) * C::KS] = x.y;
+          dst[(d + 2) * C::KS] = x.z;
+          dst[(d + 3) * C::KS] = x.w;
+        }
+#pragma unroll
+        for (int c = 0; c < kKeys * HD / 4 / kThreads; ++c) {
+          const int e = c * kThreads + tid, r = e / (HD / 4), d = e % (HD / 4) * 4, at = key0 + r;
+          float4 x = make_float4(0, 0, 0, 0);
+          if (at < s.q.keys && d < p.head_dim) {
+            if (PAGED) {
+              const int64_t page = p.table[s.b * p.table_ld + at / p.page_size];
+              if (page >= 0 && page < p.num_pages)
+                x = *reinterpret_cast<const float4*>(
+                    p.v + page * p.v_row + ((int64_t)s.h * p.page_size + at % p.page_size) * p.head_dim + d);
+            } else {
+              x = *reinterpret_cast<const float4*>(p.v + (s.q.r0 + at) * p.v_row + s.h * p.v_head + d);
+            }
+          }
+          odd |= broken(x.x) | broken(x.y) | broken(x.z) | broken(x.w);
+          *reinterpret_cast<float4*>(vs + r * HD + d) = x;
+        }
+      }
+      const bool partly = (int64_t)key0 + kKeys > all_see;
+      const bool careful = __syncthreads_or(odd) && partly;
+
+      // S: rows in pairs, four keys
+      float2 a[RP][4];
+#pragma unroll
+      for (int r = 0; r < RP; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) a[r][c] = make_float2(0, 0);
+#pragma unroll 8
+      for (int d = 0; d < HD; ++d) {
+        const float4 k4 = *reinterpret_cast<const float4*>(ks + d * C::KS + 4 * tx);
+        const float kk[4] = {k4.x, k4.y, k4.z, k4.w};
+        if (RM == 1) {
+          const float q = qs[d * C::QS + ty];
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            const float2 t = fma2(make_float2(q, q), make_float2(kk[c], kk[c + 1]), make_float2(a[0][c].x, a[0][c + 1].x));
+            a[0][c].x = t.x;
+            a[0][c + 1].x = t.y;
+          }
+        } else {
+          float q[RM];
+#pragma unroll
+          for (int r = 0; r < RM; r += 4)
+            *reinterpret_cast<float4*>(q + r) = *reinterpret_cast<const float4*>(qs + d * C::QS + ty * RM + r);
+#pragma unroll
+          for (int r = 0; r < RP; ++r)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              a[r][c] = fma2(make_float2(q[2 * r], q[2 * r + 1]), make_float2(kk[c], kk[c]), a[r][c]);
+        }
+      }
+      // softmax: a row's 64 scores lie in the 16 lanes of one ty
+      float pr[RM][4];
+#pragma unroll
+      for (int r = 0; r < RM; ++r) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          pr[r][c] = (r & 1) ? a[r >> 1][c].y : a[r >> 1][c].x;
+          if (partly && key0 + 4 * tx + c >= sees[r]) pr[r][c] = -INFINITY;
+          top = fmaxf(top, pr[r][c]);
+        }
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        top *= c2;
+        const float now = fmaxf(m[r], top);
+        const float base = now == -INFINITY ? 0.0f : now;
+        const float keep = m[r] == -INFINITY ? 1.0f : ex2(m[r] - base);
+        m[r] = now;
+        float sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          pr[r][c] = ex2(fmaf(pr[r][c], c2, -base));
+          sum += pr[r][c];
+        }
+        l[r] = l[r] * keep + sum;  // this lane's share
+#pragma unroll
+        for (int c = 0; c < 4 * NC; ++c) o[r][c] *= keep;
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float* dst = ps + (4 * tx + c) * C::QS + ty * RM;
+        if (RM == 1) {
+          dst[0] = pr[0][c];
+        } else {
+#pragma unroll
+          for (int r = 0; r + 3 < RM; r += 4)
+            *reinterpret_cast<float4*>(dst + r) = make_float4(pr[r][c], pr[r + 1][c], pr[r + 2][c], pr[r + 3][c]);
+        }
+      }
+      __syncwarp();  // a row's weights are written and read by the same half warp
+      if (!careful) {
+#pragma unroll 4
+        for (int y = 0; y < kKeys; ++y) {
+          float w[RM];
+          if (RM == 1) {
+            w[0] = ps[y * C::QS + ty];
+          } else {
+#pragma unroll
+            for (int r = 0; r + 3 < RM; r += 4)
+              *reinterpret_cast<float4*>(w + r) = *reinterpret_cast<const float4*>(ps + y * C::QS + ty * RM + r);
+          }
+#pragma unroll
+          for (int g = 0; g < NC; ++g) {
+            const float4 v = *reinterpret_cast<const float4*>(vs + y * HD + g * 64 + 4 * tx);
+#pragma unroll
+            for (int r = 0; r < RM; ++r) {
+              float2 t0 = fma2(make_float2(w[r], w[r]), make_float2(v.x, v.y), make_float2(o[r][4 * g], o[r][4 * g + 1]));
+              float2 t1 =
+                  fma2(make_float2(w[r], w[r]), make_float2(v.z, v.w), make_float2(o[r][4 * g + 2], o[r][4 * g + 3]));
+              o[r][4 * g] = t0.x;
+              o[r][4 * g + 1] = t0.y;
+              o[r][4 * g + 2] = t1.x;
+              o[r][4 * g + 3] = t1.y;
+            }
+          }
+        }
+      } else {
+        for (int y = 0; y < kKeys; ++y) {
+#pragma unroll
+          for (int r = 0; r < RM; ++r) {
+            if (key0 + y >= sees[r]) continue;
+            const float w = ps[y * C::QS + ty * RM + r];
+#pragma unroll
+            for (int c = 0; c < 4 * NC; ++c) o[r][c] = fmaf(w, vs[y * HD + (c >> 2) * 64 + 4 * tx + (c & 3)], o[r][c]);
+          }
+        }
+      }
+    }
+
+#pragma unroll
+    for (int r = 0; r < RM; ++r) {
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+      if (m[r] == -INFINITY && l[r] != l[r]) m[r] = 0.0f;  // every score it saw was NaN
+    }
+    const bool whole = s.whole();
+    const int64_t part = (int64_t)blockIdx.x * 2 + (s.j0 > 0 ? 0 : 1);
+#pragma unroll
+    for (int r = 0; r < RM; ++r) {
+      const int row = ty * RM + r, token = row / p.group, head = row - token * p.group;
+      if (token >= s.tile.tokens) continue;
+      if (whole) {
+        const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+        float* dst = p.out + (s.q.r0 + s.tile.t0 + token) * p.out_row + (int64_t)(s.h * p.group + head) * p.out_head;
+#pragma unroll
+        for (int g = 0; g < NC; ++g) {
+          const int d = g * 64 + 4 * tx;
+          if (d < p.head_dim)
+            *reinterpret_cast<float4*>(dst + d) = make_float4(o[r][4 * g] * inv, o[r][4 * g + 1] * inv,
+                                                              o[r][4 * g + 2] * inv, o[r][4 * g + 3] * inv);
+        }
+      } else {
+        float* dst = p.partials + (part * C::BM + row) * HD;
+#pragma unroll
+        for (int g = 0; g < NC; ++g)
+          __stcg(reinterpret_cast<float4*>(dst + g * 64 + 4 * tx),
+                 make_float4(o[r][4 * g], o[r][4 * g + 1], o[r][4 * g + 2], o[r][4 * g + 3]));
+        if (tx == 0) __stcg(p.part_ml + part * C::BM + row, make_float2(m[r], l[r]));
+      }
+    }
+    if (!whole) {
+      // the CTA that finishes a cut tile last joins its parts in order
+      const int64_t c_first = s.first / per, c_last = (s.first + s.tile.steps - 1) / per;
+      __syncthreads();
+      if (tid == 0) ticket = ticket_acq_rel(p.counters + c_first);
+      __syncthreads();
+      if (ticket == (unsigned)(c_last - c_first)) {
+        const int rows = s.tile.tokens * p.group, vecs = p.head_dim / 4;
+        for (int e = tid; e < rows * vecs; e += kThreads) {
+          const int row = e / vecs, d = e % vecs * 4, token = row / p.group, head = row - token * p.group;
+          float top = -INFINITY;
+          for (int64_t c = c_first; c <= c_last; ++c)
+            top = fmaxf(top, __ldcg(p.part_ml + (c * 2 + (c == c_first ? 1 : 0)) * C::BM + row).x);
+          float sum = 0.0f;
+          float4 x = make_float4(0, 0, 0, 0);
+          for (int64_t c = c_first; c <= c_last; ++c) {
+            const int64_t at = (c * 2 + (c == c_first ? 1 : 0)) * C::BM + row;
+            const float2 ml = __ldcg(p.part_ml + at);
+            if (ml.x == -INFINITY) continue;
+            const float w = top == INFINITY ? 1.0f : ex2(ml.x - top);
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(p.partials + at * HD + d));
+            sum += ml.y * w;
+            x.x += y.x * w;
+            x.y += y.y * w;
+            x.z += y.z * w;
+            x.w += y.w * w;
+          }
+          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+          *reinterpret_cast<float4*>(p.out + (s.q.r0 + s.tile.t0 + token) * p.out_row +
+                                     (int64_t)(s.h * p.group + head) * p.out_head + d) =
+              make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        }
+        if (tid == 0) p.counters[c_first] = 0u;
+      }
+    }
+  }
+}
+
+template <int HD, int RM, bool PAGED>
+cudaError_t launch_one(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
+  auto kernel = attention_f32_kernel<HD, RM, PAGED>;
+  if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kernel), Cfg<HD, RM>::BYTES)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<HD, RM>::BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int HD, bool PAGED>
+cudaError_t launch_rows(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
+  if (p.tile_rows == 16) return launch_one<HD, 1, PAGED>(p, grid, pdl, st);
+  if (p.tile_rows == 64) return launch_one<HD, 4, PAGED>(p, grid, pdl, st);
+  return launch_one<HD, 8, PAGED>(p, grid, pdl, st);
+}
+
+}  // namespace
+
+cudaError_t launch_attention_f32(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
+  if (p.head_dim <= 64)
+    return p.table ? launch_rows<64, true>(p, grid, pdl, st) : launch_rows<64, false>(p, grid, pdl, st);
+  return p.table ? launch_rows<128, true>(p, grid, pdl, st) : launch_rows<128, false>(p, grid, pdl, st);
+}
+
+}  // namespace mtrtq

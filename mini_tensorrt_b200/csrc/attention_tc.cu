@@ -28,7 +28,7 @@
 #include <math.h>
 
 #include "../../include/mtrtq.h"
-#include "attention.h"
+#include "attention_sched.cuh"
 #include "q8_common.cuh"
 
 namespace mtrtq {
@@ -117,95 +117,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-
-// ---- the list of steps -----------------------------------------------------------
-
-struct Request {
-  int64_t r0;
-  int m;        // rows
-  int64_t ctx;  // position of row 0 (negative: rows before the first position see nothing)
-  int keys;     // keys it has
-};
-
-struct Tile {
-  int t0, tokens;  // its tokens, of the request's rows
-  bool pair;
-  int blocks, steps;
-};
-
-struct Segment {
-  Request q;
-  Tile tile;
-  int b, h;
-  int j0, j1;     // its steps of the tile's
-  int64_t first;  // the tile's first step in the list
-  __device__ bool whole() const { return j0 == 0 && j1 == tile.steps; }
-};
-
-__device__ __forceinline__ Request load_request(const TcAttention& p, int b) {
-  Request q;
-  const int64_t lo = p.cu_rows[b], hi = p.cu_rows[b + 1];
-  q.r0 = lo < 0 ? 0 : lo > p.rows ? p.rows : lo;
-  q.m = (int)((hi < q.r0 ? q.r0 : hi > p.rows ? p.rows : hi) - q.r0);
-  if (p.table) {
-    const int64_t n = p.kv_len[b];
-    q.ctx = n - q.m;
-    q.keys = (int)(n < 0 ? 0 : n < p.max_keys ? n : p.max_keys);
-  } else {
-    q.ctx = 0;
-    q.keys = q.m;
-  }
-  return q;
-}
-
-__device__ __forceinline__ Tile make_tile(const TcAttention& p, const Request& q, int i) {
-  Tile t;
-  t.t0 = i * 2 * p.slot_tokens;
-  t.tokens = min(2 * p.slot_tokens, q.m - t.t0);
-  t.pair = t.tokens > p.slot_tokens;
-  const int64_t seen = q.ctx + t.t0 + t.tokens;
-  const int keys = (int)(seen < q.keys ? seen : q.keys);
-  t.blocks = keys <= 0 ? 1 : (keys + kBlock - 1) / kBlock;
-  t.steps = t.pair ? t.blocks : (t.blocks + 1) >> 1;
-  return t;
-}
-
-__device__ __forceinline__ int tile_count(const TcAttention& p, const Request& q) {
-  return (q.m + 2 * p.slot_tokens - 1) / (2 * p.slot_tokens);
-}
-
-struct Walk {
-  int64_t u, end;
-  int b, h, i, j;
-  Request q;
-
-  __device__ bool next(const TcAttention& p, Segment& s) {
-    if (u >= end) return false;
-    s.q = q;
-    s.tile = make_tile(p, q, i);
-    s.b = b;
-    s.h = h;
-    s.j0 = j;
-    s.first = u - j;
-    const int64_t take = min((int64_t)(s.tile.steps - j), end - u);
-    s.j1 = j + (int)take;
-    u += take;
-    j = s.j1;
-    if (j == s.tile.steps) {
-      j = 0;
-      if (++i == tile_count(p, q)) {
-        i = 0;
-        if (++h == p.kv_heads) {
-          h = 0;
-          if (u < end) {
-            do q = load_request(p, ++b); while (q.m == 0);
-          }
-        }
-      }
-    }
-    return true;
-  }
-};
 
 // K and V blocks of a segment in the order the products need them: `at` 0 .. 2 n - 1
 // for n blocks.
@@ -308,88 +219,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
-  // Steps of each request, then their running total.
-  for (int b = warp; b < p.batch; b += kThreads / 32) {
-    const Request q = load_request(p, b);
-    const int n = tile_count(p, q);
-    int64_t sum = 0;
-    for (int i = lane; i < n; i += 32) sum += make_tile(p, q, i).steps;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) prefix[b + 1] = sum;
-  }
-  if (tid == 0) prefix[0] = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = misc[0];
-  if (warp == 0) {
-    int64_t run = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      int64_t v = b0 + lane < p.batch ? prefix[b0 + lane + 1] * p.kv_heads : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += w;
-      }
-      if (b0 + lane < p.batch) prefix[b0 + lane + 1] = run + v;
-      run += __shfl_sync(0xffffffffu, v, 31);
-    }
-  }
-  __syncthreads();
-  const int64_t total = prefix[p.batch];
-  int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < p.min_steps) per = p.min_steps;
-  Walk walk0;
-  walk0.u = min(total, per * blockIdx.x);
-  walk0.end = min(total, walk0.u + per);
-  if (warp == 0 && walk0.u < walk0.end) {
-    int lo = 0, hi = p.batch - 1;  // the last request whose first step is not after u
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] <= walk0.u) lo = mid; else hi = mid - 1;
-    }
-    const Request q = load_request(p, lo);
-    const int64_t each = (prefix[lo + 1] - prefix[lo]) / p.kv_heads;
-    int64_t left = walk0.u - prefix[lo];
-    const int h = (int)(left / each);
-    left -= h * each;
-    const int n = tile_count(p, q);
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      int64_t v = i0 + lane < n ? make_tile(p, q, i0 + lane).steps : 0;
-      const int64_t mine = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += w;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, v > left);
-      if (past) {
-        if (lane == __ffs(past) - 1) {
-          s_start[0] = lo;
-          s_start[1] = h;
-          s_start[2] = i0 + lane;
-          s_start[3] = (int)(left - (v - mine));
-        }
-        break;
-      }
-      left -= __shfl_sync(0xffffffffu, v, 31);
-    }
-  }
-  __syncthreads();
-  if (walk0.u < walk0.end) {
-    walk0.b = s_start[0];
-    walk0.h = s_start[1];
-    walk0.i = s_start[2];
-    walk0.j = s_start[3];
-    walk0.q = load_request(p, walk0.b);
-  }
+  int64_t per;
+  const Walk<kBlock> walk0 = find_run<kBlock, kThreads>(p, prefix, s_start, per);
   // The kernel that stored the new keys and cast the rows is complete from here on.
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int ksteps = (p.head_dim + 15) / 16;
   Segment s;
-  Walk walk = walk0;
+  Walk<kBlock> walk = walk0;
 
   // 256 threads of 200 registers and 128 of 104: the 384 x 168 of the launch.
   if (warp < 8) {

@@ -15,79 +15,100 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .matmulq import Workspace, _stream_ptr
+from .matmulq import Workspace
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 _workspaces: dict = {}
 
 
+def _stream_ptr(stream, index: int) -> int:
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(index)
+    return stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
+
+
+def _call(where: str, index: int, *args) -> None:
+    """Calls the library with that device current. (These calls are a few microseconds of
+    host time, so the device is only switched where it has to be.)"""
+    fn = getattr(lib(), where)
+    if torch.cuda.current_device() == index:
+        check(fn(*args), where)
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args), where)
+
+
 def _workspace(workspace, device, stream_ptr: int, nbytes: int):
-    """The caller's workspace (a Workspace, or a tensor), or one kept for each stream:
-    calls that share a workspace must be ordered."""
-    if isinstance(workspace, torch.Tensor):
-        return workspace
+    """(address, bytes) of the caller's workspace (a Workspace, or a tensor), or of one
+    kept for each stream: calls that share a workspace must be ordered."""
     if workspace is None:
         key = (device.index, stream_ptr)
         workspace = _workspaces.get(key)
         if workspace is None:
             workspace = _workspaces[key] = Workspace(device)
-    return workspace.get(nbytes)
+    if isinstance(workspace, Workspace):
+        workspace = workspace.get(nbytes)
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-def _rows(name: str, x: torch.Tensor, heads: int | None, dim: int | None, rows: int | None, dtype=None):
-    if x.dim() != 3 or x.dtype not in _DTYPES or not x.is_cuda:
-        raise ValueError(f"{name} must be a float32 or bfloat16 CUDA tensor [rows, heads, head_dim]")
-    if x.stride(2) != 1 and x.shape[2] > 1:
+def _rows(name: str, x: torch.Tensor, shape, dtype, device):
+    """Checks rows of heads; returns their strides."""
+    if x.shape != shape or x.dtype != dtype or x.device != device:
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on {device}, got {x.dtype} {list(x.shape)} on {x.device}")
+    s = x.stride()
+    if s[2] != 1 and shape[2] > 1:
         raise ValueError(f"{name} must have unit stride along head_dim")
-    want = (x.shape[0] if rows is None else rows, x.shape[1] if heads is None else heads,
-            x.shape[2] if dim is None else dim)
-    if tuple(x.shape) != want or (dtype is not None and x.dtype != dtype):
-        raise ValueError(f"{name} must be {dtype or 'float32 or bfloat16'} {list(want)}, got {x.dtype} {list(x.shape)}")
+    return s
 
 
 def _ints(name: str, x: torch.Tensor, shape, device):
-    if x.dtype != torch.int32 or x.device != device or tuple(x.shape) != tuple(shape):
+    if x.dtype != torch.int32 or x.device != device or x.shape != shape:
         raise ValueError(f"{name} must be int32 {list(shape)} on {device}, got {x.dtype} {list(x.shape)} on {x.device}")
-    if x.shape and x.shape[-1] > 1 and x.stride(-1) != 1:
+    s = x.stride()
+    if s[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name} must have unit stride along its last dimension")
+    return s
 
 
-def _out(out, q, dtype, stream):
+def _attend(where, q, k, v, out, out_dtype, kv_heads, cu_rows, scale, workspace, stream, pages=None):
+    dtype, device = q.dtype, q.device
+    if q.dim() != 3 or dtype not in _DTYPES or device.type != "cuda":
+        raise ValueError("q must be a float32 or bfloat16 CUDA tensor [rows, heads, head_dim]")
+    shape = q.shape
+    T, H, D = shape
+    a = _lib.AttentionArgs()
+    s = _rows("q", q, shape, dtype, device)
+    a.q, a.q_row, a.q_head = q.data_ptr(), s[0], s[1]
+    if k is not None:
+        s = _rows("k", k, (T, kv_heads, D), dtype, device)
+        a.k, a.k_row, a.k_head = k.data_ptr(), s[0], s[1]
+        s = _rows("v", v, (T, kv_heads, D), dtype, device)
+        a.v, a.v_row, a.v_head = v.data_ptr(), s[0], s[1]
+    if out_dtype not in _DTYPES:
+        raise ValueError("the result is float32 or bfloat16")
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        out = torch.empty(shape, dtype=out_dtype, device=device)
         if isinstance(stream, torch.cuda.Stream):
             out.record_stream(stream)
-    else:
-        _rows("out", out, q.shape[1], q.shape[2], q.shape[0], dtype)
-    return out
-
-
-def _args(q, k, v, out, cu_rows, scale):
-    a = _lib.AttentionArgs()
-    T, H, D = q.shape
-    a.q, a.out, a.cu_rows = q.data_ptr(), out.data_ptr(), cu_rows.data_ptr()
-    a.q_row, a.q_head = q.stride(0), q.stride(1)
-    a.out_row, a.out_head = out.stride(0), out.stride(1)
-    if k is not None:
-        a.k, a.v = k.data_ptr(), v.data_ptr()
-        a.k_row, a.k_head = k.stride(0), k.stride(1)
-        a.v_row, a.v_head = v.stride(0), v.stride(1)
-    a.rows, a.batch, a.heads, a.head_dim = T, cu_rows.shape[0] - 1, H, D
-    a.x_dtype, a.dtype = _DTYPES[q.dtype], _DTYPES[out.dtype]
+    s = _rows("out", out, shape, out_dtype, device)
+    a.out, a.out_row, a.out_head = out.data_ptr(), s[0], s[1]
+    if cu_rows.dim() != 1:
+        raise ValueError("the row bounds must be int32 [requests + 1]")
+    batch = cu_rows.shape[0] - 1
+    _ints("the row bounds", cu_rows, (batch + 1,), device)
+    a.cu_rows, a.rows, a.batch, a.heads, a.kv_heads, a.head_dim = cu_rows.data_ptr(), T, batch, H, kv_heads, D
+    a.x_dtype, a.dtype = _DTYPES[dtype], _DTYPES[out_dtype]
     a.scale = 1.0 / math.sqrt(D) if scale is None else scale
-    return a
-
-
-def _attend(fn, where, a, q, workspace, stream):
-    with torch.cuda.device(q.device):
-        sp = _stream_ptr(stream)
-        need = lib().mtrtq_attention_workspace_bytes(ctypes.byref(a))
-        if need < 0:
-            # the call repeats the check and says what is wrong
-            check(fn(ctypes.byref(a), None, 0, sp), where)
-        ws = _workspace(workspace, q.device, sp, need)
-        check(fn(ctypes.byref(a), ws.data_ptr() if ws is not None else None,
-                 ws.numel() * ws.element_size() if ws is not None else 0, sp), where)
+    if pages is not None:
+        (a.k_pages, a.v_pages, a.page_stride, a.num_pages, a.page_size, a.table, a.table_ld, a.table_width,
+         a.kv_len) = pages
+    sp = _stream_ptr(stream, device.index)
+    ref = ctypes.byref(a)
+    need = lib().mtrtq_attention_workspace_bytes(ref)
+    # arguments that the query refuses are refused by the call, with the reason
+    ws, nbytes = _workspace(workspace, device, sp, need) if need > 0 else (None, 0)
+    _call(where, device.index, ref, ws, nbytes, sp)
+    return out
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, *,
@@ -99,17 +120,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
     out_dtype: torch.bfloat16 (tensor cores) or torch.float32 (fp32 throughout, f32
     rows only); by default q's. scale defaults to 1 / sqrt(head_dim)."""
-    _rows("q", q, None, None, None)
-    _rows("k", k, None, q.shape[2], q.shape[0], q.dtype)
-    _rows("v", v, k.shape[1], q.shape[2], q.shape[0], q.dtype)
-    if cu_seqlens.dim() != 1:
-        raise ValueError("cu_seqlens must be int32 [requests + 1]")
-    _ints("cu_seqlens", cu_seqlens, cu_seqlens.shape, q.device)
-    out = _out(out, q, out_dtype or (out.dtype if out is not None else q.dtype), stream)
-    a = _args(q, k, v, out, cu_seqlens, scale)
-    a.kv_heads = k.shape[1]
-    _attend(lib().mtrtq_prompt_attention, "mtrtq_prompt_attention", a, q, workspace, stream)
-    return out
+    if out_dtype is None:
+        out_dtype = q.dtype if out is None else out.dtype
+    return _attend("mtrtq_prompt_attention", q, k, v, out, out_dtype, k.shape[1], cu_seqlens, scale, workspace, stream)
 
 
 def paged_attention(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None, k_pages: torch.Tensor,
@@ -124,35 +137,30 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | N
     k_pages, v_pages [pages, kv_heads, page_size, head_dim] (float32, or bfloat16 with
     q, k, v of either type); table int32 [requests, columns] of page numbers; kv_len
     int32 [requests] counts the new tokens too. The result has the cache's type."""
-    _rows("q", q, None, None, None)
     if k_pages.dim() != 4 or k_pages.dtype not in _DTYPES or k_pages.device != q.device:
         raise ValueError("k_pages must be float32 or bfloat16 [pages, kv_heads, page_size, head_dim] on q's device")
-    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or v_pages.device != q.device:
+    shape, s, dtype, device = k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.device
+    if v_pages.shape != shape or v_pages.dtype != dtype or v_pages.device != device:
         raise ValueError("v_pages must be like k_pages")
-    P, KV, S, D = k_pages.shape
-    if D != q.shape[2]:
-        raise ValueError(f"the pages' head_dim is {D}, q's {q.shape[2]}")
-    for name, x in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if x.stride(0) != k_pages.stride(0) or P == 0 or not x[0].is_contiguous():
-            raise ValueError(f"each page of {name} must be contiguous")
+    P, KV, S, D = shape
+    # (strides of single heads say nothing)
+    if P == 0 or s[1:] != (S * D, D, 1) and not k_pages[0].is_contiguous() or v_pages.stride() != s \
+            and (v_pages.stride(0) != s[0] or not v_pages[0].is_contiguous()):
+        raise ValueError("pages of k_pages and v_pages must be contiguous, and equally far apart")
+    if D != q.shape[-1]:
+        raise ValueError(f"the pages' head_dim is {D}, q's {q.shape[-1]}")
     if (k is None) != (v is None):
         raise ValueError("k and v are given together")
-    if k is not None:
-        _rows("k", k, KV, D, q.shape[0], q.dtype)
-        _rows("v", v, KV, D, q.shape[0], q.dtype)
     if kv_len.dim() != 1 or table.dim() != 2:
         raise ValueError("kv_len must be int32 [requests], table int32 [requests, columns]")
-    B = kv_len.shape[0]
-    _ints("kv_len", kv_len, (B,), q.device)
-    _ints("table", table, (B, table.shape[1]), q.device)
-    _ints("cu_rows", cu_rows, (B + 1,), q.device)
-    out = _out(out, q, k_pages.dtype, stream)
-    a = _args(q, k, v, out, cu_rows, scale)
-    a.kv_heads, a.page_size, a.num_pages, a.page_stride = KV, S, P, k_pages.stride(0)
-    a.k_pages, a.v_pages, a.kv_len = k_pages.data_ptr(), v_pages.data_ptr(), kv_len.data_ptr()
-    a.table, a.table_ld, a.table_width = table.data_ptr(), table.stride(0), table.shape[1]
-    _attend(lib().mtrtq_paged_attention, "mtrtq_paged_attention", a, q, workspace, stream)
-    return out
+    B, width = table.shape
+    _ints("kv_len", kv_len, (B,), device)
+    ld = _ints("table", table, (B, width), device)[0]
+    if cu_rows.shape != (B + 1,):
+        raise ValueError(f"cu_rows must be int32 [{B + 1}]")
+    pages = (k_pages.data_ptr(), v_pages.data_ptr(), s[0], P, S, table.data_ptr(), ld if B > 1 else width, width,
+             kv_len.data_ptr())
+    return _attend("mtrtq_paged_attention", q, k, v, out, dtype, KV, cu_rows, scale, workspace, stream, pages)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor, eos: int = -1, *,
@@ -170,7 +178,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor, 
     if done.dtype != torch.uint8 or done.shape != scores.shape or done.device != dev or not done.is_contiguous():
         raise ValueError("done must be contiguous uint8 [requests, beams]")
     if logits.dim() != 2 or logits.dtype != torch.float32 or logits.shape[0] != B * W or logits.device != dev \
-            or logits.stride(1) != 1:
+            or logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("logits must be float32 [requests * beams, vocab] with unit stride along vocab")
     if out is None:
         out = (torch.empty_like(scores), torch.empty((B, W), dtype=torch.int32, device=dev),
@@ -183,15 +191,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor, 
             if x.shape != scores.shape or x.dtype != t or x.device != dev or not x.is_contiguous():
                 raise ValueError("out is (float32, int32, int32, uint8), each contiguous [requests, beams]")
     V = logits.shape[1]
-    with torch.cuda.device(dev):
-        sp = _stream_ptr(stream)
-        need = lib().mtrtq_beam_workspace_bytes(B, W, V)
-        ws = _workspace(workspace, dev, sp, need) if need >= 0 else None
-        check(lib().mtrtq_beam_select(logits.data_ptr(), logits.stride(0), scores.data_ptr(), done.data_ptr(), eos, B,
-                                      W, V, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
-                                      out[3].data_ptr(), ws.data_ptr() if ws is not None else None,
-                                      ws.numel() * ws.element_size() if ws is not None else 0, sp),
-              "mtrtq_beam_select")
+    sp = _stream_ptr(stream, dev.index)
+    need = lib().mtrtq_beam_workspace_bytes(B, W, V)
+    ws, nbytes = _workspace(workspace, dev, sp, need) if need > 0 else (None, 0)
+    _call("mtrtq_beam_select", dev.index, logits.data_ptr(), logits.stride(0) if B * W > 1 else V, scores.data_ptr(), done.data_ptr(), eos,
+          B, W, V, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), ws, nbytes, sp)
     return out
 
 
@@ -212,19 +216,20 @@ def beam_reorder(parent: torch.Tensor, table: torch.Tensor, owned: torch.Tensor,
     if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or v_pages.device != k_pages.device:
         raise ValueError("v_pages must be like k_pages")
     L, P, KV, S, D = k_pages.shape
-    for name, x in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if x.stride()[:2] != k_pages.stride()[:2] or 0 in (L, P) or not x[0, 0].is_contiguous():
-            raise ValueError(f"each page of {name} must be contiguous")
+    s = k_pages.stride()
+    if 0 in (L, P) or s[2:] != (S * D, D, 1) and not k_pages[0, 0].is_contiguous() or v_pages.stride() != s \
+            and (v_pages.stride()[:2] != s[:2] or not v_pages[0, 0].is_contiguous()):
+        raise ValueError("pages of k_pages and v_pages must be contiguous, and equally far apart")
     B, W = parent.shape
     dev = k_pages.device
-    _ints("parent", parent, (B, W), dev)
-    if not parent.is_contiguous():
+    if _ints("parent", parent, (B, W), dev)[0] != W and B > 1:
         raise ValueError("parent must be contiguous")
-    _ints("table", table, (B * W, table.shape[1]), dev)
-    _ints("owned", owned, tuple(table.shape), dev)
+    width = table.shape[1]
+    ld = _ints("table", table, (B * W, width), dev)[0]
+    ldo = _ints("owned", owned, (B * W, width), dev)[0]
+    if B * W == 1:
+        ld = ldo = width
     _ints("kv_len", kv_len, (B,), dev)
-    with torch.cuda.device(dev):
-        check(lib().mtrtq_beam_reorder(parent.data_ptr(), B, W, table.data_ptr(), table.stride(0), owned.data_ptr(),
-                                       owned.stride(0), table.shape[1], kv_len.data_ptr(), k_pages.data_ptr(),
-                                       v_pages.data_ptr(), L, k_pages.stride(0), k_pages.stride(1), P, KV, S, D,
-                                       _DTYPES[k_pages.dtype], _stream_ptr(stream)), "mtrtq_beam_reorder")
+    _call("mtrtq_beam_reorder", dev.index, parent.data_ptr(), B, W, table.data_ptr(), ld, owned.data_ptr(),
+          ldo, width, kv_len.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), L, s[0], s[1], P, KV, S, D,
+          _DTYPES[k_pages.dtype], _stream_ptr(stream, dev.index))
