@@ -17,15 +17,6 @@ namespace {
 
 typedef mtrtq_attention_args Args;
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // Rows of request b, with malformed bounds clamped so that no access leaves the rows.
 __device__ __forceinline__ void request_rows(const Args& a, int64_t b, int64_t& r0, int64_t& r1) {
   const int64_t lo = a.cu_rows[b], hi = a.cu_rows[b + 1];
@@ -33,16 +24,19 @@ __device__ __forceinline__ void request_rows(const Args& a, int64_t b, int64_t& 
   r1 = hi < r0 ? r0 : hi > a.rows ? a.rows : hi;
 }
 
-// The request that owns row r, or -1: the last b with cu_rows[b] <= r.
-__device__ int64_t request_of(const Args& a, int64_t r) {
-  int64_t lo = 0, hi = a.batch;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    if (mid < a.batch && a.cu_rows[mid] <= r) lo = mid; else hi = mid - 1;
+// The request that owns row r, or -1: every thread of the block looks at a few requests
+// (one round of loads; a row in two requests goes to the later one).
+__device__ int request_of(const Args& a, int64_t r) {
+  __shared__ int found;
+  if (threadIdx.x == 0) found = -1;
+  __syncthreads();
+  for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+    int64_t r0, r1;
+    request_rows(a, b, r0, r1);
+    if (r >= r0 && r < r1) atomicMax(&found, b);
   }
-  int64_t r0, r1;
-  request_rows(a, lo, r0, r1);
-  return r >= r0 && r < r1 ? lo : -1;
+  __syncthreads();
+  return found;
 }
 
 // Where token i of request b lies in the pages of head g (elements); -1 if its page
@@ -55,48 +49,63 @@ __device__ __forceinline__ int64_t page_offset(const Args& a, int64_t b, int64_t
   return n * a.page_stride + (g * a.page_size + i % a.page_size) * a.head_dim;
 }
 
+// Four elements from src, as TC, to dst (16-byte aligned f32, 8-byte aligned bf16).
+__device__ __forceinline__ float4 load4(const float* src) { return *reinterpret_cast<const float4*>(src); }
+__device__ __forceinline__ float4 load4(const __nv_bfloat16* src) {
+  const uint2 u = *reinterpret_cast<const uint2*>(src);
+  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                     __uint_as_float(u.y & 0xffff0000u));
+}
+__device__ __forceinline__ void store4(float* dst, float4 x) { *reinterpret_cast<float4*>(dst) = x; }
+__device__ __forceinline__ void store4(__nv_bfloat16* dst, float4 x) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x, x.y), hi = __floats2bfloat162_rn(x.z, x.w);
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(reinterpret_cast<const uint32_t&>(lo), reinterpret_cast<const uint32_t&>(hi));
+}
+
 // One block per new row: its k and v go to its position's page, rounded to the
 // cache's type; q_rows (if not null) gets q in that type, [rows, heads, head_dim].
+constexpr int kRowThreads = 256;
 template <typename TX, typename TC>
-__global__ void append_kernel(const __grid_constant__ Args a, TC* q_rows) {
+__global__ void __launch_bounds__(kRowThreads) append_kernel(const __grid_constant__ Args a, TC* q_rows) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t r = blockIdx.x;
+  const int quads = a.head_dim / 4;
   if (q_rows) {
-    for (int e = threadIdx.x; e < a.heads * a.head_dim; e += blockDim.x) {
-      const int h = e / a.head_dim, d = e - h * a.head_dim;
-      q_rows[r * a.heads * a.head_dim + e] =
-          from_f32<TC>(to_f32(static_cast<const TX*>(a.q)[r * a.q_row + h * a.q_head + d]));
+    for (int e = threadIdx.x; e < a.heads * quads; e += kRowThreads) {
+      const int h = e / quads, d = (e - h * quads) * 4;
+      store4(q_rows + (r * a.heads + h) * a.head_dim + d, load4(static_cast<const TX*>(a.q) + r * a.q_row + h * a.q_head + d));
     }
   }
   if (!a.k) return;
-  const int64_t b = request_of(a, r);
+  const int b = request_of(a, r);
   if (b < 0) return;
   int64_t r0, r1;
   request_rows(a, b, r0, r1);
   const int64_t i = (int64_t)a.kv_len[b] - (r1 - r0) + (r - r0);
-  for (int e = threadIdx.x; e < a.kv_heads * a.head_dim; e += blockDim.x) {
-    const int g = e / a.head_dim, d = e - g * a.head_dim;
+  for (int e = threadIdx.x; e < a.kv_heads * quads; e += kRowThreads) {
+    const int g = e / quads, d = (e - g * quads) * 4;
+    const float4 k = load4(static_cast<const TX*>(a.k) + r * a.k_row + g * a.k_head + d);
+    const float4 v = load4(static_cast<const TX*>(a.v) + r * a.v_row + g * a.v_head + d);
     const int64_t at = page_offset(a, b, i, g);
     if (at < 0) continue;
-    static_cast<TC*>(a.k_pages)[at + d] =
-        from_f32<TC>(to_f32(static_cast<const TX*>(a.k)[r * a.k_row + g * a.k_head + d]));
-    static_cast<TC*>(a.v_pages)[at + d] =
-        from_f32<TC>(to_f32(static_cast<const TX*>(a.v)[r * a.v_row + g * a.v_head + d]));
+    store4(static_cast<TC*>(a.k_pages) + at + d, k);
+    store4(static_cast<TC*>(a.v_pages) + at + d, v);
   }
 }
 
 // Rows of q, k and v in bf16, [rows, heads + 2 kv_heads, head_dim].
 template <typename TX>
-__global__ void cast_kernel(const __grid_constant__ Args a, __nv_bfloat16* rows) {
+__global__ void __launch_bounds__(kRowThreads) cast_kernel(const __grid_constant__ Args a, __nv_bfloat16* rows) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t r = blockIdx.x;
-  const int hq = a.heads, hk = a.kv_heads, all = hq + 2 * hk;
-  for (int e = threadIdx.x; e < all * a.head_dim; e += blockDim.x) {
-    const int h = e / a.head_dim, d = e - h * a.head_dim;
+  const int hq = a.heads, hk = a.kv_heads, all = hq + 2 * hk, quads = a.head_dim / 4;
+  for (int e = threadIdx.x; e < all * quads; e += kRowThreads) {
+    const int h = e / quads, d = (e - h * quads) * 4;
     const TX* src = h < hq        ? static_cast<const TX*>(a.q) + r * a.q_row + h * a.q_head
                     : h < hq + hk ? static_cast<const TX*>(a.k) + r * a.k_row + (h - hq) * a.k_head
                                   : static_cast<const TX*>(a.v) + r * a.v_row + (h - hq - hk) * a.v_head;
-    rows[r * all * a.head_dim + e] = from_f32<__nv_bfloat16>(to_f32(src[d]));
+    store4(rows + (r * all + h) * a.head_dim + d, load4(src + d));
   }
 }
 
@@ -138,7 +147,7 @@ int check_args(const Args* a, bool paged) {
   if (a->page_size != 16 && a->page_size != 32 && a->page_size != 64 && a->page_size != 128)
     return report_error(MTRTQ_ERR_INVALID_ARG, "page_size (%d) is 16, 32, 64 or 128", a->page_size);
   if (a->num_pages < 1 || a->num_pages > 2147483647 || a->table_width < 1 ||
-      a->table_width * a->page_size > 2147483647 || a->table_ld < a->table_width)
+      a->table_width * a->page_size > (int64_t(1) << 30) || a->table_ld < a->table_width)
     return report_error(MTRTQ_ERR_INVALID_ARG, "num_pages (%lld), table_width (%lld) or table_ld (%lld) is out of range",
                         (long long)a->num_pages, (long long)a->table_width, (long long)a->table_ld);
   if (a->page_stride < (int64_t)a->kv_heads * a->page_size * a->head_dim || a->page_stride >= (int64_t(1) << 36))
@@ -235,12 +244,12 @@ int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cuda
   const bool before = l.cast || (paged && a.k);
   if (before) {
     if (!paged) {
-      if (a.x_dtype == MTRTQ_DTYPE_F32) cast_kernel<float><<<(unsigned)a.rows, 256, 0, st>>>(a, rows);
-      else cast_kernel<__nv_bfloat16><<<(unsigned)a.rows, 256, 0, st>>>(a, rows);
+      if (a.x_dtype == MTRTQ_DTYPE_F32) cast_kernel<float><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, rows);
+      else cast_kernel<__nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, rows);
     } else if (a.x_dtype == MTRTQ_DTYPE_F32) {
-      append_kernel<float, __nv_bfloat16><<<(unsigned)a.rows, 256, 0, st>>>(a, l.cast ? rows : nullptr);
+      append_kernel<float, __nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, l.cast ? rows : nullptr);
     } else {
-      append_kernel<__nv_bfloat16, __nv_bfloat16><<<(unsigned)a.rows, 256, 0, st>>>(a, l.cast ? rows : nullptr);
+      append_kernel<__nv_bfloat16, __nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, l.cast ? rows : nullptr);
     }
     if (int rc = cuda_status(cudaGetLastError(), "attention rows launch")) return rc;
   }
@@ -320,7 +329,7 @@ int launch_f32(const Args& a, bool paged, void* workspace, cudaStream_t st) {
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const bool before = paged && a.k;
   if (before) {
-    append_kernel<float, float><<<(unsigned)a.rows, 256, 0, st>>>(a, nullptr);
+    append_kernel<float, float><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, nullptr);
     if (int rc = cuda_status(cudaGetLastError(), "attention rows launch")) return rc;
   }
   F32Attention p = {};

@@ -34,9 +34,9 @@ struct Cfg {
   static constexpr int OFF_V = OFF_K + HD * KS;         // [kKeys][HD]
   static constexpr int OFF_P = OFF_V + kKeys * HD;      // [kKeys][QS]
   static constexpr int FLOATS = OFF_P + kKeys * QS;
-  static constexpr int BYTES = FLOATS * 4 + (MTRTQ_MAX_BATCH + 1) * 8;
-  static constexpr int CTAS = BYTES <= 112 * 1024 ? 2 : 1;
-  static_assert(BYTES <= 226 * 1024 && FLOATS % 2 == 0, "shared memory per CTA");
+  static constexpr int BYTES = FLOATS * 4;  // and the list of steps
+  static constexpr int CTAS = HD == 64 || RM == 1 ? 2 : 1;
+  static_assert(CTAS * (BYTES + 5 * 1024) <= 228 * 1024 && FLOATS % 4 == 0, "shared memory per CTA");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -55,26 +55,28 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
   extern __shared__ float4 raw4[];
   float* sm = reinterpret_cast<float*>(raw4);
   float *qs = sm + C::OFF_Q, *ks = sm + C::OFF_K, *vs = sm + C::OFF_V, *ps = sm + C::OFF_P;
-  int64_t* prefix = reinterpret_cast<int64_t*>(sm + C::FLOATS);
-  __shared__ int start[4];
+  const StepList list(sm + C::FLOATS, p.batch);
+  __shared__ Walk walks[kThreads / 32];
+  __shared__ Segment segments[kThreads / 32];
   __shared__ unsigned ticket;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, lane = tid & 31, warp = tid >> 5;
 
-  int64_t per;
-  Walk<kKeys> walk = find_run<kKeys, kThreads>(p, prefix, start, per);
+  make_list<kKeys, kThreads>(p, list, walks);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float c2 = p.scale * 1.4426950408889634f;  // scale log2 e
 
-  Segment s;
-  while (walk.next(p, s)) {
+  Segment& s = segments[warp];
+  while (next_segment<kKeys>(p, list, walks[warp], s)) {
+    const int64_t r0 = list.req[s.b].r0;  // where the request's rows start
+    const int tokens = s.tokens, keys = s.keys;
     // Q, transposed; rows past the tile's tokens and dimensions past the head's are zero.
     __syncthreads();
     for (int e = tid; e < C::BM * (HD / 4); e += kThreads) {
       const int row = e % C::BM, d = e / C::BM * 4;
       const int token = row / p.group, head = row - token * p.group;
       float4 x = make_float4(0, 0, 0, 0);
-      if (token < s.tile.tokens && d < p.head_dim)
-        x = *reinterpret_cast<const float4*>(p.q + (s.q.r0 + s.tile.t0 + token) * p.q_row +
+      if (token < tokens && d < p.head_dim)
+        x = *reinterpret_cast<const float4*>(p.q + (s.row0 + (int64_t)token) * p.q_row +
                                              (int64_t)(s.h * p.group + head) * p.q_head + d);
       qs[d * C::QS + row] = x.x;
       qs[(d + 1) * C::QS + row] = x.y;
@@ -83,7 +85,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
     }
     float m[RM], l[RM], o[RM][4 * NC];
     int sees[RM];  // keys the row sees
-    int least = 0x7fffffff;
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
       m[r] = -INFINITY;
@@ -91,14 +92,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
 #pragma unroll
       for (int c = 0; c < 4 * NC; ++c) o[r][c] = 0.0f;
       const int token = (ty * RM + r) / p.group;
-      const int64_t n = s.q.ctx + s.tile.t0 + token + 1;
-      sees[r] = token < s.tile.tokens ? (int)max((int64_t)0, min(n, (int64_t)s.q.keys)) : 0;
-      if (token < s.tile.tokens) least = min(least, sees[r]);
+      sees[r] = token < tokens ? max(0, min(s.see0 + token, keys)) : 0;
     }
-    const int64_t first_sees = s.q.ctx + s.tile.t0 + 1;
-    const int64_t all_see = first_sees < s.q.keys ? first_sees : s.q.keys;
+    const int all_see = s.all_see(), k1 = s.k0 + s.n;
 
-    for (int j = s.j0; j < s.j1; ++j) {
+    for (int j = s.k0; j < k1; ++j) {
       const int key0 = j * kKeys;
       __syncthreads();
       // K transposed: a lane per key; V as it is. Tokens past the keys, and pages out of
@@ -107,13 +105,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
       {
         const int key = key0 + (warp & 1) * 32 + lane;
         const float* src = nullptr;
-        if (key < s.q.keys) {
+        if (key < keys) {
           if (PAGED) {
             const int64_t page = p.table[s.b * p.table_ld + key / p.page_size];
             if (page >= 0 && page < p.num_pages)
               src = p.k + page * p.k_row + ((int64_t)s.h * p.page_size + key % p.page_size) * p.head_dim;
           } else {
-            src = p.k + (s.q.r0 + key) * p.k_row + s.h * p.k_head;
+            src = p.k + (r0 + key) * p.k_row + s.h * p.k_head;
           }
         }
         float* dst = ks + (warp & 1) * 32 + lane;
@@ -130,21 +128,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
         for (int c = 0; c < kKeys * HD / 4 / kThreads; ++c) {
           const int e = c * kThreads + tid, r = e / (HD / 4), d = e % (HD / 4) * 4, at = key0 + r;
           float4 x = make_float4(0, 0, 0, 0);
-          if (at < s.q.keys && d < p.head_dim) {
+          if (at < keys && d < p.head_dim) {
             if (PAGED) {
               const int64_t page = p.table[s.b * p.table_ld + at / p.page_size];
               if (page >= 0 && page < p.num_pages)
                 x = *reinterpret_cast<const float4*>(
                     p.v + page * p.v_row + ((int64_t)s.h * p.page_size + at % p.page_size) * p.head_dim + d);
             } else {
-              x = *reinterpret_cast<const float4*>(p.v + (s.q.r0 + at) * p.v_row + s.h * p.v_head + d);
+              x = *reinterpret_cast<const float4*>(p.v + (r0 + at) * p.v_row + s.h * p.v_head + d);
             }
           }
           odd |= broken(x.x) | broken(x.y) | broken(x.z) | broken(x.w);
           *reinterpret_cast<float4*>(vs + r * HD + d) = x;
         }
       }
-      const bool partly = (int64_t)key0 + kKeys > all_see;
+      const bool partly = key0 + kKeys > all_see;
       const bool careful = __syncthreads_or(odd) && partly;
 
       // S: rows in pairs, four keys
@@ -262,15 +260,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
       for (int x = 8; x > 0; x >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
       if (m[r] == -INFINITY && l[r] != l[r]) m[r] = 0.0f;  // every score it saw was NaN
     }
-    const bool whole = s.whole();
-    const int64_t part = (int64_t)blockIdx.x * 2 + (s.j0 > 0 ? 0 : 1);
+    const bool whole = s.whole;
+    const int64_t part = (int64_t)blockIdx.x * 2 + s.part;
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
       const int row = ty * RM + r, token = row / p.group, head = row - token * p.group;
-      if (token >= s.tile.tokens) continue;
+      if (token >= tokens) continue;
       if (whole) {
         const float inv = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
-        float* dst = p.out + (s.q.r0 + s.tile.t0 + token) * p.out_row + (int64_t)(s.h * p.group + head) * p.out_head;
+        float* dst = p.out + (s.row0 + (int64_t)token) * p.out_row + (int64_t)(s.h * p.group + head) * p.out_head;
 #pragma unroll
         for (int g = 0; g < NC; ++g) {
           const int d = g * 64 + 4 * tx;
@@ -289,12 +287,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
     }
     if (!whole) {
       // the CTA that finishes a cut tile last joins its parts in order
-      const int64_t c_first = s.first / per, c_last = (s.first + s.tile.steps - 1) / per;
+      const int64_t c_first = s.c_first, c_last = s.c_last;
       __syncthreads();
       if (tid == 0) ticket = ticket_acq_rel(p.counters + c_first);
       __syncthreads();
       if (ticket == (unsigned)(c_last - c_first)) {
-        const int rows = s.tile.tokens * p.group, vecs = p.head_dim / 4;
+        const int rows = tokens * p.group, vecs = p.head_dim / 4;
         for (int e = tid; e < rows * vecs; e += kThreads) {
           const int row = e / vecs, d = e % vecs * 4, token = row / p.group, head = row - token * p.group;
           float top = -INFINITY;
@@ -315,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
             x.w += y.w * w;
           }
           const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          *reinterpret_cast<float4*>(p.out + (s.q.r0 + s.tile.t0 + token) * p.out_row +
+          *reinterpret_cast<float4*>(p.out + (s.row0 + (int64_t)token) * p.out_row +
                                      (int64_t)(s.h * p.group + head) * p.out_head + d) =
               make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
         }
@@ -328,11 +326,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
 template <int HD, int RM, bool PAGED>
 cudaError_t launch_one(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
   auto kernel = attention_f32_kernel<HD, RM, PAGED>;
-  if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kernel), Cfg<HD, RM>::BYTES)) return e;
+  constexpr int most = Cfg<HD, RM>::BYTES + StepList::bytes(MTRTQ_MAX_BATCH);
+  static_assert(most + 3 * 1024 <= 227 * 1024, "shared memory per CTA");
+  if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kernel), most)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<HD, RM>::BYTES;
+  cfg.dynamicSmemBytes = Cfg<HD, RM>::BYTES + StepList::bytes(p.batch);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -7,179 +7,234 @@
 // order request, head, tile, block, are cut into equal runs, one for each CTA.
 #pragma once
 
+#include "../../include/mtrtq.h"
 #include "attention.h"
 
 namespace mtrtq {
 
+// A request's rows r0 .. r0 + m - 1, the position of the first (negative: rows before
+// the first position see nothing), and the keys it has.
 struct Request {
-  int64_t r0;
-  int m;        // rows
-  int64_t ctx;  // position of row 0 (negative: rows before the first position see nothing)
-  int keys;     // keys it has
+  int r0, m, ctx, keys;
 };
 
-struct Tile {
-  int t0, tokens;  // its tokens, of the request's rows
-  bool pair;       // its rows fill more than one slot (f32: always; slot_tokens is 0)
-  int blocks, steps;
-};
-
+// What a role needs to know of its next run of one tile's steps. Every warp keeps its own
+// walk and segment in shared memory, out of the registers.
 struct Segment {
-  Request q;
-  Tile tile;
   int b, h;
-  int j0, j1;     // its steps of the tile's
-  int64_t first;  // the tile's first step in the list
-  __device__ bool whole() const { return j0 == 0 && j1 == tile.steps; }
+  int row0;        // the tile's first row
+  int tokens;      // its tokens
+  int see0;        // keys that the first row sees, if the request has them
+  int keys;        // keys the request has
+  int pair;        // the rows fill more than one slot (f32: always)
+  int k0, n;       // blocks of keys k0 .. k0 + n - 1
+  int cnt[2];      // of them, blocks of each slot
+  int whole;       // all of the tile's steps
+  int part;        // else: which of the CTA's two partials
+  int c_first, c_last;  // else: the CTAs that have parts of the tile
+  int buf;         // halves: which of the two Q buffers
+  int q_use[2];    // earlier uses of the Q buffers
+  __device__ int all_see() const { return min(see0, keys); }
+};
+
+struct Walk {
+  int64_t u, end, per;
+  int b, h, i, j;
+  int buf, q_use[2];
+};
+
+struct StepList {
+  Request* req;
+  int64_t* prefix;  // steps before each request
+  static constexpr int bytes(int batch) { return batch * (int)sizeof(Request) + (batch + 2) / 2 * 16; }
+  __device__ StepList(void* shared, int batch)
+      : req(static_cast<Request*>(shared)), prefix(reinterpret_cast<int64_t*>(req + batch)) {}
 };
 
 __device__ __forceinline__ Request load_request(const AttentionList& p, int b) {
+  const int lo = p.cu_rows[b], hi = p.cu_rows[b + 1], rows = (int)p.rows;
+  const int n = p.table ? p.kv_len[b] : 0;
   Request q;
-  const int64_t lo = p.cu_rows[b], hi = p.cu_rows[b + 1];
-  q.r0 = lo < 0 ? 0 : lo > p.rows ? p.rows : lo;
-  q.m = (int)((hi < q.r0 ? q.r0 : hi > p.rows ? p.rows : hi) - q.r0);
-  if (p.table) {
-    const int64_t n = p.kv_len[b];
-    q.ctx = n - q.m;
-    q.keys = (int)(n < 0 ? 0 : n < p.max_keys ? n : p.max_keys);
-  } else {
-    q.ctx = 0;
-    q.keys = q.m;
-  }
+  q.r0 = min(max(lo, 0), rows);
+  q.m = min(max(hi, q.r0), rows) - q.r0;
+  q.ctx = p.table ? max(n, -(1 << 30)) - q.m : 0;
+  q.keys = p.table ? min(max(n, 0), (int)p.max_keys) : q.m;
   return q;
-}
-
-template <int BLOCK>
-__device__ __forceinline__ Tile make_tile(const AttentionList& p, const Request& q, int i) {
-  Tile t;
-  t.t0 = i * p.tile_tokens;
-  t.tokens = min(p.tile_tokens, q.m - t.t0);
-  t.pair = t.tokens > p.slot_tokens;
-  const int64_t seen = q.ctx + t.t0 + t.tokens;
-  const int keys = (int)(seen < q.keys ? seen : q.keys);
-  t.blocks = keys <= 0 ? 1 : (keys + BLOCK - 1) / BLOCK;
-  t.steps = t.pair ? t.blocks : (t.blocks + 1) >> 1;
-  return t;
 }
 
 __device__ __forceinline__ int tile_count(const AttentionList& p, const Request& q) {
   return (q.m + p.tile_tokens - 1) / p.tile_tokens;
 }
 
+// Blocks of keys that tokens t0 .. t0 + tokens - 1 see together; at least one, so that
+// rows that see none are written too.
 template <int BLOCK>
-struct Walk {
-  int64_t u, end;
-  int b, h, i, j;
-  Request q;
+__device__ __forceinline__ int block_count(const Request& q, int t0, int tokens) {
+  return max(1, (min(q.keys, q.ctx + t0 + tokens) + BLOCK - 1) / BLOCK);
+}
 
-  __device__ bool next(const AttentionList& p, Segment& s) {
-    if (u >= end) return false;
-    s.q = q;
-    s.tile = make_tile<BLOCK>(p, q, i);
-    s.b = b;
-    s.h = h;
-    s.j0 = j;
-    s.first = u - j;
-    const int64_t take = min((int64_t)(s.tile.steps - j), end - u);
-    s.j1 = j + (int)take;
-    u += take;
-    j = s.j1;
-    if (j == s.tile.steps) {
-      j = 0;
-      if (++i == tile_count(p, q)) {
-        i = 0;
-        if (++h == p.kv_heads) {
-          h = 0;
-          if (u < end) {
-            do q = load_request(p, ++b); while (q.m == 0);
+template <int BLOCK>
+__device__ __forceinline__ int tile_steps(const AttentionList& p, const Request& q, int i) {
+  const int t0 = i * p.tile_tokens, tokens = min(p.tile_tokens, q.m - t0);
+  const int blocks = block_count<BLOCK>(q, t0, tokens);
+  return tokens > p.slot_tokens ? blocks : (blocks + 1) >> 1;
+}
+
+// The whole warp calls it; false at the end of the CTA's run.
+template <int BLOCK>
+__device__ bool next_segment(const AttentionList& p, const StepList list, Walk& w, Segment& s) {
+  int more = 0;
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0 && w.u < w.end) {
+    more = 1;
+    const Request q = list.req[w.b];
+    const int t0 = w.i * p.tile_tokens, tokens = min(p.tile_tokens, q.m - t0);
+    const int blocks = block_count<BLOCK>(q, t0, tokens);
+    const bool pair = tokens > p.slot_tokens;
+    const int steps = pair ? blocks : (blocks + 1) >> 1;
+    const int take = (int)min((int64_t)(steps - w.j), w.end - w.u), j1 = w.j + take;
+    s.b = w.b;
+    s.h = w.h;
+    s.row0 = q.r0 + t0;
+    s.tokens = tokens;
+    s.see0 = q.ctx + t0 + 1;
+    s.keys = q.keys;
+    s.pair = pair;
+    s.k0 = pair ? w.j : 2 * w.j;
+    s.n = (pair ? j1 : min(2 * j1, blocks)) - s.k0;
+    if (pair) {
+      const int sees = min(q.keys, q.ctx + t0 + p.slot_tokens);  // slot 0's last row
+      s.cnt[0] = max(0, min(j1, sees <= 0 ? 0 : (sees + BLOCK - 1) / BLOCK) - w.j);
+      s.cnt[1] = s.n;
+    } else {
+      s.cnt[0] = (s.n + 1) >> 1;
+      s.cnt[1] = s.n >> 1;
+    }
+    s.whole = take == steps;
+    if (!s.whole) {
+      const int64_t first = w.u - w.j;
+      s.part = w.j > 0 ? 0 : 1;
+      s.c_first = (int)(first / w.per);
+      s.c_last = (int)((first + steps - 1) / w.per);
+    }
+    s.buf = w.buf;
+    s.q_use[0] = w.q_use[0];
+    s.q_use[1] = w.q_use[1];
+    if (pair) {
+      ++w.q_use[0];
+      ++w.q_use[1];
+      w.buf = 0;
+    } else {
+      ++w.q_use[w.buf];
+      w.buf ^= 1;
+    }
+    w.u += take;
+    w.j = j1;
+    if (j1 == steps) {
+      w.j = 0;
+      if (++w.i == tile_count(p, q)) {
+        w.i = 0;
+        if (++w.h == p.kv_heads) {
+          w.h = 0;
+          if (w.u < w.end) {
+            do ++w.b; while (list.req[w.b].m == 0);
           }
         }
       }
     }
-    return true;
   }
-};
+  more = __shfl_sync(0xffffffffu, more, 0);
+  __syncwarp();
+  return more != 0;
+}
 
-// This CTA's run, and the steps of a run in `per`. All threads; prefix has batch + 1
-// entries and start 4 in shared memory.
+// Fills the list and this CTA's walk (of every warp). All threads.
 template <int BLOCK, int THREADS>
-__device__ Walk<BLOCK> find_run(const AttentionList& p, int64_t* prefix, volatile int* start, int64_t& per) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // Steps of each request, then their running total.
-  for (int b = warp; b < p.batch; b += THREADS / 32) {
+__device__ void make_list(const AttentionList& p, const StepList list, Walk* walks) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // Requests, and the steps of those with few tiles: a thread each.
+  bool many = false;
+  for (int b = tid; b < p.batch; b += THREADS) {
     const Request q = load_request(p, b);
+    list.req[b] = q;
     const int n = tile_count(p, q);
     int64_t sum = 0;
-    for (int i = lane; i < n; i += 32) sum += make_tile<BLOCK>(p, q, i).steps;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) prefix[b + 1] = sum;
+    if (n <= 8) {
+      for (int i = 0; i < n; ++i) sum += tile_steps<BLOCK>(p, q, i);
+    } else {
+      sum = -1;
+      many = true;
+    }
+    list.prefix[b + 1] = sum;
   }
-  if (threadIdx.x == 0) prefix[0] = 0;
-  __syncthreads();
+  if (tid == 0) list.prefix[0] = 0;
+  if (__syncthreads_or(many)) {
+    for (int b = warp; b < p.batch; b += THREADS / 32) {
+      if (list.prefix[b + 1] >= 0) continue;
+      const Request q = list.req[b];
+      const int n = tile_count(p, q);
+      int64_t sum = 0;
+      for (int i = lane; i < n; i += 32) sum += tile_steps<BLOCK>(p, q, i);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      __syncwarp();
+      if (lane == 0) list.prefix[b + 1] = sum;
+    }
+    __syncthreads();
+  }
   if (warp == 0) {
     int64_t run = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      int64_t v = b0 + lane < p.batch ? prefix[b0 + lane + 1] * p.kv_heads : 0;
+      int64_t v = b0 + lane < p.batch ? list.prefix[b0 + lane + 1] * p.kv_heads : 0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += w;
       }
-      if (b0 + lane < p.batch) prefix[b0 + lane + 1] = run + v;
+      if (b0 + lane < p.batch) list.prefix[b0 + lane + 1] = run + v;
       run += __shfl_sync(0xffffffffu, v, 31);
     }
-  }
-  __syncthreads();
-  const int64_t total = prefix[p.batch];
-  per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < p.min_steps) per = p.min_steps;
-  Walk<BLOCK> walk;
-  walk.u = min(total, per * blockIdx.x);
-  walk.end = min(total, walk.u + per);
-  if (warp == 0 && walk.u < walk.end) {
-    int lo = 0, hi = p.batch - 1;  // the last request whose first step is not after u
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] <= walk.u) lo = mid; else hi = mid - 1;
-    }
-    const Request q = load_request(p, lo);
-    const int64_t each = (prefix[lo + 1] - prefix[lo]) / p.kv_heads;
-    int64_t left = walk.u - prefix[lo];
-    const int h = (int)(left / each);
-    left -= h * each;
-    const int n = tile_count(p, q);
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      int64_t v = i0 + lane < n ? make_tile<BLOCK>(p, q, i0 + lane).steps : 0;
-      const int64_t mine = v;
+    __syncwarp();
+    const int64_t total = run, per = max((total + gridDim.x - 1) / gridDim.x, p.min_steps);
+    Walk w;
+    w.per = per;
+    w.u = min(total, per * blockIdx.x);
+    w.end = min(total, w.u + per);
+    w.b = w.h = w.i = w.j = w.buf = w.q_use[0] = w.q_use[1] = 0;
+    if (w.u < w.end) {
+      int lo = 0, hi = p.batch - 1;  // the last request whose first step is not after u
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (list.prefix[mid] <= w.u) lo = mid; else hi = mid - 1;
+      }
+      const Request q = list.req[lo];
+      const int64_t each = (list.prefix[lo + 1] - list.prefix[lo]) / p.kv_heads;
+      int64_t left = w.u - list.prefix[lo];
+      w.b = lo;
+      w.h = (int)(left / each);
+      left -= w.h * each;
+      const int n = tile_count(p, q);
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        int64_t v = i0 + lane < n ? tile_steps<BLOCK>(p, q, i0 + lane) : 0;
+        const int64_t mine = v;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += w;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, v > left);
-      if (past) {
-        if (lane == __ffs(past) - 1) {
-          start[0] = lo;
-          start[1] = h;
-          start[2] = i0 + lane;
-          start[3] = (int)(left - (v - mine));
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t x = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += x;
         }
-        break;
+        const unsigned past = __ballot_sync(0xffffffffu, v > left);
+        if (past) {
+          const int at = __ffs(past) - 1;
+          w.i = i0 + at;
+          w.j = (int)__shfl_sync(0xffffffffu, left - (v - mine), at);
+          break;
+        }
+        left -= __shfl_sync(0xffffffffu, v, 31);
       }
-      left -= __shfl_sync(0xffffffffu, v, 31);
     }
+    if (lane < THREADS / 32) walks[lane] = w;
   }
   __syncthreads();
-  walk.b = walk.h = walk.i = walk.j = 0;
-  if (walk.u < walk.end) {
-    walk.b = start[0];
-    walk.h = start[1];
-    walk.i = start[2];
-    walk.j = start[3];
-    walk.q = load_request(p, walk.b);
-  }
-  return walk;
 }
 
 }  // namespace mtrtq

@@ -27,6 +27,8 @@
 // tokens see are taken out and listed; the epilogue adds them to the rows that see them.
 #include <math.h>
 
+#include <type_traits>
+
 #include "../../include/mtrtq.h"
 #include "attention_sched.cuh"
 #include "q8_common.cuh"
@@ -45,14 +47,20 @@ struct Cfg {
   static constexpr int STAGES = DP == 128 ? 4 : 8;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_PREFIX = OFF_KV + STAGES * TILE;
-  static constexpr int OFF_ML = OFF_PREFIX + (MTRTQ_MAX_BATCH + 1) * 8;  // slot 1's (m, l), then its rows
-  static constexpr int OFF_BAD = OFF_ML + kBlock * 8;                    // [2][2][kBadMax] keys
+  static constexpr int OFF_LIST = OFF_KV + STAGES * TILE;
+  static constexpr int OFF_WALK = OFF_LIST + StepList::bytes(MTRTQ_MAX_BATCH);
+  static constexpr int OFF_SEG = OFF_WALK + kThreads / 32 * ((sizeof(Walk) + 15) / 16 * 16);
+  static constexpr int OFF_ML = OFF_SEG + kThreads / 32 * ((sizeof(Segment) + 15) / 16 * 16);  // slot 1's (m, l)
+  static constexpr int OFF_BAD = OFF_ML + kBlock * 8;                                         // [2][2][kBadMax] keys
   static constexpr int OFF_BAR = OFF_BAD + 4 * kBadMax * 4;
-  static constexpr int NBAR = 3 * STAGES + 13;
+  static constexpr int NBAR = 3 * STAGES + 17;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 64 + 1024;
   static constexpr int COL_O = 256;
+  // One pair of exponentials in this many is a polynomial on the FMA units: the special
+  // function units alone would take as long as both products (128 dimensions) or twice
+  // as long (64).
+  static constexpr int POLY = DP == 128 ? 4 : 2;
   static_assert(BYTES <= 227 * 1024, "shared memory per CTA");
 };
 
@@ -112,6 +120,28 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Largest of three, NaN if any is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// 2^x for finite x <= 8, below 2^-126 rounded up to about that: x = n + f with n whole and
+// |f| <= 1/2, 2^f by the cubic with the least relative error (7.5e-5, an eighth of a bf16
+// rounding), n added to the exponent.
+__device__ __forceinline__ float2 exp2_cubic(float2 x) {
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 big = make_float2(12582912.0f, 12582912.0f), nbig = make_float2(-12582912.0f, -12582912.0f);
+  const float2 t = __fadd2_rn(x, big);  // n in the low bits
+  const float2 n = __fadd2_rn(t, nbig);
+  const float2 f = __fadd2_rn(x, make_float2(-n.x, -n.y));
+  float2 y = fma2(f, make_float2(0.0551716685f, 0.0551716685f), make_float2(0.2426111251f, 0.2426111251f));
+  y = fma2(y, f, make_float2(0.6932609677f, 0.6932609677f));
+  y = fma2(y, f, make_float2(0.9999280572f, 0.9999280572f));
+  return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(y.x)),
+                     __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(y.y)));
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -157,6 +187,42 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
   while (!mbar_try_wait(bar, parity) && clock64() - t0 < kSpinLimitCycles) {}
 }
 
+// One row of a cut tile from the parts of CTAs c_first .. c_last, in order.
+template <int DP>
+__device__ __noinline__ void join_parts(const TcAttention& p, int c_first, int c_last, int prow, __nv_bfloat16* out) {
+  const int64_t rows = p.part_rows;
+  float top = -INFINITY;
+  for (int c = c_first; c <= c_last; ++c)
+    top = fmaxf(top, __ldcg(p.part_ml + (c * 2 + (c == c_first)) * rows + prow).x);
+  float sum = 0.0f;
+  for (int c = c_first; c <= c_last; ++c) {
+    const float2 ml = __ldcg(p.part_ml + (c * 2 + (c == c_first)) * rows + prow);
+    if (ml.x != -INFINITY) sum += ml.y * (top == INFINITY ? 1.0f : ex2(ml.x - top));
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  for (int i = 0; i < p.head_dim; i += 8) {
+    float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int c = c_first; c <= c_last; ++c) {
+      const int64_t part = c * 2 + (c == c_first);
+      const float pm = __ldcg(p.part_ml + part * rows + prow).x;
+      if (pm == -INFINITY) continue;
+      const float w = top == INFINITY ? 1.0f : ex2(pm - top);
+      const float4* po = reinterpret_cast<const float4*>(p.partials) + part * rows * (DP / 4) + prow;
+      const float4 a = __ldcg(po + (i / 4) * rows), b = __ldcg(po + (i / 4 + 1) * rows);
+      o[0] += w * a.x;
+      o[1] += w * a.y;
+      o[2] += w * a.z;
+      o[3] += w * a.w;
+      o[4] += w * b.x;
+      o[5] += w * b.y;
+      o[6] += w * b.z;
+      o[7] += w * b.w;
+    }
+    *reinterpret_cast<uint4*>(out + i) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv),
+                                                    pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
+  }
+}
+
 // After a bounded wait gives up, every role goes on through its loops without waiting,
 // copying or multiplying (each wait returns at once), so that all reach the barriers
 // between them and the end.
@@ -168,44 +234,48 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int NH = DP / 64;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  int64_t* prefix = reinterpret_cast<int64_t*>(smem + C::OFF_PREFIX);
+  const StepList list(smem + C::OFF_LIST, MTRTQ_MAX_BATCH);
   float2* ml1 = reinterpret_cast<float2*>(smem + C::OFF_ML);
   int* bad = reinterpret_cast<int*>(smem + C::OFF_BAD);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* empty = full + C::STAGES;
   uint64_t* checked = empty + C::STAGES;
-  uint64_t* q_full = checked + C::STAGES;
-  uint64_t* q_free = q_full + 1;
-  uint64_t* s_full = q_free + 1;   // [2]
-  uint64_t* p_full = s_full + 2;   // [2]
-  uint64_t* o_full = p_full + 2;   // [2]
-  uint64_t* o_free = o_full + 2;   // [2]
-  uint64_t* list_free = o_free + 2;  // [2]
+  uint64_t* q_full = checked + C::STAGES;  // [2], a barrier for each slot or buffer
+  uint64_t* q_free = q_full + 2;
+  uint64_t* s_full = q_free + 2;
+  uint64_t* p_half = s_full + 2;           // the weights of the block's first 64 keys
+  uint64_t* p_full = p_half + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* o_free = o_full + 2;
+  uint64_t* list_free = o_free + 2;
   uint64_t* drained = list_free + 2;
   uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* s_abort = reinterpret_cast<volatile int*>(misc + 1);
   volatile unsigned* s_ticket = misc + 2;
   volatile int* bad_count = reinterpret_cast<volatile int*>(misc + 4);  // [2][2]
-  volatile int* s_start = reinterpret_cast<volatile int*>(misc + 8);    // b, h, i, j
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  Walk* walks = reinterpret_cast<Walk*>(smem + C::OFF_WALK);
+  Walk& walk = walks[warp];
+  Segment& s = reinterpret_cast<Segment*>(smem + C::OFF_SEG)[warp];
 
   if (tid == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 3);  // the products, two checking warps
-      mbar_init(&checked[s], 2);
+    for (int x = 0; x < C::STAGES; ++x) {
+      mbar_init(&full[x], 1);
+      mbar_init(&empty[x], 3);  // the products, two checking warps
+      mbar_init(&checked[x], 2);
     }
-    mbar_init(q_full, 1);
-    mbar_init(q_free, 1);
-    mbar_init(drained, 1);
     for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_free[t], 1);
       mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
       mbar_init(&o_free[t], 4);
       mbar_init(&list_free[t], 8);
     }
+    mbar_init(drained, 1);
     *s_abort = 0;
     for (int x = 0; x < 4; ++x) bad_count[x] = 0;
     fence_barrier_init();
@@ -220,109 +290,119 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&vmap);
   }
   tc_fence_before();
-  __syncthreads();
+  make_list<kBlock, kThreads>(p, list, walks);
   tc_fence_after();
   const uint32_t tmem = misc[0];
-  int64_t per;
-  const Walk<kBlock> walk0 = find_run<kBlock, kThreads>(p, prefix, s_start, per);
   // The kernel that stored the new keys and cast the rows is complete from here on.
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int ksteps = (p.head_dim + 15) / 16;
-  Segment s;
-  Walk<kBlock> walk = walk0;
 
   // 256 threads of 200 registers and 128 of 104: the 384 x 168 of the launch.
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------- softmax and epilogue ----------------
-    const int t = warp >> 2;          // slot
-    const int row = tid & 127;        // of the slot's tile
+    const int t = warp >> 2;                           // slot
+    const int row = tid & 127;                         // of the slot's tile
     const uint32_t quad = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp & 3) .. of TMEM
     const uint32_t s_addr = tmem + quad + t * kBlock, o_addr = tmem + quad + C::COL_O + t * DP;
     const int token = row / p.group, head = row - token * p.group;
     const float c2 = p.scale * 1.4426950408889634f;  // scale log2 e
+    const float2 cc = make_float2(c2, c2);
     uint32_t n_s = 0, n_o = 0;
-    int seg = 0;
-    for (; walk.next(p, s); ++seg) {
-      const bool pair = s.tile.pair;
-      const int k0 = pair ? s.j0 : 2 * s.j0;
-      const int n = (pair ? s.j1 : min(2 * s.j1, s.tile.blocks)) - k0;
-      const int tok = s.tile.t0 + (pair ? t * p.slot_tokens : 0) + token;
-      const bool live = token < p.slot_tokens && tok < s.tile.t0 + s.tile.tokens;
-      const int64_t seen = s.q.ctx + tok + 1;
-      const int keys = !live ? 0 : (int)max((int64_t)0, min(seen, (int64_t)s.q.keys));  // this row sees
-      int cnt;
-      if (pair && t == 0) {
-        const int64_t seen0 = s.q.ctx + s.tile.t0 + p.slot_tokens;
-        const int keys0 = (int)(seen0 < s.q.keys ? seen0 : s.q.keys);
-        cnt = max(0, min(s.j1, keys0 <= 0 ? 0 : (keys0 + kBlock - 1) / kBlock) - s.j0);
-      } else {
-        cnt = pair ? n : t == 0 ? (n + 1) >> 1 : n >> 1;
-      }
+    for (int seg = 0; next_segment<kBlock>(p, list, walk, s); ++seg) {
+      const int tok = (s.pair ? t * p.slot_tokens : 0) + token;  // of the tile's
+      const bool live = token < p.slot_tokens && tok < s.tokens;
+      const int keys = live ? max(0, min(s.see0 + tok, s.keys)) : 0;  // that this row sees
       const bool warp_live = __any_sync(0xffffffffu, live);
+      const int cnt = s.cnt[t], stride = s.pair ? kBlock : 2 * kBlock;
+      int left = keys - (s.k0 + (s.pair ? 0 : t)) * kBlock;  // columns of the block that it sees
       float m = -INFINITY, l = 0.0f;
-      for (int x = 0; x < cnt; ++x) {
-        const int key0 = (k0 + (pair ? x : 2 * x + t)) * kBlock;
+      for (int x = 0; x < cnt; ++x, left -= stride) {
         const bool ok = wait_all(&s_full[t], n_s & 1, s_abort, p.status);
         ++n_s;
-        if (ok && warp_live) {
-          tc_fence_after();
-          float v[kBlock];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + 32 * i, v + 32 * i);
-          tmem_wait_ld();
-          const int left = keys - key0;  // columns this row sees
-          if (__any_sync(0xffffffffu, left < kBlock)) {
-#pragma unroll
-            for (int i = 0; i < kBlock; ++i) v[i] = i < left ? v[i] : -INFINITY;
+        if (!ok || !warp_live) {
+          if (lane == 0) {
+            mbar_arrive(&p_half[t]);
+            mbar_arrive(&p_full[t]);
           }
-          float top = -INFINITY;
+          continue;
+        }
+        tc_fence_after();
+        float v[kBlock];
 #pragma unroll
-          for (int i = 0; i < kBlock; i += 2) top = fmaxf(top, fmaxf(v[i], v[i + 1]));
-          top *= c2;
-          const bool grow = top > m + 8.0f || (m == -INFINITY && top > m);
-          if (__any_sync(0xffffffffu, grow)) {
-            const float m1 = grow ? top : m;
-            const float keep = m1 == -INFINITY ? 1.0f : ex2(m - m1);
-            l *= keep;
-            m = m1;
-            if (x > 0) {
-              // this slot's earlier products are complete: their scores came after them
+        for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + 32 * i, v + 32 * i);
+        tmem_wait_ld();
+        if (__any_sync(0xffffffffu, left < kBlock)) {
+#pragma unroll
+          for (int i = 0; i < kBlock; ++i) v[i] = i < left ? v[i] : -INFINITY;
+        }
+        float top = max3(v[0], v[1], v[2]), top1 = max3(v[3], v[4], v[5]);
+#pragma unroll
+        for (int i = 6; i + 3 < kBlock; i += 4) {
+          top = max3(top, v[i], v[i + 1]);
+          top1 = max3(top1, v[i + 2], v[i + 3]);
+        }
+        top = max3(top, top1, max3(v[kBlock - 2], v[kBlock - 1], top1)) * c2;
+        // Masked, infinite or NaN scores: every exponential by the instruction, which
+        // keeps them exact.
+        const bool exact = __any_sync(0xffffffffu, left < kBlock || !(fabsf(top) < INFINITY));
+        const bool grow = top > m + 8.0f || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m1 = grow ? top : m;
+          const float keep = m1 == -INFINITY ? 1.0f : ex2(m - m1);
+          l *= keep;
+          m = m1;
+          if (x > 0) {
+            // this slot's earlier products are complete: their scores came after them
 #pragma unroll 1
-              for (int i = 0; i < DP; i += 16) {
-                uint32_t o[16];
-                tmem_ld_32x32b_x16(o_addr + i, o);
-                tmem_wait_ld();
+            for (int i = 0; i < DP; i += 16) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(o_addr + i, o);
+              tmem_wait_ld();
 #pragma unroll
-                for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * keep);
-                tmem_st16(o_addr + i, o);
-              }
+              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * keep);
+              tmem_st16(o_addr + i, o);
             }
           }
-          const float base = m == -INFINITY ? 0.0f : m;
-          float2 sum = make_float2(0.0f, 0.0f);
-          const float2 cc = make_float2(c2, c2), mm = make_float2(-base, -base);
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float2 sum = make_float2(0.0f, 0.0f);
+        const float2 mm = make_float2(-base, -base);
+        auto weights = [&](auto some_cubic) {
 #pragma unroll
           for (int i = 0; i < kBlock; i += 32) {
             uint32_t w[16];
 #pragma unroll
             for (int y = 0; y < 16; ++y) {
               float2 e = fma2(make_float2(v[i + 2 * y], v[i + 2 * y + 1]), cc, mm);
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
+              if (decltype(some_cubic)::value && y % C::POLY == C::POLY - 1) {
+                e = exp2_cubic(e);
+              } else {
+                e.x = ex2(e.x);
+                e.y = ex2(e.y);
+              }
               sum = __fadd2_rn(sum, e);
               w[y] = pack_bf16(e.x, e.y);
             }
             tmem_st16(s_addr + (i >> 1), w);
+            if (i == kBlock / 2 - 32) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_half[t]);
+            }
           }
-          l += sum.x + sum.y;
-          tmem_wait_st();
-          tc_fence_before();
-        }
+        };
+        if (exact) weights(std::false_type());
+        else weights(std::true_type());
+        tmem_wait_st();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
+        l += sum.x + sum.y;
       }
+
       if (m == -INFINITY && l != l) m = 0.0f;  // every score it saw was NaN
       bool ok = true;
       if (cnt > 0) {
@@ -330,49 +410,76 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++n_o;
         tc_fence_after();
       }
-      // The V rows taken out of the last blocks (the epilogue of a whole tile or of the
-      // CTA that joins one adds them; they are the same in every part that has them).
-      const int par = seg & 1;
-      const int64_t t0_sees = s.q.ctx + s.tile.t0 + 1;
-      // A slot without blocks here has not waited for the check, and sees none of it.
-      const bool any_checked = cnt > 0 && (int64_t)(k0 + n) * kBlock > min(t0_sees, (int64_t)s.q.keys);
-      float other_m = -INFINITY, other_l = 0.0f;
-      bool mine = pair || t == 0;  // this thread finishes its row
-      if (!pair) {
-        if (t == 1) ml1[row] = cnt > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.0f);
+      // halves: slot 0's threads join the two slots' rows
+      const bool mine = s.pair || t == 0, two = !s.pair && s.n > 1;
+      float w0 = 1.0f, w1 = 0.0f;
+      if (!s.pair) {
+        if (t == 1) ml1[row] = make_float2(m, l);
         tc_fence_before();
         named_bar_sync(1, 256);
         tc_fence_after();
-        if (t == 0) {
-          other_m = ml1[row].x;
-          other_l = ml1[row].y;
+        if (two && t == 0) {
+          const float2 ml = ml1[row];
+          const float top = fmaxf(m, ml.x);
+          w0 = m == -INFINITY ? 0.0f : top == INFINITY ? 1.0f : ex2(m - top);
+          w1 = ml.x == -INFINITY ? 0.0f : top == INFINITY ? 1.0f : ex2(ml.x - top);
+          l = l * w0 + ml.y * w1;
+          m = top;
         }
       }
-      const bool two = !pair && n > 1;  // slot 1 has products too
-      const float top = fmaxf(m, other_m);
-      float w0 = m == -INFINITY ? 0.0f : ex2(m - top), w1 = other_m == -INFINITY ? 0.0f : ex2(other_m - top);
-      if (top == INFINITY) w0 = w1 = 1.0f;  // sums and products are NaN by then
-      const float lsum = l * w0 + other_l * w1;
-      const bool whole = s.whole();
-      const int64_t out_at = (s.q.r0 + tok) * p.out_row + (int64_t)(s.h * p.group + head) * p.out_head;
-      const int rows_cap = p.part_rows;
-      // Columns [i, i + 32) of this row's products, joined over the slots, with the
-      // infinities and NaN that were taken out.
-      auto columns = [&](int i, float* o) {
-        if (cnt > 0) {
-          tmem_ld32(o_addr + i, o);
-          tmem_wait_ld();
+      if (m == -INFINITY) w0 = 0.0f;  // no key seen (and perhaps no product formed)
+      const int prow = (s.pair ? t * kBlock : 0) + row;
+      const int64_t at_out =
+          (int64_t)(s.row0 + tok) * p.out_row + (int64_t)(s.h * p.group + head) * p.out_head;
+      const int64_t part = (int64_t)blockIdx.x * 2 + s.part;
+      float* to_part = p.partials + (part * p.part_rows * (DP / 4) + prow) * 4;
+      if (mine && ok) {
+        if (s.whole) {
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          w0 *= inv;
+          w1 *= inv;
         }
+#pragma unroll 1
+        for (int i = 0; i < p.head_dim; i += 32) {
+          float o[32];
+          if (cnt > 0) {
+            tmem_ld32(o_addr + i, o);
+            tmem_wait_ld();
+          }
 #pragma unroll
-        for (int y = 0; y < 32; ++y) o[y] = w0 == 0.0f ? 0.0f : o[y] * w0;
-        if (two) {
-          float o1[32];
-          tmem_ld32(o_addr + DP + i, o1);
-          tmem_wait_ld();
+          for (int y = 0; y < 32; ++y) o[y] = w0 == 0.0f ? 0.0f : o[y] * w0;
+          if (two) {
+            float o1[32];
+            tmem_ld32(o_addr + DP + i, o1);
+            tmem_wait_ld();
+            if (w1 != 0.0f) {
 #pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] += w1 == 0.0f ? 0.0f : o1[y] * w1;
+              for (int y = 0; y < 32; ++y) o[y] = fmaf(o1[y], w1, o[y]);
+            }
+          }
+          if (live) {
+            if (s.whole) {
+#pragma unroll
+              for (int y = 0; y < 32; y += 8) {
+                if (i + y < p.head_dim)
+                  *reinterpret_cast<uint4*>(p.out + at_out + i + y) =
+                      make_uint4(pack_bf16(o[y], o[y + 1]), pack_bf16(o[y + 2], o[y + 3]),
+                                 pack_bf16(o[y + 4], o[y + 5]), pack_bf16(o[y + 6], o[y + 7]));
+              }
+            } else {
+#pragma unroll
+              for (int y = 0; y < 32; y += 4)
+                __stcg(reinterpret_cast<float4*>(to_part + (int64_t)(i + y) * p.part_rows),
+                       make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]));
+            }
+          }
         }
-        if (any_checked) {
+        if (live && !s.whole) __stcg(p.part_ml + part * p.part_rows + prow, make_float2(m, l));
+        // The infinities and NaN that were taken out of the last blocks' V, for the rows
+        // that see them. A slot without blocks here has not waited for the check, and
+        // sees none of it.
+        const int par = seg & 1;
+        if (cnt > 0 && (s.k0 + s.n) * kBlock > s.all_see()) {
           for (int w = 0; w < 2; ++w) {
             const int have = min(kBadMax, bad_count[par * 2 + w]);
             for (int x = 0; x < have; ++x) {
@@ -383,51 +490,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int64_t page = p.table[s.b * p.table_ld + key / p.page_size];
                 src = p.v + page * p.v_row + ((int64_t)s.h * p.page_size + key % p.page_size) * p.head_dim;
               } else {
-                src = p.v + (s.q.r0 + key) * p.v_row + s.h * p.v_head;
+                src = p.v + (int64_t)(list.req[s.b].r0 + key) * p.v_row + s.h * p.v_head;
               }
-              for (int y = 0; y < 32 && i + y < p.head_dim; ++y) {
-                const float z = __bfloat162float(src[i + y]);
-                if (!(fabsf(z) < INFINITY)) {
-#pragma unroll
-                  for (int q = 0; q < 32; ++q)
-                    if (q == y) o[q] += z;
+              for (int d = 0; d < p.head_dim; ++d) {
+                const float z = __bfloat162float(src[d]);
+                if (fabsf(z) < INFINITY) continue;
+                if (s.whole) {
+                  p.out[at_out + d] = __float2bfloat16_rn(__bfloat162float(p.out[at_out + d]) + z);
+                } else {
+                  float* to = to_part + (int64_t)(d & ~3) * p.part_rows + (d & 3);
+                  __stcg(to, __ldcg(to) + z);
                 }
               }
             }
           }
         }
-      };
-      if (mine && ok && whole) {
-        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-#pragma unroll
-        for (int i = 0; i < DP; i += 32) {
-          float o[32];
-          columns(i, o);
-          if (live) {
-#pragma unroll
-            for (int y = 0; y < 32; y += 8) {
-              if (i + y < p.head_dim)
-                *reinterpret_cast<uint4*>(p.out + out_at + i + y) =
-                    make_uint4(pack_bf16(o[y] * inv, o[y + 1] * inv), pack_bf16(o[y + 2] * inv, o[y + 3] * inv),
-                               pack_bf16(o[y + 4] * inv, o[y + 5] * inv), pack_bf16(o[y + 6] * inv, o[y + 7] * inv));
-            }
-          }
-        }
-      } else if (mine && ok) {
-        const int prow = (pair ? t * kBlock : 0) + row;
-        const int64_t part = (int64_t)blockIdx.x * 2 + (s.j0 > 0 ? 0 : 1);
-        float4* po = reinterpret_cast<float4*>(p.partials) + part * rows_cap * (DP / 4);
-#pragma unroll
-        for (int i = 0; i < DP; i += 32) {
-          float o[32];
-          columns(i, o);
-          if (live) {
-#pragma unroll
-            for (int y = 0; y < 32; y += 4)
-              __stcg(po + (int64_t)((i + y) / 4) * rows_cap + prow, make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]));
-          }
-        }
-        if (live) __stcg(p.part_ml + part * rows_cap + prow, make_float2(top, lsum));
       }
       // O and the list have been read.
       tc_fence_before();
@@ -435,158 +512,115 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         if (mine && cnt > 0) mbar_arrive(&o_free[t]);
         if (two && t == 0) mbar_arrive(&o_free[1]);
-        mbar_arrive(&list_free[par]);
+        mbar_arrive(&list_free[seg & 1]);
       }
-      if (!pair) named_bar_sync(2, 256);  // ml1 has been read
-      if (!whole && mine) {
-        const int id = pair ? 3 : 4, count = pair ? 256 : 128;
-        const int64_t c_first = s.first / per, c_last = (s.first + s.tile.steps - 1) / per;
+      if (!s.pair) named_bar_sync(2, 256);  // ml1 has been read
+      if (!s.whole && mine) {
+        const int id = s.pair ? 3 : 4, count = s.pair ? 256 : 128;
         named_bar_sync(id, count);
-        if (tid == 0) *s_ticket = ticket_acq_rel(p.counters + c_first);
+        if (tid == 0) *s_ticket = ticket_acq_rel(p.counters + s.c_first);
         named_bar_sync(id, count);
-        const bool last = *s_ticket == (unsigned)(c_last - c_first);
-        if (last && live) {
-          const int prow = (pair ? t * kBlock : 0) + row;
-          float mx = -INFINITY;
-          for (int64_t c = c_first; c <= c_last; ++c)
-            mx = fmaxf(mx, __ldcg(p.part_ml + (c * 2 + (c == c_first ? 1 : 0)) * rows_cap + prow).x);
-          float sum = 0.0f;
-          for (int64_t c = c_first; c <= c_last; ++c) {
-            const float2 ml = __ldcg(p.part_ml + (c * 2 + (c == c_first ? 1 : 0)) * rows_cap + prow);
-            if (ml.x != -INFINITY) sum += ml.y * (mx == INFINITY ? 1.0f : ex2(ml.x - mx));
-          }
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          for (int i = 0; i < p.head_dim; i += 8) {
-            float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            for (int64_t c = c_first; c <= c_last; ++c) {
-              const int64_t part = c * 2 + (c == c_first ? 1 : 0);
-              const float pm = __ldcg(p.part_ml + part * rows_cap + prow).x;
-              if (pm == -INFINITY) continue;
-              const float w = mx == INFINITY ? 1.0f : ex2(pm - mx);
-              const float4* po = reinterpret_cast<const float4*>(p.partials) + part * rows_cap * (DP / 4);
-              const float4 a = __ldcg(po + (int64_t)(i / 4) * rows_cap + prow);
-              const float4 b = __ldcg(po + (int64_t)(i / 4 + 1) * rows_cap + prow);
-              o[0] += w * a.x;
-              o[1] += w * a.y;
-              o[2] += w * a.z;
-              o[3] += w * a.w;
-              o[4] += w * b.x;
-              o[5] += w * b.y;
-              o[6] += w * b.z;
-              o[7] += w * b.w;
-            }
-            *reinterpret_cast<uint4*>(p.out + out_at + i) =
-                make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv),
-                           pack_bf16(o[4] * inv, o[5] * inv), pack_bf16(o[6] * inv, o[7] * inv));
-          }
-        }
-        if (last && tid == 0) p.counters[c_first] = 0u;
+        const bool last = *s_ticket == (unsigned)(s.c_last - s.c_first);
+        if (last && live) join_parts<DP>(p, s.c_first, s.c_last, prow, p.out + at_out);
+        if (last && tid == 0) p.counters[s.c_first] = 0u;
       }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 8) {
       // ---------------- loads ----------------
-      uint32_t seq = 0, sent = 0, q_sent = 0;
-      int seg = 0;
+      uint32_t seq = 0, sent = 0;
+      int q_sent[2] = {0, 0};
       const int pages = PAGED ? kBlock / p.page_size : 1;
       const uint32_t box = (PAGED ? p.page_size : kBlock) * 128;
-      for (; walk.next(p, s); ++seg) {
-        if (wait_all(q_free, (seg & 1) ^ 1, s_abort, p.status)) {
-          const int slots = s.tile.pair ? 2 : 1;
-          const uint32_t rows_bytes = (uint32_t)p.slot_tokens * p.group * 128;
-          ++q_sent;
-          if (lane == 0) mbar_arrive_expect_tx(q_full, rows_bytes * NH * slots);
+      const uint32_t rows_bytes = (uint32_t)p.slot_tokens * p.group * 128 * NH;
+      while (next_segment<kBlock>(p, list, walk, s)) {
+        const int k0 = s.k0, n = s.n;
+        const bool pair = s.pair;
+        for (int t = 0; t < (pair ? 2 : 1); ++t) {
+          const int buf = pair ? t : s.buf;
+          if (!wait_all(&q_free[buf], (s.q_use[buf] & 1) ^ 1, s_abort, p.status)) continue;
+          ++q_sent[buf];
+          if (lane == 0) mbar_arrive_expect_tx(&q_full[buf], rows_bytes);
           __syncwarp();
-          if (lane < slots * NH) {
-            const int t = lane / NH, half = lane % NH;
-            tma_load_4d(smem + C::OFF_Q + t * C::TILE + half * kBlock * 128, &qmap, half * 64, 0, s.h,
-                        (int)s.q.r0 + s.tile.t0 + t * p.slot_tokens, q_full);
-          }
+          if (lane < NH)
+            tma_load_4d(smem + C::OFF_Q + buf * C::TILE + lane * kBlock * 128, &qmap, lane * 64, 0, s.h,
+                        s.row0 + t * p.slot_tokens, &q_full[buf]);
         }
-        const int k0 = s.tile.pair ? s.j0 : 2 * s.j0;
-        const int n = (s.tile.pair ? s.j1 : min(2 * s.j1, s.tile.blocks)) - k0;
+        const int r0 = PAGED ? 0 : list.req[s.b].r0;
         for (int at = 0; at < 2 * n; ++at, ++seq) {
           int c;
-          const bool is_v = nth_load(s.tile.pair, at, n, c);
+          const bool is_v = nth_load(pair, at, n, c);
           const int st = seq % C::STAGES;
           const int key0 = (k0 + c) * kBlock;
           const int pg = lane % pages, half = lane / pages;
-          bool mine = lane < pages * NH;
+          bool load = lane < pages * NH;
           int page = 0;
           if (PAGED) {
-            const int col = (k0 + c) * pages + pg;
-            mine = mine && key0 + pg * p.page_size < s.q.keys;
-            if (mine) page = p.table[s.b * p.table_ld + col];
+            load = load && key0 + pg * p.page_size < s.keys;
+            if (load) page = p.table[s.b * p.table_ld + (k0 + c) * pages + pg];
           }
           if (!wait_all(&empty[st], ((seq / C::STAGES) & 1) ^ 1, s_abort, p.status)) continue;
           sent = seq + 1;
-          const unsigned who = __ballot_sync(0xffffffffu, mine);
+          const unsigned who = __ballot_sync(0xffffffffu, load);
           if (lane == 0) mbar_arrive_expect_tx(&full[st], box * __popc(who));
           __syncwarp();
-          if (mine) {
+          if (load) {
             uint8_t* dst = smem + C::OFF_KV + st * C::TILE + half * kBlock * 128 + (PAGED ? pg * box : 0);
             if (PAGED)
               tma_load_3d(dst, is_v ? &vmap : &kmap, half * 64, s.h * p.page_size, page, &full[st]);
             else
-              tma_load_3d(dst, is_v ? &vmap : &kmap, half * 64, s.h, (int)s.q.r0 + key0, &full[st]);
+              tma_load_3d(dst, is_v ? &vmap : &kmap, half * 64, s.h, r0 + key0, &full[st]);
           }
         }
       }
       // No copy may be in flight when the CTA exits: without an abort the products have
       // waited for every one.
       if (*s_abort && lane == 0) {
-        if (q_sent) drain(q_full, (q_sent - 1) & 1);
+        for (int t = 0; t < 2; ++t)
+          if (q_sent[t]) drain(&q_full[t], (q_sent[t] - 1) & 1);
         for (uint32_t x = sent > C::STAGES ? sent - C::STAGES : 0; x < sent; ++x)
           drain(&full[x % C::STAGES], (x / C::STAGES) & 1);
       }
       __syncwarp();
     } else if (warp == 9) {
       // ---------------- products ----------------
-      if (lane == 0) {
-        const uint32_t idesc_s = umma_idesc_bf16(kBlock, kBlock);
-        const uint32_t idesc_o = umma_idesc_bf16(kBlock, ksteps * 16) | (1u << 16);  // B is contiguous along N
-        uint32_t base = 0, fixed = 0;  // loads so far; phase of each stage's check
-        uint32_t n_p[2] = {0, 0}, n_seg[2] = {0, 0};
-        int seg = 0;
-        const uint32_t q_addr = smem_u32(smem + C::OFF_Q), kv_addr = smem_u32(smem + C::OFF_KV);
-        auto wait_load = [&](uint32_t at) {
-          return wait_one(&full[at % C::STAGES], (at / C::STAGES) & 1, s_abort, p.status);
-        };
-        for (; walk.next(p, s); ++seg) {
-          const bool pair = s.tile.pair;
-          const int k0 = pair ? s.j0 : 2 * s.j0;
-          const int n = (pair ? s.j1 : min(2 * s.j1, s.tile.blocks)) - k0;
-          int cnt[2];  // blocks of each slot
-          if (pair) {
-            const int64_t seen = s.q.ctx + s.tile.t0 + p.slot_tokens;
-            const int keys0 = (int)(seen < s.q.keys ? seen : s.q.keys);
-            const int blocks0 = keys0 <= 0 ? 0 : (keys0 + kBlock - 1) / kBlock;
-            cnt[0] = max(0, min(s.j1, blocks0) - s.j0);
-            cnt[1] = n;
-          } else {
-            cnt[0] = (n + 1) >> 1;
-            cnt[1] = n >> 1;
-          }
-          const int64_t t0_sees = s.q.ctx + s.tile.t0 + 1;
-          const int64_t all_see = t0_sees < s.q.keys ? t0_sees : s.q.keys;  // keys that every row sees
+      const uint32_t idesc_s = umma_idesc_bf16(kBlock, kBlock);
+      const uint32_t idesc_o = umma_idesc_bf16(kBlock, ksteps * 16) | (1u << 16);  // B is contiguous along N
+      const uint32_t q_addr = smem_u32(smem + C::OFF_Q), kv_addr = smem_u32(smem + C::OFF_KV);
+      uint32_t base = 0, fixed = 0;  // loads so far; phase of each stage's check
+      uint32_t n_p[2] = {0, 0}, n_seg[2] = {0, 0};
+      while (next_segment<kBlock>(p, list, walk, s)) {
+        if (lane == 0) {
+          const bool pair = s.pair;
+          const int n = s.n, k0 = s.k0, all_see = s.all_see();
+          const int cnt[2] = {s.cnt[0], s.cnt[1]};
           auto block_of = [&](int t, int x) { return pair ? x : 2 * x + t; };
+          auto wait_load = [&](uint32_t at) {
+            return wait_one(&full[at % C::STAGES], (at / C::STAGES) & 1, s_abort, p.status);
+          };
           auto scores = [&](int t, int x) {
-            const int c = block_of(t, x);
+            const int c = block_of(t, x), buf = pair ? t : s.buf;
             const uint32_t at = base + order_k(pair, c);
             if (!wait_load(at)) return;
             tc_fence_after();
-            const uint32_t k = kv_addr + (at % C::STAGES) * C::TILE, q = q_addr + (pair ? t : 0) * C::TILE;
+            const uint32_t k = kv_addr + (at % C::STAGES) * C::TILE, q = q_addr + buf * C::TILE;
             for (int i = 0; i < ksteps; ++i) {
               const uint32_t off = (i >> 2) * kBlock * 128 + (i & 3) * 32;
               umma_ss(tmem + t * kBlock, umma_desc_sw128(q + off), umma_desc_sw128(k + off), idesc_s, i > 0);
             }
             umma_commit(&s_full[t]);
             if (!pair || t == 1) umma_commit(&empty[at % C::STAGES]);
+            if (pair ? x == cnt[t] - 1 : c == n - 1) umma_commit(&q_free[buf]);
           };
-          bool ok = wait_one(q_full, seg & 1, s_abort, p.status);
+          bool ok = true;
+          for (int t = 0; t < (pair ? 2 : 1); ++t) {
+            const int buf = pair ? t : s.buf;
+            ok = wait_one(&q_full[buf], s.q_use[buf] & 1, s_abort, p.status) && ok;
+          }
           for (int t = 0; t < 2; ++t)
             if (ok && cnt[t] > 0) scores(t, 0);
+          if (pair && cnt[0] == 0) umma_commit(&q_free[0]);
           uint32_t was_checked = 0;  // pair: slot 0 has waited for this stage's check
           for (int x = 0; x < max(cnt[0], cnt[1]); ++x) {
             for (int t = 0; t < 2; ++t) {
@@ -595,18 +629,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint32_t at = base + order_v(pair, c, n), st = at % C::STAGES;
               if (x == 0) wait_one(&o_free[t], (n_seg[t] & 1) ^ 1, s_abort, p.status);
               wait_load(at);
-              if ((int64_t)(k0 + c + 1) * kBlock > all_see && !(pair && t == 1 && (was_checked >> st & 1))) {
+              if ((k0 + c + 1) * kBlock > all_see && !(pair && t == 1 && (was_checked >> st & 1))) {
                 wait_one(&checked[st], fixed >> st & 1, s_abort, p.status);
                 fixed ^= 1u << st;
                 was_checked |= 1u << st;
               }
-              wait_one(&p_full[t], n_p[t] & 1, s_abort, p.status);
+              const uint32_t v = kv_addr + st * C::TILE;
+              for (int half = 0; half < 2; ++half) {
+                wait_one(half ? &p_full[t] : &p_half[t], n_p[t] & 1, s_abort, p.status);
+                if (*s_abort) break;
+                tc_fence_after();
+#pragma unroll
+                for (int i = half * 4; i < half * 4 + 4; ++i)
+                  umma_ts(tmem + C::COL_O + t * DP, tmem + t * kBlock + i * 8, desc_v(v + i * 2048), idesc_o,
+                          x > 0 || i > 0);
+              }
               ++n_p[t];
               if (*s_abort) continue;
-              tc_fence_after();
-              const uint32_t v = kv_addr + st * C::TILE;
-              for (int i = 0; i < kBlock / 16; ++i)
-                umma_ts(tmem + C::COL_O + t * DP, tmem + t * kBlock + i * 8, desc_v(v + i * 2048), idesc_o, x > 0 || i > 0);
               if (!pair || t == 1) {
                 umma_commit(&empty[st]);
                 was_checked &= ~(1u << st);
@@ -615,30 +654,24 @@ __global__ void __launch_bounds__(kThreads, 1)
               else umma_commit(&o_full[t]);
             }
           }
-          // Q is free once the last scores are done; later commits only come after them.
-          umma_commit(q_free);
           for (int t = 0; t < 2; ++t)
             if (cnt[t] > 0) ++n_seg[t];
           base += 2 * n;
         }
-        if (*s_abort) {  // the products in flight end before TMEM is freed
-          umma_commit(drained);
-          drain(drained, 0);
-        }
+        __syncwarp();
+      }
+      if (lane == 0 && *s_abort) {  // the products in flight end before TMEM is freed
+        umma_commit(drained);
+        drain(drained, 0);
       }
       __syncwarp();
-    } else if (warp >= 10) {
+    } else {
       // ---------------- V blocks that not every row sees whole ----------------
       const int w = warp - 10;
       uint32_t base = 0;
-      int seg = 0;
-      for (; walk.next(p, s); ++seg) {
-        const bool pair = s.tile.pair;
-        const int k0 = pair ? s.j0 : 2 * s.j0;
-        const int n = (pair ? s.j1 : min(2 * s.j1, s.tile.blocks)) - k0;
-        const int64_t t0_sees = s.q.ctx + s.tile.t0 + 1;
-        const int64_t all_see = t0_sees < s.q.keys ? t0_sees : s.q.keys;
-        const int par = seg & 1;
+      for (int seg = 0; next_segment<kBlock>(p, list, walk, s); ++seg) {
+        const bool pair = s.pair;
+        const int n = s.n, k0 = s.k0, keys = s.keys, all_see = s.all_see(), par = seg & 1;
         bool first = true;
         for (int x = 0; x < 2 * n; ++x) {
           int c;
@@ -647,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t at = base + x, st = at % C::STAGES;
           // every load is followed, so that no phase of its barrier is taken for another
           const bool landed = wait_all(&full[st], (at / C::STAGES) & 1, s_abort, p.status);
-          if (!is_v || (int64_t)key0 + kBlock <= all_see) {
+          if (!is_v || key0 + kBlock <= all_see) {
             if (lane == 0) mbar_arrive(&empty[st]);
             continue;
           }
@@ -659,24 +692,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (landed) {
             uint8_t* v = smem + C::OFF_KV + st * C::TILE;
-  #pragma unroll
+#pragma unroll
             for (int rr = 0; rr < 2; ++rr) {
               const int r = w * 64 + rr * 32 + lane;
-              const bool live = key0 + r < s.q.keys;
+              const bool kept = key0 + r < keys;
               bool broken = false;
-              for (int x = 0; x < NH * 8; ++x) {
-                uint4* at16 = reinterpret_cast<uint4*>(v + (x >> 3) * kBlock * 128 + r * 128 + (((x & 7) ^ (r & 7)) << 4));
-                if (!live) {
+              for (int y = 0; y < NH * 8; ++y) {
+                uint4* at16 =
+                    reinterpret_cast<uint4*>(v + (y >> 3) * kBlock * 128 + r * 128 + (((y & 7) ^ (r & 7)) << 4));
+                if (!kept) {
                   *at16 = make_uint4(0, 0, 0, 0);
                   continue;
                 }
                 uint4 u = *at16;
                 uint32_t* e = reinterpret_cast<uint32_t*>(&u);
                 bool hit = false;
-  #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                  if ((e[y] & 0x7f80u) == 0x7f80u) { e[y] &= 0xffff0000u; hit = true; }
-                  if ((e[y] & 0x7f800000u) == 0x7f800000u) { e[y] &= 0xffffu; hit = true; }
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                  if ((e[z] & 0x7f80u) == 0x7f80u) { e[z] &= 0xffff0000u; hit = true; }
+                  if ((e[z] & 0x7f800000u) == 0x7f800000u) { e[z] &= 0xffffu; hit = true; }
                 }
                 if (hit) *at16 = u;
                 broken |= hit;
