@@ -21,12 +21,14 @@ struct AttentionList {
   int tile_tokens;
   int64_t max_keys;   // paged: tokens the table's columns hold
   int64_t min_steps;  // fewest steps worth a CTA
+  int tile_cost;      // steps that a tile takes besides its own
 };
 
 struct TcAttention : AttentionList {
   float scale;
   __nv_bfloat16* out;
   int64_t out_row, out_head;
+  bool out32;  // rows of out start on 32 bytes
   const __nv_bfloat16* v;  // as the tensor map has it, for values taken out of a block
   int64_t v_row, v_head;   // paged: v_row is the page stride
   unsigned* counters;      // [grid] tickets, zero

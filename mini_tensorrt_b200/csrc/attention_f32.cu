@@ -55,22 +55,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
   extern __shared__ float4 raw4[];
   float* sm = reinterpret_cast<float*>(raw4);
   float *qs = sm + C::OFF_Q, *ks = sm + C::OFF_K, *vs = sm + C::OFF_V, *ps = sm + C::OFF_P;
-  const StepList list(sm + C::FLOATS, p.batch);
-  __shared__ Walk walks[kThreads / 32];
-  __shared__ Segment segments[kThreads / 32];
+  const StepList list = {reinterpret_cast<Request*>(sm + C::FLOATS), reinterpret_cast<int64_t*>(sm)};  // the prefix lies where Q will
+  __shared__ Walk shared_walk;
+  __shared__ Segment s;
+  __shared__ int more;
   __shared__ unsigned ticket;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, lane = tid & 31, warp = tid >> 5;
 
-  make_list<kKeys, kThreads>(p, list, walks);
+  Walk walk;
+  make_list<kKeys, kThreads>(p, list, walk, &shared_walk);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float c2 = p.scale * 1.4426950408889634f;  // scale log2 e
 
-  Segment& s = segments[warp];
-  while (next_segment<kKeys>(p, list, walks[warp], s)) {
-    const int64_t r0 = list.req[s.b].r0;  // where the request's rows start
+  while (true) {
+    __syncthreads();
+    if (tid == 0) more = next_segment<kKeys>(p, list, walk, s);
+    __syncthreads();
+    if (!more) break;
+    const int64_t r0 = s.r0;  // where the request's rows start
     const int tokens = s.tokens, keys = s.keys;
     // Q, transposed; rows past the tile's tokens and dimensions past the head's are zero.
-    __syncthreads();
     for (int e = tid; e < C::BM * (HD / 4); e += kThreads) {
       const int row = e % C::BM, d = e / C::BM * 4;
       const int token = row / p.group, head = row - token * p.group;
@@ -326,13 +330,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
 template <int HD, int RM, bool PAGED>
 cudaError_t launch_one(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
   auto kernel = attention_f32_kernel<HD, RM, PAGED>;
-  constexpr int most = Cfg<HD, RM>::BYTES + StepList::bytes(MTRTQ_MAX_BATCH);
-  static_assert(most + 3 * 1024 <= 227 * 1024, "shared memory per CTA");
+  using C = Cfg<HD, RM>;
+  constexpr int most = C::BYTES + MTRTQ_MAX_BATCH * (int)sizeof(Request);
+  static_assert(most + 3 * 1024 <= 227 * 1024 && C::BYTES >= (MTRTQ_MAX_BATCH + 1) * 8, "shared memory per CTA");
   if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kernel), most)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<HD, RM>::BYTES + StepList::bytes(p.batch);
+  cfg.dynamicSmemBytes = Cfg<HD, RM>::BYTES + p.batch * (int)sizeof(Request);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

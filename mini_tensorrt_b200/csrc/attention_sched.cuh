@@ -18,11 +18,10 @@ struct Request {
   int r0, m, ctx, keys;
 };
 
-// What a role needs to know of its next run of one tile's steps. Every warp keeps its own
-// walk and segment in shared memory, out of the registers.
+// A CTA's next run of one tile's steps: what its roles need to know of it.
 struct Segment {
   int b, h;
-  int row0;        // the tile's first row
+  int r0, row0;    // the request's first row, the tile's
   int tokens;      // its tokens
   int see0;        // keys that the first row sees, if the request has them
   int keys;        // keys the request has
@@ -44,11 +43,8 @@ struct Walk {
 };
 
 struct StepList {
-  Request* req;
-  int64_t* prefix;  // steps before each request
-  static constexpr int bytes(int batch) { return batch * (int)sizeof(Request) + (batch + 2) / 2 * 16; }
-  __device__ StepList(void* shared, int batch)
-      : req(static_cast<Request*>(shared)), prefix(reinterpret_cast<int64_t*>(req + batch)) {}
+  Request* req;     // [batch]
+  int64_t* prefix;  // [batch + 1] steps before each request, while the list is made
 };
 
 __device__ __forceinline__ Request load_request(const AttentionList& p, int b) {
@@ -77,60 +73,51 @@ template <int BLOCK>
 __device__ __forceinline__ int tile_steps(const AttentionList& p, const Request& q, int i) {
   const int t0 = i * p.tile_tokens, tokens = min(p.tile_tokens, q.m - t0);
   const int blocks = block_count<BLOCK>(q, t0, tokens);
-  return tokens > p.slot_tokens ? blocks : (blocks + 1) >> 1;
+  return p.tile_cost + (tokens > p.slot_tokens ? blocks : (blocks + 1) >> 1);
 }
 
-// The whole warp calls it; false at the end of the CTA's run.
+// One thread's; false at the end of the CTA's run. A tile counts p.tile_cost steps more
+// than it has: what starting and ending it takes.
 template <int BLOCK>
 __device__ bool next_segment(const AttentionList& p, const StepList list, Walk& w, Segment& s) {
-  int more = 0;
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0 && w.u < w.end) {
-    more = 1;
+#pragma unroll 1
+  while (w.u < w.end) {
     const Request q = list.req[w.b];
     const int t0 = w.i * p.tile_tokens, tokens = min(p.tile_tokens, q.m - t0);
     const int blocks = block_count<BLOCK>(q, t0, tokens);
     const bool pair = tokens > p.slot_tokens;
     const int steps = pair ? blocks : (blocks + 1) >> 1;
-    const int take = (int)min((int64_t)(steps - w.j), w.end - w.u), j1 = w.j + take;
+    const int64_t first = w.u - w.j;  // of the tile's
+    const int cost = steps + p.tile_cost;
+    const int take = (int)min((int64_t)(cost - w.j), w.end - w.u);
+    const int j0 = max(0, w.j - p.tile_cost), j1 = max(0, w.j + take - p.tile_cost);
     s.b = w.b;
     s.h = w.h;
+    s.r0 = q.r0;
     s.row0 = q.r0 + t0;
     s.tokens = tokens;
     s.see0 = q.ctx + t0 + 1;
     s.keys = q.keys;
     s.pair = pair;
-    s.k0 = pair ? w.j : 2 * w.j;
+    s.k0 = pair ? j0 : 2 * j0;
     s.n = (pair ? j1 : min(2 * j1, blocks)) - s.k0;
     if (pair) {
       const int sees = min(q.keys, q.ctx + t0 + p.slot_tokens);  // slot 0's last row
-      s.cnt[0] = max(0, min(j1, sees <= 0 ? 0 : (sees + BLOCK - 1) / BLOCK) - w.j);
+      s.cnt[0] = max(0, min(j1, sees <= 0 ? 0 : (sees + BLOCK - 1) / BLOCK) - j0);
       s.cnt[1] = s.n;
     } else {
       s.cnt[0] = (s.n + 1) >> 1;
       s.cnt[1] = s.n >> 1;
     }
-    s.whole = take == steps;
+    s.whole = j1 - j0 == steps;
     if (!s.whole) {
-      const int64_t first = w.u - w.j;
-      s.part = w.j > 0 ? 0 : 1;
-      s.c_first = (int)(first / w.per);
-      s.c_last = (int)((first + steps - 1) / w.per);
-    }
-    s.buf = w.buf;
-    s.q_use[0] = w.q_use[0];
-    s.q_use[1] = w.q_use[1];
-    if (pair) {
-      ++w.q_use[0];
-      ++w.q_use[1];
-      w.buf = 0;
-    } else {
-      ++w.q_use[w.buf];
-      w.buf ^= 1;
+      s.part = j0 > 0 ? 0 : 1;
+      s.c_first = (int)((first + p.tile_cost) / w.per);
+      s.c_last = (int)((first + cost - 1) / w.per);
     }
     w.u += take;
-    w.j = j1;
-    if (j1 == steps) {
+    w.j += take;
+    if (w.j == cost) {
       w.j = 0;
       if (++w.i == tile_count(p, q)) {
         w.i = 0;
@@ -142,24 +129,37 @@ __device__ bool next_segment(const AttentionList& p, const StepList list, Walk& 
         }
       }
     }
+    if (j1 == j0) continue;  // the end of the run lies in what starting the tile takes
+    s.buf = w.buf;
+    s.q_use[0] = w.q_use[0];
+    s.q_use[1] = w.q_use[1];
+    if (pair) {
+      ++w.q_use[0];
+      ++w.q_use[1];
+      w.buf = 0;
+    } else {
+      ++w.q_use[w.buf];
+      w.buf ^= 1;
+    }
+    return true;
   }
-  more = __shfl_sync(0xffffffffu, more, 0);
-  __syncwarp();
-  return more != 0;
+  return false;
 }
 
-// Fills the list and this CTA's walk (of every warp). All threads.
+// Fills the list and this CTA's walk, which every thread gets, through `shared`. All threads.
 template <int BLOCK, int THREADS>
-__device__ void make_list(const AttentionList& p, const StepList list, Walk* walks) {
+__device__ void make_list(const AttentionList& p, const StepList list, Walk& walk, Walk* shared) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // Requests, and the steps of those with few tiles: a thread each.
   bool many = false;
+#pragma unroll 1
   for (int b = tid; b < p.batch; b += THREADS) {
     const Request q = load_request(p, b);
     list.req[b] = q;
     const int n = tile_count(p, q);
     int64_t sum = 0;
     if (n <= 8) {
+#pragma unroll 1
       for (int i = 0; i < n; ++i) sum += tile_steps<BLOCK>(p, q, i);
     } else {
       sum = -1;
@@ -169,13 +169,15 @@ __device__ void make_list(const AttentionList& p, const StepList list, Walk* wal
   }
   if (tid == 0) list.prefix[0] = 0;
   if (__syncthreads_or(many)) {
+#pragma unroll 1
     for (int b = warp; b < p.batch; b += THREADS / 32) {
       if (list.prefix[b + 1] >= 0) continue;
       const Request q = list.req[b];
       const int n = tile_count(p, q);
       int64_t sum = 0;
+#pragma unroll 1
       for (int i = lane; i < n; i += 32) sum += tile_steps<BLOCK>(p, q, i);
-#pragma unroll
+#pragma unroll 1
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       __syncwarp();
       if (lane == 0) list.prefix[b + 1] = sum;
@@ -184,9 +186,10 @@ __device__ void make_list(const AttentionList& p, const StepList list, Walk* wal
   }
   if (warp == 0) {
     int64_t run = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       int64_t v = b0 + lane < p.batch ? list.prefix[b0 + lane + 1] * p.kv_heads : 0;
-#pragma unroll
+#pragma unroll 1
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t w = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += w;
@@ -203,6 +206,7 @@ __device__ void make_list(const AttentionList& p, const StepList list, Walk* wal
     w.b = w.h = w.i = w.j = w.buf = w.q_use[0] = w.q_use[1] = 0;
     if (w.u < w.end) {
       int lo = 0, hi = p.batch - 1;  // the last request whose first step is not after u
+#pragma unroll 1
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (list.prefix[mid] <= w.u) lo = mid; else hi = mid - 1;
@@ -214,10 +218,11 @@ __device__ void make_list(const AttentionList& p, const StepList list, Walk* wal
       w.h = (int)(left / each);
       left -= w.h * each;
       const int n = tile_count(p, q);
+#pragma unroll 1
       for (int i0 = 0; i0 < n; i0 += 32) {
         int64_t v = i0 + lane < n ? tile_steps<BLOCK>(p, q, i0 + lane) : 0;
         const int64_t mine = v;
-#pragma unroll
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
           const int64_t x = __shfl_up_sync(0xffffffffu, v, o);
           if (lane >= o) v += x;
@@ -232,8 +237,10 @@ __device__ void make_list(const AttentionList& p, const StepList list, Walk* wal
         left -= __shfl_sync(0xffffffffu, v, 31);
       }
     }
-    if (lane < THREADS / 32) walks[lane] = w;
+    if (lane == 0) *shared = w;
   }
+  __syncthreads();
+  walk = *shared;
   __syncthreads();
 }
 

@@ -21,7 +21,7 @@
 // workspace, and the CTA that finishes last joins them in order.
 //
 // One CTA = 12 warps: 0..3 and 4..7 the slots' softmax (a thread per row, also the
-// epilogue), 8 TMA loads, 9 MMA issue, 10..11 look over the V blocks that not every row
+// epilogue), 8 TMA loads, 9 and 10 issue the slots' products, 11 looks over the V blocks that not every row
 // sees whole: rows past the request's keys are zeroed (a page's unused rows, the next
 // request's rows: 0 * NaN would reach O), and infinities and NaN in rows that only later
 // tokens see are taken out and listed; the epilogue adds them to the rows that see them.
@@ -39,7 +39,9 @@ namespace {
 
 constexpr int kBlock = 128;  // keys per block, rows per slot
 constexpr int kThreads = 384;
-constexpr int kBadMax = 192;  // listed V rows per checking warp: three blocks of 64
+constexpr int kBadMax = 384;  // listed V rows of a tile: three blocks
+
+constexpr int kRing = 4;  // segments that the roles may lie apart
 
 template <int DP>
 struct Cfg {
@@ -48,19 +50,16 @@ struct Cfg {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_LIST = OFF_KV + STAGES * TILE;
-  static constexpr int OFF_WALK = OFF_LIST + StepList::bytes(MTRTQ_MAX_BATCH);
-  static constexpr int OFF_SEG = OFF_WALK + kThreads / 32 * ((sizeof(Walk) + 15) / 16 * 16);
-  static constexpr int OFF_ML = OFF_SEG + kThreads / 32 * ((sizeof(Segment) + 15) / 16 * 16);  // slot 1's (m, l)
-  static constexpr int OFF_BAD = OFF_ML + kBlock * 8;                                         // [2][2][kBadMax] keys
-  static constexpr int OFF_BAR = OFF_BAD + 4 * kBadMax * 4;
-  static constexpr int NBAR = 3 * STAGES + 17;
+  static constexpr int OFF_SEG = OFF_LIST + MTRTQ_MAX_BATCH * sizeof(Request);
+  static constexpr int OFF_ML = OFF_SEG + kRing * ((sizeof(Segment) + 15) / 16 * 16);  // slot 1's (m, l)
+  static constexpr int OFF_BAD = OFF_ML + kBlock * 8;                                  // [kRing][kBadMax] keys
+  static constexpr int OFF_BAR = OFF_BAD + kRing * kBadMax * 4;
+  static constexpr int NBAR = 3 * STAGES + 2 * kRing + 22;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 64 + 1024;
   static constexpr int COL_O = 256;
-  // One pair of exponentials in this many is a polynomial on the FMA units: the special
-  // function units alone would take as long as both products (128 dimensions) or twice
-  // as long (64).
-  static constexpr int POLY = DP == 128 ? 4 : 2;
+  // One pair of exponentials in this many is a polynomial on the FMA units (0: none).
+  static constexpr int POLY = DP == 128 ? 0 : 4;
   static_assert(BYTES <= 227 * 1024, "shared memory per CTA");
 };
 
@@ -80,17 +79,35 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// V block as the B operand of O += P V: keys are its K side, dimensions (contiguous in
-// memory) its N side: 128-byte-swizzled rows of 64 dimensions, 8 keys per 1024 bytes
-// (stride byte offset), the next 64 dimensions 128 rows further (leading byte offset).
-__device__ __forceinline__ uint64_t desc_v(uint32_t addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)((kBlock * 128) >> 4) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
+// Operand descriptors, 128-byte swizzle: the low word has the address and the leading
+// byte offset, the high word is the same for all (groups of 8 rows 1024 bytes apart). A step
+// of the products moves the address alone, so one thread keeps the tensor cores fed: per
+// product an addition or two, where whole descriptors took longer than the product.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+// Q and K: contiguous along the dimensions, which are summed over.
+__device__ __forceinline__ uint32_t desc_qk(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | (1u << 16); }
+// V as the B operand of O += P V: keys are summed over, dimensions contiguous; the next 64
+// dimensions lie 128 rows further (leading byte offset).
+__device__ __forceinline__ uint32_t desc_v(uint32_t addr) {
+  return ((addr & 0x3FFFFu) >> 4) | ((uint32_t)(kBlock * 128 >> 4) << 16);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"((uint32_t)add), "r"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"((uint32_t)add), "r"(kDescHigh)
+      : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -126,6 +143,22 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
+// 32 bf16 of a row (`left` of them, whole groups of 8, if fewer are left): 32 bytes at a
+// time where the rows allow it, as every row is a line of its own.
+__device__ __forceinline__ void store_row(__nv_bfloat16* out, const uint32_t (&u)[16], int left, bool by32) {
+  if (by32 && left >= 32) {
+#pragma unroll
+    for (int y = 0; y < 16; y += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + 2 * y), "r"(u[y]),
+                   "r"(u[y + 1]), "r"(u[y + 2]), "r"(u[y + 3]), "r"(u[y + 4]), "r"(u[y + 5]), "r"(u[y + 6]),
+                   "r"(u[y + 7])
+                   : "memory");
+    return;
+  }
+#pragma unroll
+  for (int y = 0; y < 16; y += 4)
+    if (2 * y < left) *reinterpret_cast<uint4*>(out + 2 * y) = make_uint4(u[y], u[y + 1], u[y + 2], u[y + 3]);
+}
 // 2^x for finite x <= 8, below 2^-126 rounded up to about that: x = n + f with n whole and
 // |f| <= 1/2, 2^f by the cubic with the least relative error (7.5e-5, an eighth of a bf16
 // rounding), n added to the exponent.
@@ -148,12 +181,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return r;
 }
 
-// K and V blocks of a segment in the order the products need them: `at` 0 .. 2 n - 1
-// for n blocks.
-__device__ __forceinline__ int order_k(bool pair, int c) { return pair ? 2 * c : c < 2 ? c : 2 * c - 1; }
-__device__ __forceinline__ int order_v(bool pair, int c, int n) { return pair ? 2 * c + 1 : min(2 * c + 2, 2 * n - 1); }
-
-// The at-th of them: whether it is V, and which block c.
+// K and V blocks of a segment in the order the products need them, 2 n loads for n
+// blocks; the at-th: whether it is V, and which block c.
 __device__ __forceinline__ bool nth_load(bool pair, int at, int n, int& c) {
   if (pair) {
     c = at >> 1;
@@ -172,10 +201,21 @@ __device__ __forceinline__ bool nth_load(bool pair, int at, int n, int& c) {
 }
 
 // Bounded waits that fail at once when another role has given up.
+__device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned* status) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kSpinLimitCycles) {
+      *abort_flag = 1;
+      atomicExch(status, 6u /* MTRTQ_ERR_TIMEOUT */);
+      return false;
+    }
+  }
+  return true;
+}
 __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned* status) {
-  if (mbar_test_wait(bar, parity)) return true;
-  if (*abort_flag) return false;
-  return mbar_wait_bounded(bar, parity, abort_flag, status);
+  if (__builtin_expect(mbar_test_wait(bar, parity), 1)) return true;
+  return wait_slow(bar, parity, abort_flag, status);
 }
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned* status) {
   return __all_sync(0xffffffffu, wait_one(bar, parity, abort_flag, status));
@@ -187,21 +227,39 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
   while (!mbar_try_wait(bar, parity) && clock64() - t0 < kSpinLimitCycles) {}
 }
 
+// O's rows of this warp times keep.
+template <int DP>
+__device__ __forceinline__ void rescale(uint32_t o_addr, float keep) {
+#pragma unroll 1
+  for (int i = 0; i < DP; i += 16) {
+    uint32_t o[16];
+    tmem_ld_32x32b_x16(o_addr + i, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * keep);
+    tmem_st16(o_addr + i, o);
+  }
+}
+
 // One row of a cut tile from the parts of CTAs c_first .. c_last, in order.
 template <int DP>
-__device__ __noinline__ void join_parts(const TcAttention& p, int c_first, int c_last, int prow, __nv_bfloat16* out) {
+__device__ __forceinline__ void join_parts(const TcAttention& p, int c_first, int c_last, int prow, __nv_bfloat16* out) {
   const int64_t rows = p.part_rows;
   float top = -INFINITY;
+#pragma unroll 1
   for (int c = c_first; c <= c_last; ++c)
     top = fmaxf(top, __ldcg(p.part_ml + (c * 2 + (c == c_first)) * rows + prow).x);
   float sum = 0.0f;
+#pragma unroll 1
   for (int c = c_first; c <= c_last; ++c) {
     const float2 ml = __ldcg(p.part_ml + (c * 2 + (c == c_first)) * rows + prow);
     if (ml.x != -INFINITY) sum += ml.y * (top == INFINITY ? 1.0f : ex2(ml.x - top));
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
   for (int i = 0; i < p.head_dim; i += 8) {
     float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
     for (int c = c_first; c <= c_last; ++c) {
       const int64_t part = c * 2 + (c == c_first);
       const float pm = __ldcg(p.part_ml + part * rows + prow).x;
@@ -223,9 +281,8 @@ __device__ __noinline__ void join_parts(const TcAttention& p, int c_first, int c
   }
 }
 
-// After a bounded wait gives up, every role goes on through its loops without waiting,
-// copying or multiplying (each wait returns at once), so that all reach the barriers
-// between them and the end.
+// After a bounded wait gives up, every role's next wait fails at once and it leaves its
+// loop for the barrier at the end; there is no other barrier without a limit.
 template <int DP, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -234,7 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int NH = DP / 64;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  const StepList list(smem + C::OFF_LIST, MTRTQ_MAX_BATCH);
+  // the prefix lies where K and V will
+  const StepList list = {reinterpret_cast<Request*>(smem + C::OFF_LIST), reinterpret_cast<int64_t*>(smem + C::OFF_KV)};
   float2* ml1 = reinterpret_cast<float2*>(smem + C::OFF_ML);
   int* bad = reinterpret_cast<int*>(smem + C::OFF_BAD);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
@@ -247,37 +305,50 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* p_full = p_half + 2;
   uint64_t* o_full = p_full + 2;
   uint64_t* o_free = o_full + 2;
-  uint64_t* list_free = o_free + 2;
-  uint64_t* drained = list_free + 2;
+  uint64_t* turn = o_free + 2;
+  uint64_t* ml_full = turn + 2;
+  uint64_t* ml_free = ml_full + 1;
+  uint64_t* cut_in = ml_free + 1;   // a cut tile's part is stored
+  uint64_t* cut_out = cut_in + 1;   // its ticket is here
+  uint64_t* drained = cut_out + 1;
+  uint64_t* seg_full = drained + 2;  // [kRing]
+  uint64_t* seg_free = seg_full + kRing;
   uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* s_abort = reinterpret_cast<volatile int*>(misc + 1);
   volatile unsigned* s_ticket = misc + 2;
-  volatile int* bad_count = reinterpret_cast<volatile int*>(misc + 4);  // [2][2]
+  volatile int* bad_count = reinterpret_cast<volatile int*>(misc + 4);  // [kRing]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  Walk* walks = reinterpret_cast<Walk*>(smem + C::OFF_WALK);
-  Walk& walk = walks[warp];
-  Segment& s = reinterpret_cast<Segment*>(smem + C::OFF_SEG)[warp];
+  Segment* segments = reinterpret_cast<Segment*>(smem + C::OFF_SEG);
 
   if (tid == 0) {
     for (int x = 0; x < C::STAGES; ++x) {
       mbar_init(&full[x], 1);
-      mbar_init(&empty[x], 3);  // the products, two checking warps
-      mbar_init(&checked[x], 2);
+      mbar_init(&empty[x], 3);  // each slot's products, the check
+      mbar_init(&checked[x], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
-      mbar_init(&q_free[t], 1);
+      mbar_init(&q_free[t], 2);
       mbar_init(&s_full[t], 1);
       mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
       mbar_init(&o_free[t], 4);
-      mbar_init(&list_free[t], 8);
+      mbar_init(&turn[t], 1);
     }
-    mbar_init(drained, 1);
+    mbar_init(&drained[0], 1);
+    mbar_init(&drained[1], 1);
+    mbar_init(ml_full, 4);
+    mbar_init(ml_free, 4);
+    mbar_init(cut_in, 8);
+    mbar_init(cut_out, 1);
+    for (int r = 0; r < kRing; ++r) {
+      mbar_init(&seg_full[r], 1);
+      mbar_init(&seg_free[r], 11);  // 8 softmax warps, 2 of products, the check
+      bad_count[r] = 0;
+    }
     *s_abort = 0;
-    for (int x = 0; x < 4; ++x) bad_count[x] = 0;
     fence_barrier_init();
   }
   if (warp == 9) {
@@ -290,7 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&vmap);
   }
   tc_fence_before();
-  make_list<kBlock, kThreads>(p, list, walks);
+  Walk walk;  // warp 0's, and warp 8's: it makes the segments
+  make_list<kBlock, kThreads>(p, list, walk, reinterpret_cast<Walk*>(smem + C::OFF_SEG));
   tc_fence_after();
   const uint32_t tmem = misc[0];
   // The kernel that stored the new keys and cast the rows is complete from here on.
@@ -298,9 +370,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int ksteps = (p.head_dim + 15) / 16;
 
-  // 256 threads of 200 registers and 128 of 104: the 384 x 168 of the launch.
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_one(bar, parity, s_abort, p.status); };
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return wait_all(bar, parity, s_abort, p.status); };
+  // The ring's next segment; false at the end of the run (a segment without blocks).
+  auto next = [&](int seg) {
+    return warp_wait(&seg_full[seg % kRing], (seg / kRing) & 1) && segments[seg % kRing].n > 0;
+  };
+  auto leave = [&](int seg) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&seg_free[seg % kRing]);
+  };
+
+  // 256 threads of 208 registers and 128 of 88: the 384 x 168 of the launch.
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---------------- softmax and epilogue ----------------
     const int t = warp >> 2;                           // slot
     const int row = tid & 127;                         // of the slot's tile
@@ -310,18 +393,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float c2 = p.scale * 1.4426950408889634f;  // scale log2 e
     const float2 cc = make_float2(c2, c2);
     uint32_t n_s = 0, n_o = 0;
-    for (int seg = 0; next_segment<kBlock>(p, list, walk, s); ++seg) {
-      const int tok = (s.pair ? t * p.slot_tokens : 0) + token;  // of the tile's
+    uint32_t n_ml = 0, n_cut = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int seg = 0; ok && next(seg); leave(seg), ++seg) {
+      const Segment& s = segments[seg % kRing];
+      const bool pair = s.pair;
+      const int tok = (pair ? t * p.slot_tokens : 0) + token;  // of the tile's
       const bool live = token < p.slot_tokens && tok < s.tokens;
       const int keys = live ? max(0, min(s.see0 + tok, s.keys)) : 0;  // that this row sees
       const bool warp_live = __any_sync(0xffffffffu, live);
-      const int cnt = s.cnt[t], stride = s.pair ? kBlock : 2 * kBlock;
-      int left = keys - (s.k0 + (s.pair ? 0 : t)) * kBlock;  // columns of the block that it sees
+      const int cnt = s.cnt[t], stride = pair ? kBlock : 2 * kBlock;
+      int left = keys - (s.k0 + (pair ? 0 : t)) * kBlock;  // columns of the block that it sees
       float m = -INFINITY, l = 0.0f;
-      for (int x = 0; x < cnt; ++x, left -= stride) {
-        const bool ok = wait_all(&s_full[t], n_s & 1, s_abort, p.status);
-        ++n_s;
-        if (!ok || !warp_live) {
+#pragma unroll 1
+      for (int x = 0; x < cnt; ++x, left -= stride, ++n_s) {
+        ok = warp_wait(&s_full[t], n_s & 1);
+        if (!ok) break;
+        if (!warp_live) {
           if (lane == 0) {
             mbar_arrive(&p_half[t]);
             mbar_arrive(&p_full[t]);
@@ -333,50 +422,50 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + 32 * i, v + 32 * i);
         tmem_wait_ld();
-        if (__any_sync(0xffffffffu, left < kBlock)) {
+        float top;
+        {
+          float a[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-          for (int i = 0; i < kBlock; ++i) v[i] = i < left ? v[i] : -INFINITY;
-        }
-        float top = max3(v[0], v[1], v[2]), top1 = max3(v[3], v[4], v[5]);
+          for (int i = 4; i + 7 < kBlock; i += 8) {
 #pragma unroll
-        for (int i = 6; i + 3 < kBlock; i += 4) {
-          top = max3(top, v[i], v[i + 1]);
-          top1 = max3(top1, v[i + 2], v[i + 3]);
-        }
-        top = max3(top, top1, max3(v[kBlock - 2], v[kBlock - 1], top1)) * c2;
-        // Masked, infinite or NaN scores: every exponential by the instruction, which
-        // keeps them exact.
-        const bool exact = __any_sync(0xffffffffu, left < kBlock || !(fabsf(top) < INFINITY));
-        const bool grow = top > m + 8.0f || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float m1 = grow ? top : m;
-          const float keep = m1 == -INFINITY ? 1.0f : ex2(m - m1);
-          l *= keep;
-          m = m1;
-          if (x > 0) {
-            // this slot's earlier products are complete: their scores came after them
-#pragma unroll 1
-            for (int i = 0; i < DP; i += 16) {
-              uint32_t o[16];
-              tmem_ld_32x32b_x16(o_addr + i, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * keep);
-              tmem_st16(o_addr + i, o);
-            }
+            for (int y = 0; y < 4; ++y) a[y] = max3(a[y], v[i + 2 * y], v[i + 2 * y + 1]);
           }
+          a[0] = max3(a[0], v[kBlock - 4], v[kBlock - 3]);
+          a[1] = max3(a[1], v[kBlock - 2], v[kBlock - 1]);
+          top = max3(a[0], a[1], max3(a[2], a[3], a[3])) * c2;
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        // Masked, infinite or NaN scores: read again and masked, in short loops, and every
+        // exponential by the instruction, which keeps them exact.
+        const bool slow = __any_sync(0xffffffffu, left < kBlock || !(fabsf(top) < INFINITY));
         float2 sum = make_float2(0.0f, 0.0f);
-        const float2 mm = make_float2(-base, -base);
-        auto weights = [&](auto some_cubic) {
+        // Takes the block's maximum into account; the exponent's -m'.
+        auto raise = [&](float block_top) {
+          const bool grow = block_top > m + 8.0f || (m == -INFINITY && block_top > m);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float m1 = grow ? block_top : m;
+            const float keep = m1 == -INFINITY ? 1.0f : ex2(m - m1);
+            l *= keep;
+            m = m1;
+            if (x > 0) rescale<DP>(o_addr, keep);  // the earlier products are complete: these scores came after them
+          }
+          return m == -INFINITY ? 0.0f : -m;
+        };
+        auto half_done = [&]() {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_half[t]);
+        };
+        if (!slow) {
+          const float mm1 = raise(top);
+          const float2 mm = make_float2(mm1, mm1);
 #pragma unroll
           for (int i = 0; i < kBlock; i += 32) {
             uint32_t w[16];
 #pragma unroll
             for (int y = 0; y < 16; ++y) {
               float2 e = fma2(make_float2(v[i + 2 * y], v[i + 2 * y + 1]), cc, mm);
-              if (decltype(some_cubic)::value && y % C::POLY == C::POLY - 1) {
+              if (C::POLY && y % (C::POLY ? C::POLY : 1) == C::POLY - 1) {
                 e = exp2_cubic(e);
               } else {
                 e.x = ex2(e.x);
@@ -386,55 +475,84 @@ __global__ void __launch_bounds__(kThreads, 1)
               w[y] = pack_bf16(e.x, e.y);
             }
             tmem_st16(s_addr + (i >> 1), w);
-            if (i == kBlock / 2 - 32) {
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_half[t]);
-            }
+            if (i == kBlock / 2 - 32) half_done();
           }
-        };
-        if (exact) weights(std::false_type());
-        else weights(std::true_type());
+        } else {
+          top = -INFINITY;
+#pragma unroll 1
+          for (int i = 0; i < kBlock; i += 32) {
+            float u[32];
+            tmem_ld32(s_addr + i, u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 32; ++y) top = fmaxf(top, i + y < left ? u[y] * c2 : -INFINITY);
+          }
+          const float mm1 = raise(top);
+          const float2 mm = make_float2(mm1, mm1);
+#pragma unroll 1
+          for (int i = 0; i < kBlock; i += 32) {  // P's columns so far lie before the scores still to be read
+            float u[32];
+            tmem_ld32(s_addr + i, u);
+            tmem_wait_ld();
+            uint32_t w[16];
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+              float2 e = fma2(make_float2(i + 2 * y < left ? u[2 * y] : -INFINITY,
+                                          i + 2 * y + 1 < left ? u[2 * y + 1] : -INFINITY), cc, mm);
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              sum = __fadd2_rn(sum, e);
+              w[y] = pack_bf16(e.x, e.y);
+            }
+            tmem_st16(s_addr + (i >> 1), w);
+            if (i == kBlock / 2 - 32) half_done();
+          }
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
         l += sum.x + sum.y;
       }
+      if (!ok) break;
 
       if (m == -INFINITY && l != l) m = 0.0f;  // every score it saw was NaN
-      bool ok = true;
       if (cnt > 0) {
-        ok = wait_all(&o_full[t], n_o & 1, s_abort, p.status);
+        ok = warp_wait(&o_full[t], n_o & 1);
         ++n_o;
-        tc_fence_after();
+        if (!ok) break;
       }
       // halves: slot 0's threads join the two slots' rows
-      const bool mine = s.pair || t == 0, two = !s.pair && s.n > 1;
+      const bool mine = pair || t == 0, two = !pair && s.n > 1, whole = s.whole;
       float w0 = 1.0f, w1 = 0.0f;
-      if (!s.pair) {
-        if (t == 1) ml1[row] = make_float2(m, l);
-        tc_fence_before();
-        named_bar_sync(1, 256);
-        tc_fence_after();
-        if (two && t == 0) {
+      if (two) {
+        if (t == 1) {
+          ok = warp_wait(ml_free, (n_ml & 1) ^ 1);
+          ml1[row] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(ml_full);
+        } else {
+          ok = warp_wait(ml_full, n_ml & 1);  // slot 1's warps have waited for their products
           const float2 ml = ml1[row];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(ml_free);
           const float top = fmaxf(m, ml.x);
           w0 = m == -INFINITY ? 0.0f : top == INFINITY ? 1.0f : ex2(m - top);
           w1 = ml.x == -INFINITY ? 0.0f : top == INFINITY ? 1.0f : ex2(ml.x - top);
           l = l * w0 + ml.y * w1;
           m = top;
         }
+        ++n_ml;
+        if (!ok) break;
       }
+      tc_fence_after();
       if (m == -INFINITY) w0 = 0.0f;  // no key seen (and perhaps no product formed)
-      const int prow = (s.pair ? t * kBlock : 0) + row;
-      const int64_t at_out =
-          (int64_t)(s.row0 + tok) * p.out_row + (int64_t)(s.h * p.group + head) * p.out_head;
+      const int prow = (pair ? t * kBlock : 0) + row;
+      __nv_bfloat16* out = p.out + (int64_t)(s.row0 + tok) * p.out_row + (int64_t)(s.h * p.group + head) * p.out_head;
       const int64_t part = (int64_t)blockIdx.x * 2 + s.part;
       float* to_part = p.partials + (part * p.part_rows * (DP / 4) + prow) * 4;
-      if (mine && ok) {
-        if (s.whole) {
+      if (mine) {
+        if (whole) {
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
           w0 *= inv;
           w1 *= inv;
@@ -452,94 +570,104 @@ __global__ void __launch_bounds__(kThreads, 1)
             float o1[32];
             tmem_ld32(o_addr + DP + i, o1);
             tmem_wait_ld();
-            if (w1 != 0.0f) {
 #pragma unroll
-              for (int y = 0; y < 32; ++y) o[y] = fmaf(o1[y], w1, o[y]);
-            }
+            for (int y = 0; y < 32; ++y) o[y] += w1 == 0.0f ? 0.0f : o1[y] * w1;
           }
-          if (live) {
-            if (s.whole) {
+          if (!live) continue;
+          if (whole) {
+            uint32_t u[16];
 #pragma unroll
-              for (int y = 0; y < 32; y += 8) {
-                if (i + y < p.head_dim)
-                  *reinterpret_cast<uint4*>(p.out + at_out + i + y) =
-                      make_uint4(pack_bf16(o[y], o[y + 1]), pack_bf16(o[y + 2], o[y + 3]),
-                                 pack_bf16(o[y + 4], o[y + 5]), pack_bf16(o[y + 6], o[y + 7]));
-              }
-            } else {
+            for (int y = 0; y < 16; ++y) u[y] = pack_bf16(o[2 * y], o[2 * y + 1]);
+            store_row(out + i, u, p.head_dim - i, p.out32);
+          } else {
 #pragma unroll
-              for (int y = 0; y < 32; y += 4)
-                __stcg(reinterpret_cast<float4*>(to_part + (int64_t)(i + y) * p.part_rows),
-                       make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]));
-            }
+            for (int y = 0; y < 32; y += 4)
+              __stcg(reinterpret_cast<float4*>(to_part + (int64_t)(i + y) * p.part_rows),
+                     make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]));
           }
         }
-        if (live && !s.whole) __stcg(p.part_ml + part * p.part_rows + prow, make_float2(m, l));
+        if (live && !whole) __stcg(p.part_ml + part * p.part_rows + prow, make_float2(m, l));
         // The infinities and NaN that were taken out of the last blocks' V, for the rows
         // that see them. A slot without blocks here has not waited for the check, and
         // sees none of it.
-        const int par = seg & 1;
         if (cnt > 0 && (s.k0 + s.n) * kBlock > s.all_see()) {
-          for (int w = 0; w < 2; ++w) {
-            const int have = min(kBadMax, bad_count[par * 2 + w]);
-            for (int x = 0; x < have; ++x) {
-              const int key = bad[(par * 2 + w) * kBadMax + x];
-              if ((unsigned)key >= (unsigned)keys) continue;
-              const __nv_bfloat16* src;
-              if (PAGED) {
-                const int64_t page = p.table[s.b * p.table_ld + key / p.page_size];
-                src = p.v + page * p.v_row + ((int64_t)s.h * p.page_size + key % p.page_size) * p.head_dim;
+          const int have = min(kBadMax, bad_count[seg % kRing]);
+#pragma unroll 1
+          for (int x = 0; x < have; ++x) {
+            const int key = bad[seg % kRing * kBadMax + x];
+            if ((unsigned)key >= (unsigned)keys) continue;
+            const __nv_bfloat16* src;
+            if (PAGED) {
+              const int64_t page = p.table[s.b * p.table_ld + key / p.page_size];
+              src = p.v + page * p.v_row + ((int64_t)s.h * p.page_size + key % p.page_size) * p.head_dim;
+            } else {
+              src = p.v + (int64_t)(s.r0 + key) * p.v_row + s.h * p.v_head;
+            }
+#pragma unroll 1
+            for (int d = 0; d < p.head_dim; ++d) {
+              const float z = __bfloat162float(src[d]);
+              if (fabsf(z) < INFINITY) continue;
+              if (whole) {
+                out[d] = __float2bfloat16_rn(__bfloat162float(out[d]) + z);
               } else {
-                src = p.v + (int64_t)(list.req[s.b].r0 + key) * p.v_row + s.h * p.v_head;
-              }
-              for (int d = 0; d < p.head_dim; ++d) {
-                const float z = __bfloat162float(src[d]);
-                if (fabsf(z) < INFINITY) continue;
-                if (s.whole) {
-                  p.out[at_out + d] = __float2bfloat16_rn(__bfloat162float(p.out[at_out + d]) + z);
-                } else {
-                  float* to = to_part + (int64_t)(d & ~3) * p.part_rows + (d & 3);
-                  __stcg(to, __ldcg(to) + z);
-                }
+                float* to = to_part + (int64_t)(d & ~3) * p.part_rows + (d & 3);
+                __stcg(to, __ldcg(to) + z);
               }
             }
           }
         }
+        // O has been read.
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (cnt > 0) mbar_arrive(&o_free[t]);
+          if (two) mbar_arrive(&o_free[1]);
+        }
       }
-      // O and the list have been read.
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (mine && cnt > 0) mbar_arrive(&o_free[t]);
-        if (two && t == 0) mbar_arrive(&o_free[1]);
-        mbar_arrive(&list_free[seg & 1]);
-      }
-      if (!s.pair) named_bar_sync(2, 256);  // ml1 has been read
-      if (!s.whole && mine) {
-        const int id = s.pair ? 3 : 4, count = s.pair ? 256 : 128;
-        named_bar_sync(id, count);
-        if (tid == 0) *s_ticket = ticket_acq_rel(p.counters + s.c_first);
-        named_bar_sync(id, count);
-        const bool last = *s_ticket == (unsigned)(s.c_last - s.c_first);
-        if (last && live) join_parts<DP>(p, s.c_first, s.c_last, prow, p.out + at_out);
-        if (last && tid == 0) p.counters[s.c_first] = 0u;
+      if (!whole) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(cut_in);
+        if (tid == 0) {
+          wait(cut_in, n_cut & 1);
+          *s_ticket = ticket_acq_rel(p.counters + s.c_first);
+          mbar_arrive(cut_out);
+        }
+        __syncwarp();
+        if (mine) {
+          ok = warp_wait(cut_out, n_cut & 1);
+          const bool last = *s_ticket == (unsigned)(s.c_last - s.c_first);
+          if (ok && last && live) join_parts<DP>(p, s.c_first, s.c_last, prow, out);
+          if (last && tid == 0) p.counters[s.c_first] = 0u;
+        }
+        ++n_cut;
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 8) {
       // ---------------- loads ----------------
-      uint32_t seq = 0, sent = 0;
+      uint32_t seq = 0;
       int q_sent[2] = {0, 0};
       const int pages = PAGED ? kBlock / p.page_size : 1;
       const uint32_t box = (PAGED ? p.page_size : kBlock) * 128;
       const uint32_t rows_bytes = (uint32_t)p.slot_tokens * p.group * 128 * NH;
-      while (next_segment<kBlock>(p, list, walk, s)) {
+      bool ok = true;
+#pragma unroll 1
+      for (int seg = 0; ok; ++seg) {
+        Segment& s = segments[seg % kRing];
+        ok = warp_wait(&seg_free[seg % kRing], ((seg / kRing) & 1) ^ 1);
+        if (!ok) break;
+        if (lane == 0 && !next_segment<kBlock>(p, list, walk, s)) s.n = 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_full[seg % kRing]);
         const int k0 = s.k0, n = s.n;
+        if (n == 0) break;
         const bool pair = s.pair;
-        for (int t = 0; t < (pair ? 2 : 1); ++t) {
+#pragma unroll 1
+        for (int t = 0; ok && t < (pair ? 2 : 1); ++t) {
           const int buf = pair ? t : s.buf;
-          if (!wait_all(&q_free[buf], (s.q_use[buf] & 1) ^ 1, s_abort, p.status)) continue;
+          ok = warp_wait(&q_free[buf], (s.q_use[buf] & 1) ^ 1);
+          if (!ok) break;
           ++q_sent[buf];
           if (lane == 0) mbar_arrive_expect_tx(&q_full[buf], rows_bytes);
           __syncwarp();
@@ -547,8 +675,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_4d(smem + C::OFF_Q + buf * C::TILE + lane * kBlock * 128, &qmap, lane * 64, 0, s.h,
                         s.row0 + t * p.slot_tokens, &q_full[buf]);
         }
-        const int r0 = PAGED ? 0 : list.req[s.b].r0;
-        for (int at = 0; at < 2 * n; ++at, ++seq) {
+#pragma unroll 1
+        for (int at = 0; ok && at < 2 * n; ++at) {
           int c;
           const bool is_v = nth_load(pair, at, n, c);
           const int st = seq % C::STAGES;
@@ -560,8 +688,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             load = load && key0 + pg * p.page_size < s.keys;
             if (load) page = p.table[s.b * p.table_ld + (k0 + c) * pages + pg];
           }
-          if (!wait_all(&empty[st], ((seq / C::STAGES) & 1) ^ 1, s_abort, p.status)) continue;
-          sent = seq + 1;
+          ok = warp_wait(&empty[st], ((seq / C::STAGES) & 1) ^ 1);
+          if (!ok) break;
+          ++seq;
           const unsigned who = __ballot_sync(0xffffffffu, load);
           if (lane == 0) mbar_arrive_expect_tx(&full[st], box * __popc(who));
           __syncwarp();
@@ -570,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (PAGED)
               tma_load_3d(dst, is_v ? &vmap : &kmap, half * 64, s.h * p.page_size, page, &full[st]);
             else
-              tma_load_3d(dst, is_v ? &vmap : &kmap, half * 64, s.h, r0 + key0, &full[st]);
+              tma_load_3d(dst, is_v ? &vmap : &kmap, half * 64, s.h, s.r0 + key0, &full[st]);
           }
         }
       }
@@ -579,124 +708,136 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (*s_abort && lane == 0) {
         for (int t = 0; t < 2; ++t)
           if (q_sent[t]) drain(&q_full[t], (q_sent[t] - 1) & 1);
-        for (uint32_t x = sent > C::STAGES ? sent - C::STAGES : 0; x < sent; ++x)
+        for (uint32_t x = seq > C::STAGES ? seq - C::STAGES : 0; x < seq; ++x)
           drain(&full[x % C::STAGES], (x / C::STAGES) & 1);
       }
       __syncwarp();
-    } else if (warp == 9) {
-      // ---------------- products ----------------
+    } else if (warp < 11) {
+      // ---------------- products: a warp for each slot ----------------
+      // It follows every load in order (so that no phase of a barrier is taken for another)
+      // and lets go at once of those that its slot does not use.
+      const int t = warp - 9;
       const uint32_t idesc_s = umma_idesc_bf16(kBlock, kBlock);
       const uint32_t idesc_o = umma_idesc_bf16(kBlock, ksteps * 16) | (1u << 16);  // B is contiguous along N
-      const uint32_t q_addr = smem_u32(smem + C::OFF_Q), kv_addr = smem_u32(smem + C::OFF_KV);
-      uint32_t base = 0, fixed = 0;  // loads so far; phase of each stage's check
-      uint32_t n_p[2] = {0, 0}, n_seg[2] = {0, 0};
-      while (next_segment<kBlock>(p, list, walk, s)) {
+      const uint32_t q_desc = desc_qk(smem_u32(smem + C::OFF_Q)), k_desc = desc_qk(smem_u32(smem + C::OFF_KV)),
+                     v_desc = desc_v(smem_u32(smem + C::OFF_KV));
+      const uint32_t s_col = tmem + t * kBlock, o_col = tmem + C::COL_O + t * DP;
+      uint32_t seq = 0, fixed = 0;  // loads so far; phase of each stage's check
+      uint32_t n_p = 0, n_o = 0, n_turn = 0;
+      // A turn: one block's PV and the next one's scores. Slot 0 has the first; a slot with
+      // fewer blocks passes its turns on. Without turns the slots fall into step, and the
+      // tensor cores wait for both.
+      auto take_turn = [&]() { return wait(&turn[t], (n_turn++ & 1) ^ (t ^ 1)); };
+      auto end_turn = [&]() { mbar_arrive(&turn[t ^ 1]); };
+#pragma unroll 1
+      for (int seg = 0; next(seg); leave(seg), ++seg) {
         if (lane == 0) {
+          const Segment& s = segments[seg % kRing];
           const bool pair = s.pair;
-          const int n = s.n, k0 = s.k0, all_see = s.all_see();
-          const int cnt[2] = {s.cnt[0], s.cnt[1]};
-          auto block_of = [&](int t, int x) { return pair ? x : 2 * x + t; };
-          auto wait_load = [&](uint32_t at) {
-            return wait_one(&full[at % C::STAGES], (at / C::STAGES) & 1, s_abort, p.status);
-          };
-          auto scores = [&](int t, int x) {
-            const int c = block_of(t, x), buf = pair ? t : s.buf;
-            const uint32_t at = base + order_k(pair, c);
-            if (!wait_load(at)) return;
-            tc_fence_after();
-            const uint32_t k = kv_addr + (at % C::STAGES) * C::TILE, q = q_addr + buf * C::TILE;
-            for (int i = 0; i < ksteps; ++i) {
-              const uint32_t off = (i >> 2) * kBlock * 128 + (i & 3) * 32;
-              umma_ss(tmem + t * kBlock, umma_desc_sw128(q + off), umma_desc_sw128(k + off), idesc_s, i > 0);
-            }
-            umma_commit(&s_full[t]);
-            if (!pair || t == 1) umma_commit(&empty[at % C::STAGES]);
-            if (pair ? x == cnt[t] - 1 : c == n - 1) umma_commit(&q_free[buf]);
-          };
+          const uint32_t turns = n_turn + max(s.cnt[0], s.cnt[1]) + 1;
+          const int n = s.n, cnt = s.cnt[t], buf = pair ? t : s.buf;
+          const int checked_from = max(0, s.all_see() / kBlock - s.k0);  // blocks from there on
           bool ok = true;
-          for (int t = 0; t < (pair ? 2 : 1); ++t) {
-            const int buf = pair ? t : s.buf;
-            ok = wait_one(&q_full[buf], s.q_use[buf] & 1, s_abort, p.status) && ok;
+          if (pair) {
+            ok = wait(&q_full[t ^ 1], s.q_use[t ^ 1] & 1);
+            mbar_arrive(&q_free[t ^ 1]);
           }
-          for (int t = 0; t < 2; ++t)
-            if (ok && cnt[t] > 0) scores(t, 0);
-          if (pair && cnt[0] == 0) umma_commit(&q_free[0]);
-          uint32_t was_checked = 0;  // pair: slot 0 has waited for this stage's check
-          for (int x = 0; x < max(cnt[0], cnt[1]); ++x) {
-            for (int t = 0; t < 2; ++t) {
-              if (x >= cnt[t]) continue;
-              const int c = block_of(t, x);
-              const uint32_t at = base + order_v(pair, c, n), st = at % C::STAGES;
-              if (x == 0) wait_one(&o_free[t], (n_seg[t] & 1) ^ 1, s_abort, p.status);
-              wait_load(at);
-              if ((k0 + c + 1) * kBlock > all_see && !(pair && t == 1 && (was_checked >> st & 1))) {
-                wait_one(&checked[st], fixed >> st & 1, s_abort, p.status);
-                fixed ^= 1u << st;
-                was_checked |= 1u << st;
-              }
-              const uint32_t v = kv_addr + st * C::TILE;
-              for (int half = 0; half < 2; ++half) {
-                wait_one(half ? &p_full[t] : &p_half[t], n_p[t] & 1, s_abort, p.status);
-                if (*s_abort) break;
-                tc_fence_after();
+          ok = ok && wait(&q_full[buf], s.q_use[buf] & 1);
+          if (cnt == 0) mbar_arrive(&q_free[buf]);
+          const uint32_t q = q_desc + buf * (C::TILE >> 4);
+          int x_k = 0, x_v = 0;  // of this slot's blocks
+#pragma unroll 1
+          for (int at = 0; ok && at < 2 * n; ++at, ++seq) {
+            int c;
+            const bool is_v = nth_load(pair, at, n, c);
+            const uint32_t st = seq % C::STAGES;
+            ok = wait(&full[st], (seq / C::STAGES) & 1);
+            const bool mine = pair ? c < cnt : (c & 1) == t;
+            if (is_v && c >= checked_from) {
+              if (mine) ok = ok && wait(&checked[st], fixed >> st & 1);
+              fixed ^= 1u << st;
+            }
+            if (!ok) break;
+            if (!mine) {
+              mbar_arrive(&empty[st]);
+              continue;
+            }
+            if (!is_v) {
+              if (x_k == 0) ok = take_turn();
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t k = k_desc + st * (C::TILE >> 4);
 #pragma unroll
-                for (int i = half * 4; i < half * 4 + 4; ++i)
-                  umma_ts(tmem + C::COL_O + t * DP, tmem + t * kBlock + i * 8, desc_v(v + i * 2048), idesc_o,
-                          x > 0 || i > 0);
+              for (int i = 0; i < DP / 16; ++i)
+                if (i < ksteps)
+                  mma_ss(s_col, q + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2,
+                         k + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2, idesc_s, i > 0);
+              umma_commit(&s_full[t]);
+              end_turn();
+              umma_commit(&empty[st]);
+              if (++x_k == cnt) umma_commit(&q_free[buf]);
+            } else {
+              if (x_v == 0) ok = wait(&o_free[t], (n_o & 1) ^ 1);
+              ok = ok && wait(&p_half[t], n_p & 1) && take_turn();
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t v = v_desc + st * (C::TILE >> 4);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) mma_ts(o_col, s_col + i * 8, v + i * (2048 >> 4), idesc_o, x_v > 0 || i > 0);
+              ok = wait(&p_full[t], n_p & 1);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int i = 4; i < 8; ++i) mma_ts(o_col, s_col + i * 8, v + i * (2048 >> 4), idesc_o, true);
+              ++n_p;
+              umma_commit(&empty[st]);
+              if (++x_v == cnt) {
+                umma_commit(&o_full[t]);
+                ++n_o;
+                end_turn();
               }
-              ++n_p[t];
-              if (*s_abort) continue;
-              if (!pair || t == 1) {
-                umma_commit(&empty[st]);
-                was_checked &= ~(1u << st);
-              }
-              if (x + 1 < cnt[t]) scores(t, x + 1);
-              else umma_commit(&o_full[t]);
             }
           }
-          for (int t = 0; t < 2; ++t)
-            if (cnt[t] > 0) ++n_seg[t];
-          base += 2 * n;
+#pragma unroll 1
+          while (ok && n_turn < turns) {
+            ok = take_turn();
+            end_turn();
+          }
         }
         __syncwarp();
       }
       if (lane == 0 && *s_abort) {  // the products in flight end before TMEM is freed
-        umma_commit(drained);
-        drain(drained, 0);
+        umma_commit(&drained[t]);
+        drain(&drained[t], 0);
       }
       __syncwarp();
     } else {
       // ---------------- V blocks that not every row sees whole ----------------
-      const int w = warp - 10;
-      uint32_t base = 0;
-      for (int seg = 0; next_segment<kBlock>(p, list, walk, s); ++seg) {
+      uint32_t seq = 0;
+      bool ok = true;
+#pragma unroll 1
+      for (int seg = 0; ok && next(seg); leave(seg), ++seg) {
+        const Segment& s = segments[seg % kRing];
         const bool pair = s.pair;
-        const int n = s.n, k0 = s.k0, keys = s.keys, all_see = s.all_see(), par = seg & 1;
-        bool first = true;
-        for (int x = 0; x < 2 * n; ++x) {
+        const int n = s.n, k0 = s.k0, keys = s.keys, slot = seg % kRing;
+        const int checked_from = max(0, s.all_see() / kBlock - k0);
+        if (lane == 0) bad_count[slot] = 0;
+        __syncwarp();
+#pragma unroll 1
+        for (int at = 0; ok && at < 2 * n; ++at, ++seq) {
           int c;
-          const bool is_v = nth_load(pair, x, n, c);
-          const int key0 = (k0 + c) * kBlock;
-          const uint32_t at = base + x, st = at % C::STAGES;
-          // every load is followed, so that no phase of its barrier is taken for another
-          const bool landed = wait_all(&full[st], (at / C::STAGES) & 1, s_abort, p.status);
-          if (!is_v || key0 + kBlock <= all_see) {
-            if (lane == 0) mbar_arrive(&empty[st]);
-            continue;
-          }
-          if (first) {
-            wait_all(&list_free[par], ((seg >> 1) & 1) ^ 1, s_abort, p.status);
-            if (lane == 0) bad_count[par * 2 + w] = 0;
-            __syncwarp();
-            first = false;
-          }
-          if (landed) {
+          const bool is_v = nth_load(pair, at, n, c);
+          const uint32_t st = seq % C::STAGES;
+          ok = warp_wait(&full[st], (seq / C::STAGES) & 1);
+          if (!ok) break;
+          if (is_v && c >= checked_from) {
             uint8_t* v = smem + C::OFF_KV + st * C::TILE;
-#pragma unroll
-            for (int rr = 0; rr < 2; ++rr) {
-              const int r = w * 64 + rr * 32 + lane;
+            const int key0 = (k0 + c) * kBlock;
+#pragma unroll 1
+            for (int r = lane; r < kBlock; r += 32) {
               const bool kept = key0 + r < keys;
               bool broken = false;
+#pragma unroll
               for (int y = 0; y < NH * 8; ++y) {
                 uint4* at16 =
                     reinterpret_cast<uint4*>(v + (y >> 3) * kBlock * 128 + r * 128 + (((y & 7) ^ (r & 7)) << 4));
@@ -704,38 +845,41 @@ __global__ void __launch_bounds__(kThreads, 1)
                   *at16 = make_uint4(0, 0, 0, 0);
                   continue;
                 }
-                uint4 u = *at16;
-                uint32_t* e = reinterpret_cast<uint32_t*>(&u);
-                bool hit = false;
+                const uint4 u = *at16;
+                const uint32_t e[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                  if ((e[z] & 0x7f80u) == 0x7f80u) { e[z] &= 0xffff0000u; hit = true; }
-                  if ((e[z] & 0x7f800000u) == 0x7f800000u) { e[z] &= 0xffffu; hit = true; }
+                for (int z = 0; z < 4; ++z)
+                  broken |= (e[z] & 0x7f80u) == 0x7f80u || (e[z] & 0x7f800000u) == 0x7f800000u;
+              }
+              if (broken) {
+#pragma unroll 1
+                for (int y = 0; y < NH * 32; ++y) {
+                  uint32_t* at4 = reinterpret_cast<uint32_t*>(v + (y >> 5) * kBlock * 128 + r * 128 +
+                                                              ((((y >> 2) & 7) ^ (r & 7)) << 4) + (y & 3) * 4);
+                  uint32_t e = *at4;
+                  if ((e & 0x7f80u) == 0x7f80u) e &= 0xffff0000u;
+                  if ((e & 0x7f800000u) == 0x7f800000u) e &= 0xffffu;
+                  *at4 = e;
                 }
-                if (hit) *at16 = u;
-                broken |= hit;
               }
               const unsigned who = __ballot_sync(0xffffffffu, broken);
               if (who) {
-                const int had = bad_count[par * 2 + w];
+                const int had = bad_count[slot];
                 __syncwarp();
                 const int to = had + __popc(who & ((1u << lane) - 1));
-                if (broken && to < kBadMax) bad[(par * 2 + w) * kBadMax + to] = key0 + r;
+                if (broken && to < kBadMax) bad[slot * kBadMax + to] = key0 + r;
                 __threadfence_block();  // slot 0 may read while slot 1's last blocks are looked over
                 __syncwarp();
-                if (lane == 0) bad_count[par * 2 + w] = min(kBadMax, had + __popc(who));
+                if (lane == 0) bad_count[slot] = min(kBadMax, had + __popc(who));
                 __syncwarp();
               }
             }
             fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&checked[st]);
           }
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&checked[st]);
-            mbar_arrive(&empty[st]);
-          }
+          if (lane == 0) mbar_arrive(&empty[st]);
         }
-        base += 2 * n;
       }
     }
   }
