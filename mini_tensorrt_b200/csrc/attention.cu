@@ -290,6 +290,7 @@ int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cuda
   p.tile_tokens = 2 * l.slot_tokens;
   p.min_steps = 4;
   p.tile_cost = 2;
+  p.pair_cost = 3;
   p.scale = a.scale;
   p.out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_row % 16 == 0 && a.out_head % 16 == 0;
   p.out = static_cast<__nv_bfloat16*>(a.out);
@@ -339,7 +340,7 @@ int launch_f32(const Args& a, bool paged, void* workspace, cudaStream_t st) {
   p.slot_tokens = 0;
   p.tile_tokens = l.tile_rows / p.group;
   p.min_steps = 3;
-  p.tile_cost = 1;
+  p.pair_cost = 1;  // (every f32 tile is of that kind)
   p.scale = a.scale;
   p.q = static_cast<const float*>(a.q);
   p.k = static_cast<const float*>(paged ? a.k_pages : a.k);

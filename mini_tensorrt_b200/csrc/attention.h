@@ -21,7 +21,7 @@ struct AttentionList {
   int tile_tokens;
   int64_t max_keys;   // paged: tokens the table's columns hold
   int64_t min_steps;  // fewest steps worth a CTA
-  int tile_cost;      // steps that a tile takes besides its own
+  int tile_cost, pair_cost;  // steps that a tile takes besides its own, in one slot's rows or more
 };
 
 struct TcAttention : AttentionList {

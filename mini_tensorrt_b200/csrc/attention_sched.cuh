@@ -73,11 +73,11 @@ template <int BLOCK>
 __device__ __forceinline__ int tile_steps(const AttentionList& p, const Request& q, int i) {
   const int t0 = i * p.tile_tokens, tokens = min(p.tile_tokens, q.m - t0);
   const int blocks = block_count<BLOCK>(q, t0, tokens);
-  return p.tile_cost + (tokens > p.slot_tokens ? blocks : (blocks + 1) >> 1);
+  return tokens > p.slot_tokens ? p.pair_cost + blocks : p.tile_cost + ((blocks + 1) >> 1);
 }
 
-// One thread's; false at the end of the CTA's run. A tile counts p.tile_cost steps more
-// than it has: what starting and ending it takes.
+// One thread's; false at the end of the CTA's run. A tile counts tile_cost or
+// pair_cost steps more than it has: what starting and ending it takes.
 template <int BLOCK>
 __device__ bool next_segment(const AttentionList& p, const StepList list, Walk& w, Segment& s) {
 #pragma unroll 1
@@ -88,9 +88,9 @@ __device__ bool next_segment(const AttentionList& p, const StepList list, Walk& 
     const bool pair = tokens > p.slot_tokens;
     const int steps = pair ? blocks : (blocks + 1) >> 1;
     const int64_t first = w.u - w.j;  // of the tile's
-    const int cost = steps + p.tile_cost;
+    const int extra = pair ? p.pair_cost : p.tile_cost, cost = steps + extra;
     const int take = (int)min((int64_t)(cost - w.j), w.end - w.u);
-    const int j0 = max(0, w.j - p.tile_cost), j1 = max(0, w.j + take - p.tile_cost);
+    const int j0 = max(0, w.j - extra), j1 = max(0, w.j + take - extra);
     s.b = w.b;
     s.h = w.h;
     s.r0 = q.r0;
@@ -112,7 +112,7 @@ __device__ bool next_segment(const AttentionList& p, const StepList list, Walk& 
     s.whole = j1 - j0 == steps;
     if (!s.whole) {
       s.part = j0 > 0 ? 0 : 1;
-      s.c_first = (int)((first + p.tile_cost) / w.per);
+      s.c_first = (int)((first + extra) / w.per);
       s.c_last = (int)((first + cost - 1) / w.per);
     }
     w.u += take;

@@ -59,7 +59,7 @@ struct Cfg {
   static constexpr int BYTES = OFF_MISC + 64 + 1024;
   static constexpr int COL_O = 256;
   // One pair of exponentials in this many is a polynomial on the FMA units (0: none).
-  static constexpr int POLY = DP == 128 ? 0 : 4;
+  static constexpr int POLY = 8;
   static_assert(BYTES <= 227 * 1024, "shared memory per CTA");
 };
 
@@ -715,7 +715,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp < 11) {
       // ---------------- products: a warp for each slot ----------------
       // It follows every load in order (so that no phase of a barrier is taken for another)
-      // and lets go at once of those that its slot does not use.
+      // and lets go at once of those that its slot does not use. A turn is one block's PV and
+      // the next one's scores, with nothing but the products between them: whatever else
+      // they need is waited for before. Slot 0 has the first turn; a slot with fewer blocks
+      // passes its turns on. (Without turns the slots fall into step, and the tensor cores
+      // wait for both.)
       const int t = warp - 9;
       const uint32_t idesc_s = umma_idesc_bf16(kBlock, kBlock);
       const uint32_t idesc_o = umma_idesc_bf16(kBlock, ksteps * 16) | (1u << 16);  // B is contiguous along N
@@ -724,17 +728,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t s_col = tmem + t * kBlock, o_col = tmem + C::COL_O + t * DP;
       uint32_t seq = 0, fixed = 0;  // loads so far; phase of each stage's check
       uint32_t n_p = 0, n_o = 0, n_turn = 0;
-      // A turn: one block's PV and the next one's scores. Slot 0 has the first; a slot with
-      // fewer blocks passes its turns on. Without turns the slots fall into step, and the
-      // tensor cores wait for both.
       auto take_turn = [&]() { return wait(&turn[t], (n_turn++ & 1) ^ (t ^ 1)); };
       auto end_turn = [&]() { mbar_arrive(&turn[t ^ 1]); };
+      auto landed = [&]() { return wait(&full[seq % C::STAGES], (seq / C::STAGES) & 1); };
+      // The scores of a block; the other slot may go on shortly before the end.
+      auto scores = [&](uint32_t q, uint32_t k) {
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          if (i == DP / 32) end_turn();
+          if (i < ksteps)
+            mma_ss(s_col, q + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2,
+                   k + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2, idesc_s, i > 0);
+        }
+        umma_commit(&s_full[t]);
+      };
 #pragma unroll 1
       for (int seg = 0; next(seg); leave(seg), ++seg) {
         if (lane == 0) {
           const Segment& s = segments[seg % kRing];
           const bool pair = s.pair;
-          const uint32_t turns = n_turn + max(s.cnt[0], s.cnt[1]) + 1;
+          const uint32_t turns = n_turn + max(s.cnt[0], s.cnt[1]) + 1, end = seq + 2 * s.n;
           const int n = s.n, cnt = s.cnt[t], buf = pair ? t : s.buf;
           const int checked_from = max(0, s.all_see() / kBlock - s.k0);  // blocks from there on
           bool ok = true;
@@ -744,60 +757,69 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ok = ok && wait(&q_full[buf], s.q_use[buf] & 1);
           if (cnt == 0) mbar_arrive(&q_free[buf]);
-          const uint32_t q = q_desc + buf * (C::TILE >> 4);
-          int x_k = 0, x_v = 0;  // of this slot's blocks
+          const uint32_t q = q_desc + buf * (C::TILE >> 4), first = seq;
+          // Passes over the loads of the other slot's blocks before `to`.
+          auto skip = [&](uint32_t to) {
 #pragma unroll 1
-          for (int at = 0; ok && at < 2 * n; ++at, ++seq) {
-            int c;
-            const bool is_v = nth_load(pair, at, n, c);
-            const uint32_t st = seq % C::STAGES;
-            ok = wait(&full[st], (seq / C::STAGES) & 1);
-            const bool mine = pair ? c < cnt : (c & 1) == t;
-            if (is_v && c >= checked_from) {
-              if (mine) ok = ok && wait(&checked[st], fixed >> st & 1);
-              fixed ^= 1u << st;
+            for (; ok && seq < to; ++seq) {
+              int c;
+              const bool is_v = nth_load(pair, seq - first, n, c);
+              ok = landed();
+              if (is_v && c >= checked_from) fixed ^= 1u << (seq % C::STAGES);
+              if (ok) mbar_arrive(&empty[seq % C::STAGES]);
             }
-            if (!ok) break;
-            if (!mine) {
-              mbar_arrive(&empty[st]);
-              continue;
-            }
-            if (!is_v) {
-              if (x_k == 0) ok = take_turn();
-              if (!ok) break;
+          };
+          if (cnt > 0) {
+            skip(first + (pair ? 0 : t));
+            ok = ok && landed() && take_turn();
+            if (ok) {
               tc_fence_after();
-              const uint32_t k = k_desc + st * (C::TILE >> 4);
-#pragma unroll
-              for (int i = 0; i < DP / 16; ++i)
-                if (i < ksteps)
-                  mma_ss(s_col, q + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2,
-                         k + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2, idesc_s, i > 0);
-              umma_commit(&s_full[t]);
-              end_turn();
-              umma_commit(&empty[st]);
-              if (++x_k == cnt) umma_commit(&q_free[buf]);
-            } else {
-              if (x_v == 0) ok = wait(&o_free[t], (n_o & 1) ^ 1);
+              scores(q, k_desc + seq % C::STAGES * (C::TILE >> 4));
+              umma_commit(&empty[seq % C::STAGES]);
+              if (cnt == 1) umma_commit(&q_free[buf]);
+              ++seq;
+            }
+#pragma unroll 1
+            for (int x = 0; ok && x < cnt; ++x) {
+              const int c = pair ? x : 2 * x + t;
+              skip(first + (pair ? 2 * c + 1 : min(2 * c + 2, 2 * n - 1)));
+              ok = ok && landed();
+              if (!ok) break;
+              const uint32_t st_v = seq % C::STAGES, v = v_desc + st_v * (C::TILE >> 4);
+              if (c >= checked_from) {
+                ok = wait(&checked[st_v], fixed >> st_v & 1);
+                fixed ^= 1u << st_v;
+              }
+              ++seq;
+              const bool more = x + 1 < cnt;  // the next load is this slot's next K
+              const uint32_t st_k = seq % C::STAGES, k = k_desc + st_k * (C::TILE >> 4);
+              if (more) ok = ok && landed();
+              if (x == 0) ok = ok && wait(&o_free[t], (n_o & 1) ^ 1);
               ok = ok && wait(&p_half[t], n_p & 1) && take_turn();
               if (!ok) break;
               tc_fence_after();
-              const uint32_t v = v_desc + st * (C::TILE >> 4);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) mma_ts(o_col, s_col + i * 8, v + i * (2048 >> 4), idesc_o, x_v > 0 || i > 0);
+              for (int i = 0; i < 4; ++i) mma_ts(o_col, s_col + i * 8, v + i * (2048 >> 4), idesc_o, x > 0 || i > 0);
               ok = wait(&p_full[t], n_p & 1);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll
               for (int i = 4; i < 8; ++i) mma_ts(o_col, s_col + i * 8, v + i * (2048 >> 4), idesc_o, true);
               ++n_p;
-              umma_commit(&empty[st]);
-              if (++x_v == cnt) {
+              if (more) {
+                scores(q, k);
+                umma_commit(&empty[st_k]);
+                if (x + 2 == cnt) umma_commit(&q_free[buf]);
+                ++seq;
+              } else {
+                end_turn();
                 umma_commit(&o_full[t]);
                 ++n_o;
-                end_turn();
               }
+              umma_commit(&empty[st_v]);
             }
           }
+          skip(end);
 #pragma unroll 1
           while (ok && n_turn < turns) {
             ok = take_turn();
