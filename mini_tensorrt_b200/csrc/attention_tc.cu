@@ -20,14 +20,13 @@
 // the lengths in device memory. A tile cut between CTAs leaves partial (m, l, O) in the
 // workspace, and the CTA that finishes last joins them in order.
 //
-// One CTA = 12 warps: 0..3 and 4..7 the slots' softmax (a thread per row, also the
-// epilogue), 8 TMA loads, 9 and 10 issue the slots' products, 11 looks over the V blocks that not every row
+// One CTA = 20 warps: 0..7 and 8..15 the slots' softmax (two threads per row, of 64 keys
+// each, also the epilogue), 16 TMA loads, 17 and 18 issue the slots' products, 19 looks over
+// the V blocks that not every row
 // sees whole: rows past the request's keys are zeroed (a page's unused rows, the next
 // request's rows: 0 * NaN would reach O), and infinities and NaN in rows that only later
 // tokens see are taken out and listed; the epilogue adds them to the rows that see them.
 #include <math.h>
-
-#include <type_traits>
 
 #include "../../include/mtrtq.h"
 #include "attention_sched.cuh"
@@ -38,7 +37,8 @@ namespace mtrtq {
 namespace {
 
 constexpr int kBlock = 128;  // keys per block, rows per slot
-constexpr int kThreads = 384;
+constexpr int kThreads = 640;
+constexpr int kLoadWarp = 16;  // after the softmax warps
 constexpr int kBadMax = 384;  // listed V rows of a tile: three blocks
 
 constexpr int kRing = 4;  // segments that the roles may lie apart
@@ -52,14 +52,13 @@ struct Cfg {
   static constexpr int OFF_LIST = OFF_KV + STAGES * TILE;
   static constexpr int OFF_SEG = OFF_LIST + MTRTQ_MAX_BATCH * sizeof(Request);
   static constexpr int OFF_ML = OFF_SEG + kRing * ((sizeof(Segment) + 15) / 16 * 16);  // slot 1's (m, l)
-  static constexpr int OFF_BAD = OFF_ML + kBlock * 8;                                  // [kRing][kBadMax] keys
+  static constexpr int OFF_TOP = OFF_ML + kBlock * 8;  // [2 phases][2 slots][2 halves][rows]
+  static constexpr int OFF_BAD = OFF_TOP + 8 * kBlock * 4;                                  // [kRing][kBadMax] keys
   static constexpr int OFF_BAR = OFF_BAD + kRing * kBadMax * 4;
   static constexpr int NBAR = 3 * STAGES + 2 * kRing + 22;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
-  static constexpr int BYTES = OFF_MISC + 64 + 1024;
+  static constexpr int BYTES = OFF_MISC + 128 + 1024;
   static constexpr int COL_O = 256;
-  // One pair of exponentials in this many is a polynomial on the FMA units (0: none).
-  static constexpr int POLY = 8;
   static_assert(BYTES <= 227 * 1024, "shared memory per CTA");
 };
 
@@ -137,43 +136,23 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Largest of three, NaN if any is.
+// Largest of three.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-// 32 bf16 of a row (`left` of them, whole groups of 8, if fewer are left): 32 bytes at a
-// time where the rows allow it, as every row is a line of its own.
-__device__ __forceinline__ void store_row(__nv_bfloat16* out, const uint32_t (&u)[16], int left, bool by32) {
-  if (by32 && left >= 32) {
-#pragma unroll
-    for (int y = 0; y < 16; y += 8)
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + 2 * y), "r"(u[y]),
-                   "r"(u[y + 1]), "r"(u[y + 2]), "r"(u[y + 3]), "r"(u[y + 4]), "r"(u[y + 5]), "r"(u[y + 6]),
-                   "r"(u[y + 7])
-                   : "memory");
+// 16 bf16 of a row, or 8 if only 8 are left: 32 bytes at a time where the rows allow it, as
+// every row is a line of its own.
+__device__ __forceinline__ void store_row(__nv_bfloat16* out, const uint32_t* u, int left, bool by32) {
+  if (by32 && left >= 16) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "r"(u[0]), "r"(u[1]), "r"(u[2]),
+                 "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+                 : "memory");
     return;
   }
-#pragma unroll
-  for (int y = 0; y < 16; y += 4)
-    if (2 * y < left) *reinterpret_cast<uint4*>(out + 2 * y) = make_uint4(u[y], u[y + 1], u[y + 2], u[y + 3]);
-}
-// 2^x for finite x <= 8, below 2^-126 rounded up to about that: x = n + f with n whole and
-// |f| <= 1/2, 2^f by the cubic with the least relative error (7.5e-5, an eighth of a bf16
-// rounding), n added to the exponent.
-__device__ __forceinline__ float2 exp2_cubic(float2 x) {
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
-  const float2 big = make_float2(12582912.0f, 12582912.0f), nbig = make_float2(-12582912.0f, -12582912.0f);
-  const float2 t = __fadd2_rn(x, big);  // n in the low bits
-  const float2 n = __fadd2_rn(t, nbig);
-  const float2 f = __fadd2_rn(x, make_float2(-n.x, -n.y));
-  float2 y = fma2(f, make_float2(0.0551716685f, 0.0551716685f), make_float2(0.2426111251f, 0.2426111251f));
-  y = fma2(y, f, make_float2(0.6932609677f, 0.6932609677f));
-  y = fma2(y, f, make_float2(0.9999280572f, 0.9999280572f));
-  return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(y.x)),
-                     __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(y.y)));
+  *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+  if (left > 8) *reinterpret_cast<uint4*>(out + 8) = make_uint4(u[4], u[5], u[6], u[7]);
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
@@ -241,9 +220,10 @@ __device__ __forceinline__ void rescale(uint32_t o_addr, float keep) {
   }
 }
 
-// One row of a cut tile from the parts of CTAs c_first .. c_last, in order.
+// Dimensions d0 .. d1 - 1 of one row of a cut tile from the parts of CTAs c_first .. c_last, in order.
 template <int DP>
-__device__ __forceinline__ void join_parts(const TcAttention& p, int c_first, int c_last, int prow, __nv_bfloat16* out) {
+__device__ __forceinline__ void join_parts(const TcAttention& p, int c_first, int c_last, int prow, int d0, int d1,
+                                           __nv_bfloat16* out) {
   const int64_t rows = p.part_rows;
   float top = -INFINITY;
 #pragma unroll 1
@@ -257,7 +237,7 @@ __device__ __forceinline__ void join_parts(const TcAttention& p, int c_first, in
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll 1
-  for (int i = 0; i < p.head_dim; i += 8) {
+  for (int i = d0; i < d1; i += 8) {
     float o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
     for (int c = c_first; c <= c_last; ++c) {
@@ -293,6 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   // the prefix lies where K and V will
   const StepList list = {reinterpret_cast<Request*>(smem + C::OFF_LIST), reinterpret_cast<int64_t*>(smem + C::OFF_KV)};
+  float* tops = reinterpret_cast<float*>(smem + C::OFF_TOP);
   float2* ml1 = reinterpret_cast<float2*>(smem + C::OFF_ML);
   int* bad = reinterpret_cast<int*>(smem + C::OFF_BAD);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
@@ -301,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = checked + C::STAGES;  // [2], a barrier for each slot or buffer
   uint64_t* q_free = q_full + 2;
   uint64_t* s_full = q_free + 2;
-  uint64_t* p_half = s_full + 2;           // the weights of the block's first 64 keys
+  uint64_t* p_half = s_full + 2;           // the weights of the block's first 64 keys, and O rescaled
   uint64_t* p_full = p_half + 2;
   uint64_t* o_full = p_full + 2;
   uint64_t* o_free = o_full + 2;
@@ -331,37 +312,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[t], 1);
       mbar_init(&q_free[t], 2);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_half[t], 4);
+      mbar_init(&p_half[t], 8);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
-      mbar_init(&o_free[t], 4);
+      mbar_init(&o_free[t], 8);
       mbar_init(&turn[t], 1);
     }
     mbar_init(&drained[0], 1);
     mbar_init(&drained[1], 1);
     mbar_init(ml_full, 4);
-    mbar_init(ml_free, 4);
-    mbar_init(cut_in, 8);
+    mbar_init(ml_free, 8);
+    mbar_init(cut_in, 16);
+    for (int x = 0; x < 8; ++x) misc[8 + x] = 0;
     mbar_init(cut_out, 1);
     for (int r = 0; r < kRing; ++r) {
       mbar_init(&seg_full[r], 1);
-      mbar_init(&seg_free[r], 11);  // 8 softmax warps, 2 of products, the check
+      mbar_init(&seg_free[r], kLoadWarp + 3);  // all but the load warp
       bad_count[r] = 0;
     }
     *s_abort = 0;
     fence_barrier_init();
   }
-  if (warp == 9) {
+  if (warp == kLoadWarp + 1) {
     tmem_alloc(misc, 512);
     tmem_relinquish();
   }
-  if (warp == 8 && lane == 0) {
+  if (warp == kLoadWarp && lane == 0) {
     prefetch_tensormap(&qmap);
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
   tc_fence_before();
-  Walk walk;  // warp 0's, and warp 8's: it makes the segments
+  Walk walk;  // the load warp makes the segments
   make_list<kBlock, kThreads>(p, list, walk, reinterpret_cast<Walk*>(smem + C::OFF_SEG));
   tc_fence_after();
   const uint32_t tmem = misc[0];
@@ -381,18 +363,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) mbar_arrive(&seg_free[seg % kRing]);
   };
 
-  // 256 threads of 208 registers and 128 of 88: the 384 x 168 of the launch.
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  // 512 threads of 104 registers and 128 of 64: the 640 x 96 of the launch.
+  if (warp < kLoadWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // ---------------- softmax and epilogue ----------------
-    const int t = warp >> 2;                           // slot
-    const int row = tid & 127;                         // of the slot's tile
+    const int t = warp >> 3, half = (warp >> 2) & 1;   // slot; which 64 keys, and half of the dimensions
+    const int row = (warp & 3) * 32 + lane;            // of the slot's tile
     const uint32_t quad = (uint32_t)(warp & 3) << 21;  // lanes 32 (warp & 3) .. of TMEM
-    const uint32_t s_addr = tmem + quad + t * kBlock, o_addr = tmem + quad + C::COL_O + t * DP;
+    const uint32_t s_addr = tmem + quad + t * kBlock + half * 64;  // scores
+    const uint32_t p_addr = tmem + quad + t * kBlock + half * 32;  // weights, two keys a column
+    const uint32_t o_addr = tmem + quad + C::COL_O + t * DP;
+    const int d0 = half * (DP / 2), d1 = min(p.head_dim, d0 + DP / 2);
+    volatile int* const pair_failed = reinterpret_cast<volatile int*>(misc + 8) + t * 4 + (warp & 3);
+    float* const mine_top = tops + (t * 2 + half) * kBlock + row;
+    const float* const other_top = tops + (t * 2 + (half ^ 1)) * kBlock + row;
     const int token = row / p.group, head = row - token * p.group;
     const float c2 = p.scale * 1.4426950408889634f;  // scale log2 e
     const float2 cc = make_float2(c2, c2);
-    uint32_t n_s = 0, n_o = 0;
+    uint32_t n_s = 0, n_o = 0, n_x = 0;
+    // Gives this half's value of the row to the other half's thread, and gets its; false
+    // if either warp's last wait gave up (so both leave together: this barrier has no limit,
+    // but neither warp can fail to reach it).
+    auto swap = [&](bool fine, float x, float& y) {
+      const uint32_t at = (n_x++ & 1) * 4 * kBlock;
+      mine_top[at] = x;
+      if (!fine) *pair_failed = 1;
+      named_bar_sync(1 + t * 4 + (warp & 3), 64);
+      y = other_top[at];
+      return *pair_failed == 0;
+    };
     uint32_t n_ml = 0, n_cut = 0;
     bool ok = true;
 #pragma unroll 1
@@ -404,117 +403,87 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int keys = live ? max(0, min(s.see0 + tok, s.keys)) : 0;  // that this row sees
       const bool warp_live = __any_sync(0xffffffffu, live);
       const int cnt = s.cnt[t], stride = pair ? kBlock : 2 * kBlock;
-      int left = keys - (s.k0 + (pair ? 0 : t)) * kBlock;  // columns of the block that it sees
+      int left = keys - (s.k0 + (pair ? 0 : t)) * kBlock - half * 64;  // of these 64 columns
       float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
       for (int x = 0; x < cnt; ++x, left -= stride, ++n_s) {
         ok = warp_wait(&s_full[t], n_s & 1);
-        if (!ok) break;
         if (!warp_live) {
+          if (!ok) break;
           if (lane == 0) {
             mbar_arrive(&p_half[t]);
-            mbar_arrive(&p_full[t]);
+            if (half) mbar_arrive(&p_full[t]);
           }
           continue;
         }
         tc_fence_after();
-        float v[kBlock];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32(s_addr + 32 * i, v + 32 * i);
+        float v[64];
+        tmem_ld32(s_addr, v);
+        tmem_ld32(s_addr + 32, v + 32);
         tmem_wait_ld();
-        float top;
-        {
-          float a[4] = {v[0], v[1], v[2], v[3]};
+        if (__any_sync(0xffffffffu, left < 64)) {
 #pragma unroll
-          for (int i = 4; i + 7 < kBlock; i += 8) {
-#pragma unroll
-            for (int y = 0; y < 4; ++y) a[y] = max3(a[y], v[i + 2 * y], v[i + 2 * y + 1]);
-          }
-          a[0] = max3(a[0], v[kBlock - 4], v[kBlock - 3]);
-          a[1] = max3(a[1], v[kBlock - 2], v[kBlock - 1]);
-          top = max3(a[0], a[1], max3(a[2], a[3], a[3])) * c2;
+          for (int i = 0; i < 64; ++i) v[i] = i < left ? v[i] : -INFINITY;
         }
-        // Masked, infinite or NaN scores: read again and masked, in short loops, and every
-        // exponential by the instruction, which keeps them exact.
-        const bool slow = __any_sync(0xffffffffu, left < kBlock || !(fabsf(top) < INFINITY));
-        float2 sum = make_float2(0.0f, 0.0f);
-        // Takes the block's maximum into account; the exponent's -m'.
-        auto raise = [&](float block_top) {
-          const bool grow = block_top > m + 8.0f || (m == -INFINITY && block_top > m);
-          if (__any_sync(0xffffffffu, grow)) {
-            const float m1 = grow ? block_top : m;
-            const float keep = m1 == -INFINITY ? 1.0f : ex2(m - m1);
-            l *= keep;
-            m = m1;
-            if (x > 0) rescale<DP>(o_addr, keep);  // the earlier products are complete: these scores came after them
-          }
-          return m == -INFINITY ? 0.0f : -m;
-        };
-        auto half_done = [&]() {
+        // The largest score (NaN ones aside: they make the sum NaN).
+        float a[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int i = 4; i + 7 < 64; i += 8) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) a[y] = max3(a[y], v[i + 2 * y], v[i + 2 * y + 1]);
+        }
+        a[0] = max3(a[0], v[60], v[61]);
+        a[1] = max3(a[1], v[62], v[63]);
+        // The row's other half. Past the swap both have read their scores, which the
+        // weights overwrite.
+        float top = max3(a[0], a[1], fmaxf(a[2], a[3])), other;
+        ok = swap(ok, top, other);
+        if (!ok) break;
+        top = fmaxf(top, other) * c2;
+        const bool grow = top > m + 8.0f || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m1 = grow ? top : m;
+          const float keep = m1 == -INFINITY ? 1.0f : ex2(m - m1);
+          l *= keep;
+          m = m1;
+          if (x > 0) rescale<DP / 2>(o_addr + d0, keep);  // the earlier products are complete: these scores came after
+        }
+        if (half) {
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_half[t]);
-        };
-        if (!slow) {
-          const float mm1 = raise(top);
-          const float2 mm = make_float2(mm1, mm1);
-#pragma unroll
-          for (int i = 0; i < kBlock; i += 32) {
-            uint32_t w[16];
-#pragma unroll
-            for (int y = 0; y < 16; ++y) {
-              float2 e = fma2(make_float2(v[i + 2 * y], v[i + 2 * y + 1]), cc, mm);
-              if (C::POLY && y % (C::POLY ? C::POLY : 1) == C::POLY - 1) {
-                e = exp2_cubic(e);
-              } else {
-                e.x = ex2(e.x);
-                e.y = ex2(e.y);
-              }
-              sum = __fadd2_rn(sum, e);
-              w[y] = pack_bf16(e.x, e.y);
-            }
-            tmem_st16(s_addr + (i >> 1), w);
-            if (i == kBlock / 2 - 32) half_done();
-          }
-        } else {
-          top = -INFINITY;
-#pragma unroll 1
-          for (int i = 0; i < kBlock; i += 32) {
-            float u[32];
-            tmem_ld32(s_addr + i, u);
-            tmem_wait_ld();
-#pragma unroll
-            for (int y = 0; y < 32; ++y) top = fmaxf(top, i + y < left ? u[y] * c2 : -INFINITY);
-          }
-          const float mm1 = raise(top);
-          const float2 mm = make_float2(mm1, mm1);
-#pragma unroll 1
-          for (int i = 0; i < kBlock; i += 32) {  // P's columns so far lie before the scores still to be read
-            float u[32];
-            tmem_ld32(s_addr + i, u);
-            tmem_wait_ld();
-            uint32_t w[16];
-#pragma unroll
-            for (int y = 0; y < 16; ++y) {
-              float2 e = fma2(make_float2(i + 2 * y < left ? u[2 * y] : -INFINITY,
-                                          i + 2 * y + 1 < left ? u[2 * y + 1] : -INFINITY), cc, mm);
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-              sum = __fadd2_rn(sum, e);
-              w[y] = pack_bf16(e.x, e.y);
-            }
-            tmem_st16(s_addr + (i >> 1), w);
-            if (i == kBlock / 2 - 32) half_done();
-          }
         }
+        const float base = m == -INFINITY ? 0.0f : -m;
+        const float2 mm = make_float2(base, base);
+        float2 sum = make_float2(0.0f, 0.0f), sum1 = sum;
+#pragma unroll
+        for (int i = 0; i < 64; i += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            float2 e = fma2(make_float2(v[i + 2 * y], v[i + 2 * y + 1]), cc, mm);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            if (y & 1) sum1 = __fadd2_rn(sum1, e);
+            else sum = __fadd2_rn(sum, e);
+            w[y] = pack_bf16(e.x, e.y);
+          }
+          tmem_st16(p_addr + (i >> 1), w);
+        }
+        sum = __fadd2_rn(sum, sum1);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(half ? &p_full[t] : &p_half[t]);
         l += sum.x + sum.y;
       }
       if (!ok) break;
+      if (warp_live) {  // the row's sum: its first half's and its second's
+        float other;
+        swap(true, l, other);
+        l = half ? other + l : l + other;
+      }
 
       if (m == -INFINITY && l != l) m = 0.0f;  // every score it saw was NaN
       if (cnt > 0) {
@@ -526,12 +495,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mine = pair || t == 0, two = !pair && s.n > 1, whole = s.whole;
       float w0 = 1.0f, w1 = 0.0f;
       if (two) {
-        if (t == 1) {
+        if (t == 1 && half == 0) {
           ok = warp_wait(ml_free, (n_ml & 1) ^ 1);
           ml1[row] = make_float2(m, l);
           __syncwarp();
           if (lane == 0) mbar_arrive(ml_full);
-        } else {
+        } else if (t == 0) {
           ok = warp_wait(ml_full, n_ml & 1);  // slot 1's warps have waited for their products
           const float2 ml = ml1[row];
           __syncwarp();
@@ -558,35 +527,34 @@ __global__ void __launch_bounds__(kThreads, 1)
           w1 *= inv;
         }
 #pragma unroll 1
-        for (int i = 0; i < p.head_dim; i += 32) {
-          float o[32];
+        for (int i = d0; i < d1; i += 16) {
+          uint32_t u[16];
+          float o[16];
           if (cnt > 0) {
-            tmem_ld32(o_addr + i, o);
+            tmem_ld_32x32b_x16(o_addr + i, u);
             tmem_wait_ld();
           }
 #pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = w0 == 0.0f ? 0.0f : o[y] * w0;
+          for (int y = 0; y < 16; ++y) o[y] = w0 == 0.0f ? 0.0f : __uint_as_float(u[y]) * w0;
           if (two) {
-            float o1[32];
-            tmem_ld32(o_addr + DP + i, o1);
+            tmem_ld_32x32b_x16(o_addr + DP + i, u);
             tmem_wait_ld();
 #pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] += w1 == 0.0f ? 0.0f : o1[y] * w1;
+            for (int y = 0; y < 16; ++y) o[y] += w1 == 0.0f ? 0.0f : __uint_as_float(u[y]) * w1;
           }
           if (!live) continue;
           if (whole) {
-            uint32_t u[16];
 #pragma unroll
-            for (int y = 0; y < 16; ++y) u[y] = pack_bf16(o[2 * y], o[2 * y + 1]);
-            store_row(out + i, u, p.head_dim - i, p.out32);
+            for (int y = 0; y < 8; ++y) u[y] = pack_bf16(o[2 * y], o[2 * y + 1]);
+            store_row(out + i, u, d1 - i, p.out32);
           } else {
 #pragma unroll
-            for (int y = 0; y < 32; y += 4)
+            for (int y = 0; y < 16; y += 4)
               __stcg(reinterpret_cast<float4*>(to_part + (int64_t)(i + y) * p.part_rows),
                      make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]));
           }
         }
-        if (live && !whole) __stcg(p.part_ml + part * p.part_rows + prow, make_float2(m, l));
+        if (live && half == 0 && !whole) __stcg(p.part_ml + part * p.part_rows + prow, make_float2(m, l));
         // The infinities and NaN that were taken out of the last blocks' V, for the rows
         // that see them. A slot without blocks here has not waited for the check, and
         // sees none of it.
@@ -604,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               src = p.v + (int64_t)(s.r0 + key) * p.v_row + s.h * p.v_head;
             }
 #pragma unroll 1
-            for (int d = 0; d < p.head_dim; ++d) {
+            for (int d = d0; d < d1; ++d) {
               const float z = __bfloat162float(src[d]);
               if (fabsf(z) < INFINITY) continue;
               if (whole) {
@@ -636,15 +604,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (mine) {
           ok = warp_wait(cut_out, n_cut & 1);
           const bool last = *s_ticket == (unsigned)(s.c_last - s.c_first);
-          if (ok && last && live) join_parts<DP>(p, s.c_first, s.c_last, prow, out);
+          if (ok && last && live) join_parts<DP>(p, s.c_first, s.c_last, prow, d0, d1, out);
           if (last && tid == 0) p.counters[s.c_first] = 0u;
         }
         ++n_cut;
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == kLoadWarp) {
       // ---------------- loads ----------------
       uint32_t seq = 0;
       int q_sent[2] = {0, 0};
@@ -712,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           drain(&full[x % C::STAGES], (x / C::STAGES) & 1);
       }
       __syncwarp();
-    } else if (warp < 11) {
+    } else if (warp < kLoadWarp + 3) {
       // ---------------- products: a warp for each slot ----------------
       // It follows every load in order (so that no phase of a barrier is taken for another)
       // and lets go at once of those that its slot does not use. A turn is one block's PV and
@@ -720,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // they need is waited for before. Slot 0 has the first turn; a slot with fewer blocks
       // passes its turns on. (Without turns the slots fall into step, and the tensor cores
       // wait for both.)
-      const int t = warp - 9;
+      const int t = warp - kLoadWarp - 1;
       const uint32_t idesc_s = umma_idesc_bf16(kBlock, kBlock);
       const uint32_t idesc_o = umma_idesc_bf16(kBlock, ksteps * 16) | (1u << 16);  // B is contiguous along N
       const uint32_t q_desc = desc_qk(smem_u32(smem + C::OFF_Q)), k_desc = desc_qk(smem_u32(smem + C::OFF_KV)),
@@ -795,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const uint32_t st_k = seq % C::STAGES, k = k_desc + st_k * (C::TILE >> 4);
               if (more) ok = ok && landed();
               if (x == 0) ok = ok && wait(&o_free[t], (n_o & 1) ^ 1);
-              ok = ok && wait(&p_half[t], n_p & 1) && take_turn();
+              ok = ok && take_turn() && wait(&p_half[t], n_p & 1);
               if (!ok) break;
               tc_fence_after();
 #pragma unroll
@@ -908,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kLoadWarp + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
