@@ -31,7 +31,7 @@ __device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY;
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 4096;   // logits of one row that a block looks at, 16 per thread
-constexpr int kGroups = 64;    // of 4 threads: their maxima bound a chunk's best from below
+constexpr int kGroups = 64;    // of 4 threads: their maxima bound the best keys from below
 constexpr int kList = 256;     // candidates above that bound which are ranked side by side
 
 // Workspace: a ticket per request, 4 KiB of them | per row and chunk (max, sum of exponentials) | per row
@@ -64,28 +64,14 @@ struct BeamArgs {
   unsigned long long* keys;
 };
 
-__device__ float block_max(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) v = fmaxf(v, red[w]);
-  return v;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-__device__ float block_sum(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-#pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) v += red[w];
-  return v;
-}
+// exp(x - m): the difference first, so that a large m costs no bits of the exponent.
+__device__ __forceinline__ float exp_below(float x, float m) { return ex2((x - m) * 1.4426950408889634f); }
+
 __device__ unsigned long long block_best(unsigned long long k, unsigned long long* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -107,7 +93,9 @@ struct Shared {
   unsigned long long group[kGroups];
   unsigned long long best[MTRTQ_MAX_BEAMS + 1];
   float lse[MTRTQ_MAX_BEAMS];
-  int count, flag;
+  int count;
+  // of a chunk
+  float group_max[kGroups], warp_max[kThreads / 32], warp_sum[kThreads / 32], bound;
 };
 
 // The `want` largest of the block's keys (distinct, 0 = none), best first, in sh.best; 0
@@ -186,7 +174,6 @@ __device__ __forceinline__ float row_score(float base, float x, float lse) {
 // again (also when the candidates left are all -infinity).
 __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ BeamArgs p) {
   __shared__ Shared sh;
-  __shared__ float red[kThreads / 32];
   __shared__ unsigned ticket;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int chunk = blockIdx.x, w0 = blockIdx.y, want = p.beams + 1;
@@ -196,34 +183,111 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
   const int64_t part = row * p.chunks + chunk;
   const bool used = p.done[row] == 0 && p.scores[row] > -INFINITY;
   if (used) {
+    // 16-byte loads from the boundary before the row's first logit on
+    const int t0 = chunk * kChunk + tid * 4 - shift;
+    const bool inside = chunk > 0 && (chunk + 1) * kChunk - shift <= p.vocab;
     float v[16];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      // 16-byte loads from the boundary before the row's first logit on
-      const int t = chunk * kChunk + (j * kThreads + tid) * 4 - shift;
+      const int t = t0 + j * kThreads * 4;
       float4 u = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      if (t < p.vocab && t + 3 >= 0) u = __ldcs(reinterpret_cast<const float4*>(x + t));
-      v[4 * j] = t >= 0 && t < p.vocab ? logit(u.x) : -INFINITY;
-      v[4 * j + 1] = t + 1 >= 0 && t + 1 < p.vocab ? logit(u.y) : -INFINITY;
-      v[4 * j + 2] = t + 2 >= 0 && t + 2 < p.vocab ? logit(u.z) : -INFINITY;
-      v[4 * j + 3] = t + 3 >= 0 && t + 3 < p.vocab ? logit(u.w) : -INFINITY;
+      if (inside || (t < p.vocab && t + 3 >= 0)) u = __ldcs(reinterpret_cast<const float4*>(x + t));
+      v[4 * j] = u.x;
+      v[4 * j + 1] = u.y;
+      v[4 * j + 2] = u.z;
+      v[4 * j + 3] = u.w;
     }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = fmaxf(v[j], -INFINITY);  // NaN counts as -infinity
+    if (!inside) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int t = t0 + (j >> 2) * kThreads * 4 + (j & 3);
+        if (t < 0 || t >= p.vocab) v[j] = -INFINITY;
+      }
+    }
+    // Maxima of groups of threads (32 of eight while they bound `want` keys well, else 64 of
+    // four) and of the warp; the warp's sum below its own maximum.
+    const int group = want <= 16 ? 8 : 4, groups = kThreads / group;
     float m = v[0];
 #pragma unroll
     for (int j = 1; j < 16; ++j) m = fmaxf(m, v[j]);
-    m = block_max(m, red);
-    float s = 0.0f;
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if (group == 4 && (lane & 3) == 0) sh.group_max[tid >> 2] = m;
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+    if (group == 8 && (lane & 7) == 0) sh.group_max[tid >> 3] = m;
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) s += exp2f((v[j] - m) * 1.4426950408889634f);
-    s = block_sum(s, red);
-    if (tid == 0) __stcg(p.stats + part, make_float2(m, m == -INFINITY ? 0.0f : s));
-    block_top(want, sh, [&](auto f) {
+    for (int j = 0; j < 16; ++j) s[j & 3] += exp_below(v[j], m);
+    float sum = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (v[j] > -INFINITY)
-          f(candidate_key(v[j], (uint32_t)(chunk * kChunk + ((j >> 2) * kThreads + tid) * 4 + (j & 3) - shift)));
-    });
-    if (tid < want) __stcg(p.keys + part * want + tid, sh.best[tid]);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      sh.warp_max[warp] = m;
+      sh.warp_sum[warp] = m == -INFINITY ? 0.0f : sum;
+    }
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    if (tid < groups) {
+      // the want-th largest of the groups' maxima
+      const float mine = sh.group_max[tid];
+      int above = 0;
+#pragma unroll 8
+      for (int g = 0; g < groups; ++g) {
+        const float o = sh.group_max[g];
+        above += o > mine || (o == mine && g < tid);
+      }
+      if (above == want - 1) sh.bound = mine;
+    } else if (tid == kThreads - 1) {
+      float top = sh.warp_max[0], all = 0.0f;
+#pragma unroll
+      for (int w = 1; w < kThreads / 32; ++w) top = fmaxf(top, sh.warp_max[w]);
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w)
+        all += sh.warp_max[w] == top ? sh.warp_sum[w] : sh.warp_sum[w] * exp_below(sh.warp_max[w], top);
+      __stcg(p.stats + part, make_float2(top, all));
+    }
+    __syncthreads();
+    const float bound = sh.bound;
+    auto key = [&](int j) {
+      return candidate_key(v[j], (uint32_t)(t0 + (j >> 2) * kThreads * 4 + (j & 3)));
+    };
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (v[j] >= bound && v[j] > -INFINITY) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kList) sh.list[at] = key(j);
+      }
+    }
+    __syncthreads();
+    const int have = sh.count;
+    unsigned long long* out = p.keys + part * want;
+    if (have <= kList) {
+      if (tid < have) {
+        const unsigned long long mine = sh.list[tid];
+        int above = 0;
+        for (int e = 0; e < have; ++e) above += sh.list[e] > mine;
+        if (above < want) __stcg(out + above, mine);
+      } else if (tid < want) {
+        __stcg(out + tid, 0ull);
+      }
+    } else {
+      // many logits reach the bound (equal ones, as a rule): a block-wide maximum each
+      unsigned long long below = ~0ull;
+      for (int i = 0; i < want; ++i) {
+        unsigned long long k = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const unsigned long long c = v[j] > -INFINITY ? key(j) : 0ull;
+          k = c < below && c > k ? c : k;
+        }
+        below = block_best(k, sh.red);
+        if (tid == 0) __stcg(out + i, below);
+      }
+    }
   }
   __syncthreads();
   if (tid == 0) ticket = ticket_acq_rel(p.tickets + request);
@@ -241,7 +305,7 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       for (int c = lane; c < p.chunks; c += 32) {
         const float2 st = __ldcg(p.stats + r * p.chunks + c);
-        s += st.x == m ? st.y : st.y * exp2f((st.x - m) * 1.4426950408889634f);
+        s += st.x == m ? st.y : st.y * exp_below(st.x, m);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
