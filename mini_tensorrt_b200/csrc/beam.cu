@@ -30,19 +30,24 @@ __device__ __forceinline__ uint32_t key_index(unsigned long long key) { return ~
 __device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY; }
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 4096;   // logits of one row that a block looks at, 16 per thread
+// Logits of one row that a block looks at: 16 per thread, 32 where that still leaves every
+// SM several blocks (a block's fixed cost is that of some 20 logits per thread; for a few
+// rows more blocks finish sooner). 64 x 8 x 50257 on a B200: 41.8 us with 32, 48.9 with 16.
+constexpr int kChunk = 4096;
 constexpr int kGroups = 64;    // of 4 threads: their maxima bound the best keys from below
 constexpr int kList = 256;     // candidates above that bound which are ranked side by side
 
 // Workspace: a ticket per request, 4 KiB of them | per row and chunk (max, sum of exponentials) | per row
 // and chunk beams + 1 keys (logit, index in the row), best first, 0 where there are fewer.
 struct BeamLayout {
-  int chunks;
+  int chunk, chunks;
   size_t off_stats, off_keys, total;
 };
 inline BeamLayout beam_layout(int64_t requests, int64_t beams, int64_t vocab) {
   BeamLayout l;
-  l.chunks = (int)((vocab + 3 + kChunk - 1) / kChunk);  // rows start up to 3 floats past 16 bytes
+  // rows start up to 3 floats past 16 bytes
+  l.chunk = requests * beams * ((vocab + 3) / kChunk) >= 3072 ? 2 * kChunk : kChunk;
+  l.chunks = (int)((vocab + 3 + l.chunk - 1) / l.chunk);
   const size_t parts = (size_t)requests * beams * l.chunks;
   l.off_stats = 4096;
   l.off_keys = (l.off_stats + parts * sizeof(float2) + 255) & ~(size_t)255;
@@ -55,7 +60,7 @@ struct BeamArgs {
   int64_t ldl;
   const float* scores;
   const uint8_t* done;
-  int eos, beams, vocab, chunks;
+  int eos, beams, vocab, chunk, chunks;
   float* out_scores;
   int32_t *parent, *token;
   uint8_t* out_done;
@@ -172,7 +177,8 @@ __device__ __forceinline__ float row_score(float base, float x, float lse) {
 // of the first one left out, at most that of the last one passed on, no worse than the
 // last beam chosen: where a chunk's (beams + 1)-th does reach it, its logits are looked at
 // again (also when the candidates left are all -infinity).
-__global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ BeamArgs p) {
+template <int E>
+__global__ void __launch_bounds__(kThreads, 5) beam_kernel(const __grid_constant__ BeamArgs p) {
   __shared__ Shared sh;
   __shared__ unsigned ticket;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -184,11 +190,11 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
   const bool used = p.done[row] == 0 && p.scores[row] > -INFINITY;
   if (used) {
     // 16-byte loads from the boundary before the row's first logit on
-    const int t0 = chunk * kChunk + tid * 4 - shift;
-    const bool inside = chunk > 0 && (chunk + 1) * kChunk - shift <= p.vocab;
-    float v[16];
+    const int t0 = chunk * E * kThreads + tid * 4 - shift;
+    const bool inside = chunk > 0 && (chunk + 1) * E * kThreads - shift <= p.vocab;
+    float v[E];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < E / 4; ++j) {
       const int t = t0 + j * kThreads * 4;
       float4 u = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       if (inside || (t < p.vocab && t + 3 >= 0)) u = __ldcs(reinterpret_cast<const float4*>(x + t));
@@ -198,10 +204,10 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
       v[4 * j + 3] = u.w;
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = fmaxf(v[j], -INFINITY);  // NaN counts as -infinity
+    for (int j = 0; j < E; ++j) v[j] = fmaxf(v[j], -INFINITY);  // NaN counts as -infinity
     if (!inside) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < E; ++j) {
         const int t = t0 + (j >> 2) * kThreads * 4 + (j & 3);
         if (t < 0 || t >= p.vocab) v[j] = -INFINITY;
       }
@@ -211,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
     const int group = want <= 16 ? 8 : 4, groups = kThreads / group;
     float m = v[0];
 #pragma unroll
-    for (int j = 1; j < 16; ++j) m = fmaxf(m, v[j]);
+    for (int j = 1; j < E; ++j) m = fmaxf(m, v[j]);
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     if (group == 4 && (lane & 3) == 0) sh.group_max[tid >> 2] = m;
@@ -221,7 +227,7 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) s[j & 3] += exp_below(v[j], m);
+    for (int j = 0; j < E; ++j) s[j & 3] += exp_below(v[j], m);
     float sum = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
       return candidate_key(v[j], (uint32_t)(t0 + (j >> 2) * kThreads * 4 + (j & 3)));
     };
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < E; ++j) {
       if (v[j] >= bound && v[j] > -INFINITY) {
         const int at = atomicAdd(&sh.count, 1);
         if (at < kList) sh.list[at] = key(j);
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
       for (int i = 0; i < want; ++i) {
         unsigned long long k = 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+        for (int j = 0; j < E; ++j) {
           const unsigned long long c = v[j] > -INFINITY ? key(j) : 0ull;
           k = c < below && c > k ? c : k;
         }
@@ -353,8 +359,8 @@ __global__ void __launch_bounds__(kThreads) beam_kernel(const __grid_constant__ 
         const float* y = p.logits + r * p.ldl;
         const int skip = (int)((reinterpret_cast<uintptr_t>(y) & 15) >> 2);
         const bool ended = p.done[r] != 0;
-        const int t1 = min(p.vocab, (c + 1) * kChunk - skip);
-        for (int t = max(0, c * kChunk - skip) + tid; t < t1; t += kThreads) {
+        const int t1 = min(p.vocab, (c + 1) * p.chunk - skip);
+        for (int t = max(0, c * p.chunk - skip) + tid; t < t1; t += kThreads) {
           const float s = ended ? (t == p.eos ? p.scores[r] : -INFINITY)
                           : p.scores[r] > -INFINITY ? row_score(p.scores[r], logit(y[t]), sh.lse[w])
                                                     : -INFINITY;
@@ -481,10 +487,12 @@ int mtrtq_beam_select(const float* logits, int64_t ldl, const float* scores, con
     return report_error(MTRTQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned, logits 4-byte");
   const BeamLayout l = beam_layout(requests, beams, vocab);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const BeamArgs p = {logits, ldl, scores, done, eos, (int)beams, (int)vocab, l.chunks, out_scores, parent, token,
+  const BeamArgs p = {logits, ldl, scores, done, eos, (int)beams, (int)vocab, l.chunk, l.chunks, out_scores, parent, token,
                       out_done, reinterpret_cast<unsigned*>(ws), reinterpret_cast<float2*>(ws + l.off_stats),
                       reinterpret_cast<unsigned long long*>(ws + l.off_keys)};
-  beam_kernel<<<dim3(l.chunks, (unsigned)beams, (unsigned)requests), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  const dim3 grid(l.chunks, (unsigned)beams, (unsigned)requests);
+  if (l.chunk == kChunk) beam_kernel<16><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  else beam_kernel<32><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MTRTQ_OK : report_cuda_error(e, "beam selection launch");
 }
