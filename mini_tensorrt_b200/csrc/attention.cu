@@ -307,8 +307,9 @@ int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cuda
   return cuda_status(launch_attention_tc(p, qm, km, vm, l.grid, before, st), "attention launch");
 }
 
-// The f32 path: tickets | partials of cut tiles. Tiles of 16 rows where requests have few
-// rows each, of 64 and 128 for longer ones (a tile holds whole groups of heads).
+// The f32 path: tickets | partials of cut tiles. Tiles of up to 8 rows where requests have
+// few rows each (a kernel of its own, bound by memory), else of 16, 64 or 128. A tile holds
+// whole groups of heads.
 struct F32Layout {
   int grid, tile_rows;
   size_t off_ml, off_part, total;
@@ -318,8 +319,11 @@ F32Layout f32_layout(const Args& a, int sm_count) {
   F32Layout l;
   const int group = a.heads / a.kv_heads, dp = a.head_dim <= 64 ? 64 : 128;
   const int64_t each = a.rows * group / a.batch;  // rows of a request's tiles, on average
-  l.tile_rows = each <= 16 && group <= 16 ? 16 : each <= 256 && group <= 64 ? 64 : 128;
-  const int ctas = dp == 64 || l.tile_rows == 16 ? 2 : 1;
+  if (each <= 8 && group <= 8)
+    l.tile_rows = each <= 1 && group == 1 ? 1 : each <= 2 && group <= 2 ? 2 : each <= 4 && group <= 4 ? 4 : 8;
+  else
+    l.tile_rows = each <= 16 && group <= 16 ? 16 : each <= 256 && group <= 64 ? 64 : 128;
+  const int ctas = l.tile_rows <= 2 || l.tile_rows == 16 || (dp == 64 && l.tile_rows > 8) ? 2 : 1;
   l.grid = sm_count * ctas < 1024 ? sm_count * ctas : 1024;
   l.off_ml = 4096;
   l.off_part = l.off_ml + round256((size_t)l.grid * 2 * l.tile_rows * sizeof(float2));
@@ -339,8 +343,8 @@ int launch_f32(const Args& a, bool paged, void* workspace, cudaStream_t st) {
   fill_list(a, paged, p);
   p.slot_tokens = 0;
   p.tile_tokens = l.tile_rows / p.group;
-  p.min_steps = 3;
-  p.pair_cost = 1;  // (every f32 tile is of that kind)
+  p.min_steps = 2;
+  p.pair_cost = l.tile_rows == 128;  // (every f32 tile is of that kind)
   p.scale = a.scale;
   p.q = static_cast<const float*>(a.q);
   p.k = static_cast<const float*>(paged ? a.k_pages : a.k);

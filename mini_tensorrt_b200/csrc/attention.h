@@ -38,7 +38,8 @@ struct TcAttention : AttentionList {
   unsigned* status;
 };
 
-// fp32 throughout, on the CUDA cores (attention_f32.cu): tiles of 16, 64 or 128 rows.
+// fp32 throughout, on the CUDA cores (attention_f32.cu): tiles of 1, 2, 4, 8, 16, 64 or
+// 128 rows.
 struct F32Attention : AttentionList {
   float scale;
   const float *q, *k, *v;  // paged: k and v are the pages, k_row and v_row the page stride

@@ -46,12 +46,46 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ bool broken(float x) { return !(fabsf(x) < INFINITY); }
 
+// The CTA that finishes a cut tile last joins its parts, in order: all threads.
+template <int HD, int BM>
+__device__ __forceinline__ void join_parts(const F32Attention& p, const Segment& s) {
+  const int c_first = s.c_first, c_last = s.c_last, rows = s.tokens * p.group, vecs = p.head_dim / 4;
+#pragma unroll 1
+  for (int e = threadIdx.x; e < rows * vecs; e += kThreads) {
+    const int row = e / vecs, d = e % vecs * 4, token = row / p.group, head = row - token * p.group;
+    float top = -INFINITY;
+    for (int64_t c = c_first; c <= c_last; ++c)
+      top = fmaxf(top, __ldcg(p.part_ml + (c * 2 + (c == c_first ? 1 : 0)) * BM + row).x);
+    float sum = 0.0f;
+    float4 x = make_float4(0, 0, 0, 0);
+    for (int64_t c = c_first; c <= c_last; ++c) {
+      const int64_t at = (c * 2 + (c == c_first ? 1 : 0)) * BM + row;
+      const float2 ml = __ldcg(p.part_ml + at);
+      if (ml.x == -INFINITY) continue;
+      const float w = top == INFINITY ? 1.0f : ex2(ml.x - top);
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(p.partials + at * HD + d));
+      sum += ml.y * w;
+      x.x += y.x * w;
+      x.y += y.y * w;
+      x.z += y.z * w;
+      x.w += y.w * w;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *reinterpret_cast<float4*>(p.out + (s.row0 + (int64_t)token) * p.out_row +
+                               (int64_t)(s.h * p.group + head) * p.out_head + d) =
+        make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  }
+  if (threadIdx.x == 0) p.counters[c_first] = 0u;
+}
+
 template <int HD, int RM, bool PAGED>
 __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
     attention_f32_kernel(const __grid_constant__ F32Attention p) {
   using C = Cfg<HD, RM>;
   constexpr int RP = RM == 1 ? 1 : RM / 2;  // row pairs of a thread
   constexpr int NC = HD / 64;               // groups of four output columns of a thread
+  constexpr int NL = HD / 16;               // 16-byte loads of K, and of V, of a thread
+  constexpr bool AHEAD = RM < 8;
   extern __shared__ float4 raw4[];
   float* sm = reinterpret_cast<float*>(raw4);
   float *qs = sm + C::OFF_Q, *ks = sm + C::OFF_K, *vs = sm + C::OFF_V, *ps = sm + C::OFF_P;
@@ -74,6 +108,44 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
     if (!more) break;
     const int64_t r0 = s.r0;  // where the request's rows start
     const int tokens = s.tokens, keys = s.keys;
+    // K and V of a block, on their way together (and while the last block is worked on, where
+    // registers allow it): a lane per key of K, which is transposed, V as it is. Tokens past
+    // the keys, and pages out of range, read as zeros.
+    float4 kr[NL], vr[NL];
+    auto fetch = [&](int key0) {
+      const int key = key0 + (warp & 1) * 32 + lane;
+      const float* src = nullptr;
+      if (key < keys) {
+        if (PAGED) {
+          const int64_t page = p.table[s.b * p.table_ld + key / p.page_size];
+          if (page >= 0 && page < p.num_pages)
+            src = p.k + page * p.k_row + ((int64_t)s.h * p.page_size + key % p.page_size) * p.head_dim;
+        } else {
+          src = p.k + (r0 + key) * p.k_row + s.h * p.k_head;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < NL; ++c) {
+        const int d = (warp >> 1) * (HD / 4) + c * 4;
+        kr[c] = src && d < p.head_dim ? *reinterpret_cast<const float4*>(src + d) : make_float4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < NL; ++c) {
+        const int e = c * kThreads + tid, at = key0 + e / (HD / 4), d = e % (HD / 4) * 4;
+        vr[c] = make_float4(0, 0, 0, 0);
+        if (at < keys && d < p.head_dim) {
+          if (PAGED) {
+            const int64_t page = p.table[s.b * p.table_ld + at / p.page_size];
+            if (page >= 0 && page < p.num_pages)
+              vr[c] = *reinterpret_cast<const float4*>(
+                  p.v + page * p.v_row + ((int64_t)s.h * p.page_size + at % p.page_size) * p.head_dim + d);
+          } else {
+            vr[c] = *reinterpret_cast<const float4*>(p.v + (r0 + at) * p.v_row + s.h * p.v_head + d);
+          }
+        }
+      }
+    };
+    if (AHEAD) fetch(s.k0 * kKeys);
     // Q, transposed; rows past the tile's tokens and dimensions past the head's are zero.
     for (int e = tid; e < C::BM * (HD / 4); e += kThreads) {
       const int row = e % C::BM, d = e / C::BM * 4;
@@ -103,51 +175,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
     for (int j = s.k0; j < k1; ++j) {
       const int key0 = j * kKeys;
       __syncthreads();
-      // K transposed: a lane per key; V as it is. Tokens past the keys, and pages out of
-      // range, read as zeros.
       bool odd = false;
-      {
-        const int key = key0 + (warp & 1) * 32 + lane;
-        const float* src = nullptr;
-        if (key < keys) {
-          if (PAGED) {
-            const int64_t page = p.table[s.b * p.table_ld + key / p.page_size];
-            if (page >= 0 && page < p.num_pages)
-              src = p.k + page * p.k_row + ((int64_t)s.h * p.page_size + key % p.page_size) * p.head_dim;
-          } else {
-            src = p.k + (r0 + key) * p.k_row + s.h * p.k_head;
-          }
-        }
-        float* dst = ks + (warp & 1) * 32 + lane;
+      if (!AHEAD) fetch(key0);
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) {
-          const int d = (warp >> 1) * (HD / 4) + c * 4;
-          const float4 x = src && d < p.head_dim ? *reinterpret_cast<const float4*>(src + d) : make_float4(0, 0, 0, 0);
-          dst[d * C::KS] = x.x;
-          dst[(d + 1) * C::KS] = x.y;
-          dst[(d + 2) * C::KS] = x.z;
-          dst[(d + 3) * C::KS] = x.w;
-        }
-#pragma unroll
-        for (int c = 0; c < kKeys * HD / 4 / kThreads; ++c) {
-          const int e = c * kThreads + tid, r = e / (HD / 4), d = e % (HD / 4) * 4, at = key0 + r;
-          float4 x = make_float4(0, 0, 0, 0);
-          if (at < keys && d < p.head_dim) {
-            if (PAGED) {
-              const int64_t page = p.table[s.b * p.table_ld + at / p.page_size];
-              if (page >= 0 && page < p.num_pages)
-                x = *reinterpret_cast<const float4*>(
-                    p.v + page * p.v_row + ((int64_t)s.h * p.page_size + at % p.page_size) * p.head_dim + d);
-            } else {
-              x = *reinterpret_cast<const float4*>(p.v + (r0 + at) * p.v_row + s.h * p.v_head + d);
-            }
-          }
-          odd |= broken(x.x) | broken(x.y) | broken(x.z) | broken(x.w);
-          *reinterpret_cast<float4*>(vs + r * HD + d) = x;
-        }
+      for (int c = 0; c < NL; ++c) {
+        float* dst = ks + ((warp >> 1) * (HD / 4) + c * 4) * C::KS + (warp & 1) * 32 + lane;
+        dst[0] = kr[c].x;
+        dst[C::KS] = kr[c].y;
+        dst[2 * C::KS] = kr[c].z;
+        dst[3 * C::KS] = kr[c].w;
+        *reinterpret_cast<float4*>(vs + (c * kThreads + tid) * 4) = vr[c];
+        odd |= broken(vr[c].x) | broken(vr[c].y) | broken(vr[c].z) | broken(vr[c].w);
       }
       const bool partly = key0 + kKeys > all_see;
       const bool careful = __syncthreads_or(odd) && partly;
+      if (AHEAD && j + 1 < k1) fetch(key0 + kKeys);
 
       // S: rows in pairs, four keys
       float2 a[RP][4];
@@ -290,54 +332,225 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
       }
     }
     if (!whole) {
-      // the CTA that finishes a cut tile last joins its parts in order
-      const int64_t c_first = s.c_first, c_last = s.c_last;
       __syncthreads();
-      if (tid == 0) ticket = ticket_acq_rel(p.counters + c_first);
+      if (tid == 0) ticket = ticket_acq_rel(p.counters + s.c_first);
       __syncthreads();
-      if (ticket == (unsigned)(c_last - c_first)) {
-        const int rows = tokens * p.group, vecs = p.head_dim / 4;
-        for (int e = tid; e < rows * vecs; e += kThreads) {
-          const int row = e / vecs, d = e % vecs * 4, token = row / p.group, head = row - token * p.group;
-          float top = -INFINITY;
-          for (int64_t c = c_first; c <= c_last; ++c)
-            top = fmaxf(top, __ldcg(p.part_ml + (c * 2 + (c == c_first ? 1 : 0)) * C::BM + row).x);
-          float sum = 0.0f;
-          float4 x = make_float4(0, 0, 0, 0);
-          for (int64_t c = c_first; c <= c_last; ++c) {
-            const int64_t at = (c * 2 + (c == c_first ? 1 : 0)) * C::BM + row;
-            const float2 ml = __ldcg(p.part_ml + at);
-            if (ml.x == -INFINITY) continue;
-            const float w = top == INFINITY ? 1.0f : ex2(ml.x - top);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(p.partials + at * HD + d));
-            sum += ml.y * w;
-            x.x += y.x * w;
-            x.y += y.y * w;
-            x.z += y.z * w;
-            x.w += y.w * w;
-          }
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          *reinterpret_cast<float4*>(p.out + (s.row0 + (int64_t)token) * p.out_row +
-                                     (int64_t)(s.h * p.group + head) * p.out_head + d) =
-              make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-        }
-        if (tid == 0) p.counters[c_first] = 0u;
-      }
+      if (ticket == (unsigned)(s.c_last - s.c_first)) join_parts<HD, C::BM>(p, s);
     }
   }
 }
 
-template <int HD, int RM, bool PAGED>
-cudaError_t launch_one(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
-  auto kernel = attention_f32_kernel<HD, RM, PAGED>;
-  using C = Cfg<HD, RM>;
-  constexpr int most = C::BYTES + MTRTQ_MAX_BATCH * (int)sizeof(Request);
-  static_assert(most + 3 * 1024 <= 227 * 1024 && C::BYTES >= (MTRTQ_MAX_BATCH + 1) * 8, "shared memory per CTA");
-  if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kernel), most)) return e;
+// ---- few rows: one token, or a few, over a cache ------------------------------------
+//
+// A tile of up to R rows (one token's group of heads, as a rule) needs 2 R products for each
+// element of K and V, so the time is that of reading them. Eight lanes (16 for 128
+// dimensions) share a key, eight dimensions each, with the rows of q in registers: four
+// keys' K and V are loaded together and used straight from the registers, without shared
+// memory or barriers. Every such group of lanes keeps its own maximum, sum and output; they
+// are joined when the CTA's run of the tile ends.
+template <int HD, int R>
+struct Few {
+  static constexpr int LANES = HD / 8;             // of a key
+  static constexpr int KEYS = 4;                   // of a lane, loaded together
+  static constexpr int BLOCK = kThreads / LANES * KEYS;
+  static constexpr int CTAS = R <= 2 ? 2 : 1;
+};
+
+template <int HD, int R, bool PAGED>
+__global__ void __launch_bounds__(kThreads, Few<HD, R>::CTAS)
+    attention_f32_few_kernel(const __grid_constant__ F32Attention p) {
+  using F = Few<HD, R>;
+  constexpr int LANES = F::LANES, KEYS = F::KEYS;
+  extern __shared__ float4 raw4[];
+  float* joined = reinterpret_cast<float*>(raw4);  // [8 warps][R][HD], then their (m, l)
+  float2* joined_ml = reinterpret_cast<float2*>(joined + 8 * R * HD);
+  // the list's prefix lies where the rows are joined
+  const StepList list = {reinterpret_cast<Request*>(joined + (8 * R * (HD + 2) > (MTRTQ_MAX_BATCH + 2) / 2 * 4 ? 8 * R * (HD + 2) : (MTRTQ_MAX_BATCH + 2) / 2 * 4)),
+                         reinterpret_cast<int64_t*>(joined)};
+  __shared__ Walk shared_walk;
+  __shared__ Segment s;
+  __shared__ int more;
+  __shared__ unsigned ticket;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int d0 = lane % LANES * 8;             // this lane's dimensions
+  const int mine = tid / LANES;                // and its first key of a block
+  const bool in0 = d0 < p.head_dim;            // (head_dim is a multiple of 8)
+
+  Walk walk;
+  make_list<F::BLOCK, kThreads>(p, list, walk, &shared_walk);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const float c2 = p.scale * 1.4426950408889634f;  // scale log2 e
+
+  while (true) {
+    __syncthreads();
+    if (tid == 0) more = next_segment<F::BLOCK>(p, list, walk, s);
+    __syncthreads();
+    if (!more) break;
+    const int64_t r0 = s.r0;
+    const int tokens = s.tokens, keys = s.keys, rows = tokens * p.group;
+    float q[R][8], o[R][8], m[R], l[R];
+    int sees[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int token = r / p.group, head = r - token * p.group;
+      float4 x = make_float4(0, 0, 0, 0), y = x;
+      if (r < rows && in0) {
+        const float* src = p.q + (s.row0 + (int64_t)token) * p.q_row + (int64_t)(s.h * p.group + head) * p.q_head + d0;
+        x = *reinterpret_cast<const float4*>(src);
+        y = *reinterpret_cast<const float4*>(src + 4);
+      }
+      q[r][0] = x.x, q[r][1] = x.y, q[r][2] = x.z, q[r][3] = x.w;
+      q[r][4] = y.x, q[r][5] = y.y, q[r][6] = y.z, q[r][7] = y.w;
+      sees[r] = r < rows ? max(0, min(s.see0 + token, keys)) : 0;
+      m[r] = -INFINITY;
+      l[r] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) o[r][d] = 0.0f;
+    }
+    const int k1 = s.k0 + s.n;
+    for (int j = s.k0; j < k1; ++j) {
+      float4 k[KEYS][2], v[KEYS][2];
+#pragma unroll
+      for (int c = 0; c < KEYS; ++c) {
+        const int key = j * F::BLOCK + c * (kThreads / LANES) + mine;
+        k[c][0] = k[c][1] = v[c][0] = v[c][1] = make_float4(0, 0, 0, 0);
+        if (key < keys && in0) {
+          const float *ks, *vs;
+          bool there = true;
+          if (PAGED) {
+            const int64_t page = p.table[s.b * p.table_ld + key / p.page_size];
+            there = page >= 0 && page < p.num_pages;  // else the token reads as zeros
+            const int64_t at = ((int64_t)s.h * p.page_size + key % p.page_size) * p.head_dim + d0;
+            ks = p.k + page * p.k_row + at;
+            vs = p.v + page * p.v_row + at;
+          } else {
+            ks = p.k + (r0 + key) * p.k_row + s.h * p.k_head + d0;
+            vs = p.v + (r0 + key) * p.v_row + s.h * p.v_head + d0;
+          }
+          if (there) {
+            k[c][0] = *reinterpret_cast<const float4*>(ks);
+            k[c][1] = *reinterpret_cast<const float4*>(ks + 4);
+            v[c][0] = *reinterpret_cast<const float4*>(vs);
+            v[c][1] = *reinterpret_cast<const float4*>(vs + 4);
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float e[KEYS], top = m[r];
+#pragma unroll
+        for (int c = 0; c < KEYS; ++c) {
+          float x = q[r][0] * k[c][0].x;
+          x = fmaf(q[r][1], k[c][0].y, x);
+          x = fmaf(q[r][2], k[c][0].z, x);
+          x = fmaf(q[r][3], k[c][0].w, x);
+          x = fmaf(q[r][4], k[c][1].x, x);
+          x = fmaf(q[r][5], k[c][1].y, x);
+          x = fmaf(q[r][6], k[c][1].z, x);
+          x = fmaf(q[r][7], k[c][1].w, x);
+#pragma unroll
+          for (int w = LANES / 2; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+          e[c] = j * F::BLOCK + c * (kThreads / LANES) + mine < sees[r] ? x : -INFINITY;
+          top = fmaxf(top, e[c] * c2);
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+        const float keep = m[r] == -INFINITY ? 1.0f : ex2(m[r] - base);
+        m[r] = top;
+        l[r] *= keep;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[r][d] *= keep;
+#pragma unroll
+        for (int c = 0; c < KEYS; ++c) {
+          // a key that the row does not see adds nothing, whatever its v
+          if (j * F::BLOCK + c * (kThreads / LANES) + mine >= sees[r]) continue;
+          const float w = ex2(fmaf(e[c], c2, -base));
+          l[r] += w;
+          o[r][0] = fmaf(w, v[c][0].x, o[r][0]);
+          o[r][1] = fmaf(w, v[c][0].y, o[r][1]);
+          o[r][2] = fmaf(w, v[c][0].z, o[r][2]);
+          o[r][3] = fmaf(w, v[c][0].w, o[r][3]);
+          o[r][4] = fmaf(w, v[c][1].x, o[r][4]);
+          o[r][5] = fmaf(w, v[c][1].y, o[r][5]);
+          o[r][6] = fmaf(w, v[c][1].z, o[r][6]);
+          o[r][7] = fmaf(w, v[c][1].w, o[r][7]);
+        }
+      }
+    }
+    // The groups of a warp, then the warps.
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (m[r] == -INFINITY && l[r] != l[r]) m[r] = 0.0f;  // every score it saw was NaN
+#pragma unroll
+      for (int w = LANES; w < 32; w <<= 1) {
+        const float m1 = __shfl_xor_sync(0xffffffffu, m[r], w), l1 = __shfl_xor_sync(0xffffffffu, l[r], w);
+        const float top = fmaxf(m[r], m1);
+        // both lanes of a pair form the same sum
+        const float a = m[r] == -INFINITY ? 0.0f : top == INFINITY ? 1.0f : ex2(m[r] - top);
+        const float b = m1 == -INFINITY ? 0.0f : top == INFINITY ? 1.0f : ex2(m1 - top);
+        const bool low = (lane & w) == 0;
+        l[r] = low ? l[r] * a + l1 * b : l1 * b + l[r] * a;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const float x = o[r][d] * a, y = __shfl_xor_sync(0xffffffffu, o[r][d], w) * b;
+          o[r][d] = low ? x + y : y + x;
+        }
+        m[r] = top;
+      }
+      if (lane < LANES) {
+        float* dst = joined + (warp * R + r) * HD + d0;
+        *reinterpret_cast<float4*>(dst) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(o[r][4], o[r][5], o[r][6], o[r][7]);
+        if (lane == 0) joined_ml[warp * R + r] = make_float2(m[r], l[r]);
+      }
+    }
+    __syncthreads();
+    const bool whole = s.whole;
+    const int64_t part = (int64_t)blockIdx.x * 2 + s.part;
+    for (int e = tid; e < rows * (HD / 4); e += kThreads) {
+      const int row = e / (HD / 4), d = e % (HD / 4) * 4, token = row / p.group, head = row - token * p.group;
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) top = fmaxf(top, joined_ml[w * R + row].x);
+      float4 x = make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const float2 ml = joined_ml[w * R + row];
+        const float a = ml.x == -INFINITY ? 0.0f : top == INFINITY ? 1.0f : ex2(ml.x - top);
+        const float4 y = *reinterpret_cast<const float4*>(joined + (w * R + row) * HD + d);
+        sum = fmaf(ml.y, a, sum);
+        x.x = fmaf(y.x, a, x.x);
+        x.y = fmaf(y.y, a, x.y);
+        x.z = fmaf(y.z, a, x.z);
+        x.w = fmaf(y.w, a, x.w);
+      }
+      if (whole) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (d < p.head_dim)
+          *reinterpret_cast<float4*>(p.out + (s.row0 + (int64_t)token) * p.out_row +
+                                     (int64_t)(s.h * p.group + head) * p.out_head + d) =
+              make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+      } else {
+        __stcg(reinterpret_cast<float4*>(p.partials + (part * R + row) * HD + d), x);
+        if (d == 0) __stcg(p.part_ml + part * R + row, make_float2(top, sum));
+      }
+    }
+    if (!whole) {
+      __syncthreads();
+      if (tid == 0) ticket = ticket_acq_rel(p.counters + s.c_first);
+      __syncthreads();
+      if (ticket == (unsigned)(s.c_last - s.c_first)) join_parts<HD, R>(p, s);
+    }
+  }
+}
+
+cudaError_t launch(void (*kernel)(F32Attention), const F32Attention& p, int bytes, int grid, bool pdl, cudaStream_t st) {
+  if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kernel),
+                                        bytes + MTRTQ_MAX_BATCH * (int)sizeof(Request)))
+    return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<HD, RM>::BYTES + p.batch * (int)sizeof(Request);
+  cfg.dynamicSmemBytes = bytes + p.batch * sizeof(Request);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -347,11 +560,31 @@ cudaError_t launch_one(const F32Attention& p, int grid, bool pdl, cudaStream_t s
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+template <int HD, int RM, bool PAGED>
+cudaError_t launch_tile(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
+  using C = Cfg<HD, RM>;
+  static_assert(C::BYTES + MTRTQ_MAX_BATCH * (int)sizeof(Request) + 3 * 1024 <= 227 * 1024 &&
+                    C::BYTES >= (MTRTQ_MAX_BATCH + 1) * 8, "shared memory per CTA");
+  return launch(attention_f32_kernel<HD, RM, PAGED>, p, C::BYTES, grid, pdl, st);
+}
+
+template <int HD, int R, bool PAGED>
+cudaError_t launch_few(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
+  const int bytes = 8 * R * (HD * 4 + 8), prefix = (MTRTQ_MAX_BATCH + 2) / 2 * 16;
+  return launch(attention_f32_few_kernel<HD, R, PAGED>, p, bytes > prefix ? bytes : prefix, grid, pdl, st);
+}
+
 template <int HD, bool PAGED>
 cudaError_t launch_rows(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
-  if (p.tile_rows == 16) return launch_one<HD, 1, PAGED>(p, grid, pdl, st);
-  if (p.tile_rows == 64) return launch_one<HD, 4, PAGED>(p, grid, pdl, st);
-  return launch_one<HD, 8, PAGED>(p, grid, pdl, st);
+  switch (p.tile_rows) {
+    case 1: return launch_few<HD, 1, PAGED>(p, grid, pdl, st);
+    case 2: return launch_few<HD, 2, PAGED>(p, grid, pdl, st);
+    case 4: return launch_few<HD, 4, PAGED>(p, grid, pdl, st);
+    case 8: return launch_few<HD, 8, PAGED>(p, grid, pdl, st);
+    case 16: return launch_tile<HD, 1, PAGED>(p, grid, pdl, st);
+    case 64: return launch_tile<HD, 4, PAGED>(p, grid, pdl, st);
+    default: return launch_tile<HD, 8, PAGED>(p, grid, pdl, st);
+  }
 }
 
 }  // namespace
