@@ -9,7 +9,7 @@ every call can be captured in a CUDA graph (with `out` and `workspace` given).
 from __future__ import annotations
 
 import ctypes
-import math
+import struct
 
 import torch
 
@@ -19,6 +19,11 @@ from .matmulq import Workspace
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 _workspaces: dict = {}
+_NO_PAGES = (0, 0, 0, 0, 0, 0, 0, 0, 0)
+# mtrtq_attention_args in the order of _lib.AttentionArgs, packed in one call (setting its
+# fields one by one takes three times as long)
+_pack = struct.Struct("@4P8q2q5if P2P2qiP2qP").pack
+assert struct.calcsize("@4P8q2q5if P2P2qiP2qP") == ctypes.sizeof(_lib.AttentionArgs)
 
 
 def _stream_ptr(stream, index: int) -> int:
@@ -53,7 +58,7 @@ def _workspace(workspace, device, stream_ptr: int, nbytes: int):
 
 def _rows(name: str, x: torch.Tensor, shape, dtype, device):
     """Checks rows of heads; returns their strides."""
-    if x.shape != shape or x.dtype != dtype or x.device != device:
+    if x.shape != shape or x.dtype is not dtype or x.device != device:
         raise ValueError(f"{name} must be {dtype} {list(shape)} on {device}, got {x.dtype} {list(x.shape)} on {x.device}")
     s = x.stride()
     if s[2] != 1 and shape[2] > 1:
@@ -70,44 +75,42 @@ def _ints(name: str, x: torch.Tensor, shape, device):
     return s
 
 
-def _attend(where, q, k, v, out, out_dtype, kv_heads, cu_rows, scale, workspace, stream, pages=None):
+def _attend(where, q, k, v, out, out_dtype, kv_heads, cu_rows, scale, workspace, stream, pages=_NO_PAGES):
     dtype, device = q.dtype, q.device
     if q.dim() != 3 or dtype not in _DTYPES or device.type != "cuda":
         raise ValueError("q must be a float32 or bfloat16 CUDA tensor [rows, heads, head_dim]")
-    shape = q.shape
-    T, H, D = shape
-    a = _lib.AttentionArgs()
-    s = _rows("q", q, shape, dtype, device)
-    a.q, a.q_row, a.q_head = q.data_ptr(), s[0], s[1]
-    if k is not None:
-        s = _rows("k", k, (T, kv_heads, D), dtype, device)
-        a.k, a.k_row, a.k_head = k.data_ptr(), s[0], s[1]
-        s = _rows("v", v, (T, kv_heads, D), dtype, device)
-        a.v, a.v_row, a.v_head = v.data_ptr(), s[0], s[1]
     if out_dtype not in _DTYPES:
         raise ValueError("the result is float32 or bfloat16")
+    shape, index = q.shape, device.index
+    T, H, D = shape
+    if D == 0:
+        raise ValueError("head_dim must be positive")
+    qs = _rows("q", q, shape, dtype, device)
+    if k is not None:
+        kv = (T, kv_heads, D)
+        ks, vs = _rows("k", k, kv, dtype, device), _rows("v", v, kv, dtype, device)
+        kp, vp = k.data_ptr(), v.data_ptr()
+    else:
+        ks, vs, kp, vp = (0, 0), (0, 0), 0, 0
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=device)
+        out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
+        os = (H * D, D)
         if isinstance(stream, torch.cuda.Stream):
             out.record_stream(stream)
-    s = _rows("out", out, shape, out_dtype, device)
-    a.out, a.out_row, a.out_head = out.data_ptr(), s[0], s[1]
+    else:
+        os = _rows("out", out, shape, out_dtype, device)
     if cu_rows.dim() != 1:
         raise ValueError("the row bounds must be int32 [requests + 1]")
     batch = cu_rows.shape[0] - 1
     _ints("the row bounds", cu_rows, (batch + 1,), device)
-    a.cu_rows, a.rows, a.batch, a.heads, a.kv_heads, a.head_dim = cu_rows.data_ptr(), T, batch, H, kv_heads, D
-    a.x_dtype, a.dtype = _DTYPES[dtype], _DTYPES[out_dtype]
-    a.scale = 1.0 / math.sqrt(D) if scale is None else scale
-    if pages is not None:
-        (a.k_pages, a.v_pages, a.page_stride, a.num_pages, a.page_size, a.table, a.table_ld, a.table_width,
-         a.kv_len) = pages
-    sp = _stream_ptr(stream, device.index)
-    ref = ctypes.byref(a)
-    need = lib().mtrtq_attention_workspace_bytes(ref)
+    a = _pack(q.data_ptr(), kp, vp, out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], T, batch, H,
+              kv_heads, D, _DTYPES[dtype], _DTYPES[out_dtype], D ** -0.5 if scale is None else scale,
+              cu_rows.data_ptr(), *pages)
+    sp = _stream_ptr(stream, index)
+    need = lib().mtrtq_attention_workspace_bytes(a)
     # arguments that the query refuses are refused by the call, with the reason
     ws, nbytes = _workspace(workspace, device, sp, need) if need > 0 else (None, 0)
-    _call(where, device.index, ref, ws, nbytes, sp)
+    _call(where, index, a, ws, nbytes, sp)
     return out
 
 
@@ -181,8 +184,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor, 
             or logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("logits must be float32 [requests * beams, vocab] with unit stride along vocab")
     if out is None:
-        out = (torch.empty_like(scores), torch.empty((B, W), dtype=torch.int32, device=dev),
-               torch.empty((B, W), dtype=torch.int32, device=dev), torch.empty_like(done))
+        out = (torch.empty_like(scores), torch.empty_like(scores, dtype=torch.int32),
+               torch.empty_like(scores, dtype=torch.int32), torch.empty_like(done))
         if isinstance(stream, torch.cuda.Stream):
             for x in out:
                 x.record_stream(stream)
