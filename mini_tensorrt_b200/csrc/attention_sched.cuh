@@ -9,6 +9,7 @@
 
 #include "../../include/mtrtq.h"
 #include "attention.h"
+#include "q8_common.cuh"
 
 namespace mtrtq {
 
@@ -239,6 +240,7 @@ __device__ void make_list(const AttentionList& p, const StepList list, Walk& wal
     }
     if (lane == 0) *shared = w;
   }
+  fence_proxy_async_smem();  // bulk copies may land where the prefix was
   __syncthreads();
   walk = *shared;
   __syncthreads();

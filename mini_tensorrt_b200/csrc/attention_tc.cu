@@ -22,10 +22,10 @@
 //
 // One CTA = 20 warps: 0..7 and 8..15 the slots' softmax (two threads per row, of 64 keys
 // each, also the epilogue), 16 TMA loads, 17 and 18 issue the slots' products, 19 looks over
-// the V blocks that not every row
-// sees whole: rows past the request's keys are zeroed (a page's unused rows, the next
-// request's rows: 0 * NaN would reach O), and infinities and NaN in rows that only later
-// tokens see are taken out and listed; the epilogue adds them to the rows that see them.
+// the V blocks that not every row sees whole: rows past the request's keys are zeroed (a
+// page's unused rows, the next request's rows: 0 * NaN would reach O), and infinities and NaN
+// in rows that only later tokens see are taken out and listed; the epilogue adds them to the
+// rows that see them.
 #include <math.h>
 
 #include "../../include/mtrtq.h"
@@ -631,6 +631,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int k0 = s.k0, n = s.n;
         if (n == 0) break;
         const bool pair = s.pair;
+        // Page numbers of 64 columns, two in each lane, read well before they are used: a
+        // read of the table on each copy's way cost more than the copy.
+        const int columns = PAGED ? (s.keys + p.page_size - 1) / p.page_size : 0;
+        auto column = [&](int col) { return col < columns ? p.table[s.b * p.table_ld + col] : 0; };
+        int window = PAGED ? k0 * pages : 0, ahead[2];
+        if (PAGED) {
+          ahead[0] = column(window + lane);
+          ahead[1] = column(window + 32 + lane);
+        }
 #pragma unroll 1
         for (int t = 0; ok && t < (pair ? 2 : 1); ++t) {
           const int buf = pair ? t : s.buf;
@@ -654,7 +663,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           int page = 0;
           if (PAGED) {
             load = load && key0 + pg * p.page_size < s.keys;
-            if (load) page = p.table[s.b * p.table_ld + (k0 + c) * pages + pg];
+            const int col = (k0 + c) * pages;
+            if (is_v && col >= window + 32) {  // every earlier column is done with
+              window += 32;
+              ahead[0] = ahead[1];
+              ahead[1] = column(window + 32 + lane);
+            }
+            const int want = (col + pg - window) & 63;
+            const int lo = __shfl_sync(0xffffffffu, ahead[0], want & 31), hi = __shfl_sync(0xffffffffu, ahead[1], want & 31);
+            page = want < 32 ? lo : hi;
           }
           ok = warp_wait(&empty[st], ((seq / C::STAGES) & 1) ^ 1);
           if (!ok) break;
