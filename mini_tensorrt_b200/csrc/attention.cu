@@ -289,7 +289,7 @@ int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cuda
   p.slot_tokens = l.slot_tokens;
   p.tile_tokens = 2 * l.slot_tokens;
   p.min_steps = 4;
-  p.tile_cost = 2;
+  p.tile_cost = 3;
   p.pair_cost = 3;
   p.scale = a.scale;
   p.out32 = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.out_row % 16 == 0 && a.out_head % 16 == 0;

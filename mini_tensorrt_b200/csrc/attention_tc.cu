@@ -403,7 +403,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int keys = live ? max(0, min(s.see0 + tok, s.keys)) : 0;  // that this row sees
       const bool warp_live = __any_sync(0xffffffffu, live);
       const int cnt = s.cnt[t], stride = pair ? kBlock : 2 * kBlock;
-      int left = keys - (s.k0 + (pair ? 0 : t)) * kBlock - half * 64;  // of these 64 columns
+      // Of these 64 columns it sees so many; rows that are no tokens' are left unmasked, so
+      // that they do not put their warp on the masked path block after block.
+      int left = (live ? keys : 0x40000000) - (s.k0 + (pair ? 0 : t)) * kBlock - half * 64;
       float m = -INFINITY, l = 0.0f;
 #pragma unroll 1
       for (int x = 0; x < cnt; ++x, left -= stride, ++n_s) {
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = swap(ok, top, other);
         if (!ok) break;
         top = fmaxf(top, other) * c2;
-        const bool grow = top > m + 8.0f || (m == -INFINITY && top > m);
+        const bool grow = live && (top > m + 8.0f || (m == -INFINITY && top > m));
         if (__any_sync(0xffffffffu, grow)) {
           const float m1 = grow ? top : m;
           const float keep = m1 == -INFINITY ? 1.0f : ex2(m - m1);
