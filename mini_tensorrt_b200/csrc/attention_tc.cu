@@ -179,10 +179,26 @@ __device__ __forceinline__ bool nth_load(bool pair, int at, int n, int& c) {
   return !(at & 1);
 }
 
-// Bounded waits that fail at once when another role has given up.
+// Tests the phase with the given parity, suspended for as long as the hardware sees fit.
+__device__ __forceinline__ bool try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded waits that fail at once when another role has given up. (Many warps wait at any
+// time: the clock and the flag are looked at every 64 tests only.)
 __device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned* status) {
   const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
     if (clock64() - t0 > kSpinLimitCycles) {
       *abort_flag = 1;
@@ -190,10 +206,9 @@ __device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volati
       return false;
     }
   }
-  return true;
 }
 __device__ __forceinline__ bool wait_one(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned* status) {
-  if (__builtin_expect(mbar_test_wait(bar, parity), 1)) return true;
+  if (__builtin_expect(try_wait(bar, parity), 1)) return true;
   return wait_slow(bar, parity, abort_flag, status);
 }
 __device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned* status) {
