@@ -20,7 +20,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmtrtq.so")
 SOURCES = ["abi.cu", "prepack.cu", "gemv.cu", "gemv_cluster.cu", "gemv_stream.cu", "gemv_tc.cu", "decoder.cu",
            "gemm_tc.cu",
-           "skinny_tc.cu", "shard.cu", "attention.cu", "attention_tc.cu", "attention_f32.cu",
+           "skinny_tc.cu", "shard.cu", "attention.cu", "attention_tc.cu", "attention_f32.cu", "attention_f32_tc.cu",
            "beam.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",

@@ -312,7 +312,8 @@ int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cuda
 // whole groups of heads.
 struct F32Layout {
   int grid, tile_rows;
-  size_t off_ml, off_part, total;
+  bool tc;  // on the tensor cores
+  size_t off_ml, off_part, off_flags, off_planes, total;
 };
 
 F32Layout f32_layout(const Args& a, int sm_count) {
@@ -328,10 +329,17 @@ F32Layout f32_layout(const Args& a, int sm_count) {
   l.off_ml = 4096;
   l.off_part = l.off_ml + round256((size_t)l.grid * 2 * l.tile_rows * sizeof(float2));
   l.total = l.off_part + (size_t)l.grid * 2 * l.tile_rows * dp * sizeof(float);
+  // Prompts from some 100 rows a request on, where the split pays (B200, 12 heads of 64: 4
+  // requests of 64 tokens 23 us against 21 on the CUDA cores, of 130 27 against 38, 8 of 300
+  // 52 against 97).
+  l.tc = !a.k_pages && a.head_dim <= 64 && each >= 96;
+  l.off_flags = round256(l.total);
+  l.off_planes = l.off_flags + round256((size_t)((a.rows + kSplitRows - 1) / kSplitRows) * sizeof(int));
+  if (l.tc) l.total = l.off_planes + (size_t)3 * a.rows * (a.heads + 2 * a.kv_heads) * a.head_dim * 2;
   return l;
 }
 
-int launch_f32(const Args& a, bool paged, void* workspace, cudaStream_t st) {
+int launch_f32(const Args& a, bool paged, void* workspace, unsigned* status, cudaStream_t st) {
   const F32Layout l = f32_layout(a, sm_count());
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const bool before = paged && a.k;
@@ -363,6 +371,32 @@ int launch_f32(const Args& a, bool paged, void* workspace, cudaStream_t st) {
   p.part_ml = reinterpret_cast<float2*>(ws + l.off_ml);
   p.partials = reinterpret_cast<float*>(ws + l.off_part);
   p.tile_rows = l.tile_rows;
+  if (l.tc) {
+    const int all = a.heads + 2 * a.kv_heads;
+    __nv_bfloat16* planes = reinterpret_cast<__nv_bfloat16*>(ws + l.off_planes);
+    int* flags = reinterpret_cast<int*>(ws + l.off_flags);
+    F32TcAttention x = {};
+    static_cast<F32Attention&>(x) = p;
+    x.tile_tokens = 128 / p.group;
+    x.tile_rows = 128;
+    x.min_steps = 2;
+    x.pair_cost = 2;
+    x.flags = flags;
+    x.status = status;
+    CUtensorMap qm, km, vm;
+    const int64_t row = (int64_t)all * a.head_dim;
+    const int64_t q_dims[4] = {a.head_dim, p.group, a.kv_heads, 3 * a.rows};
+    const int64_t q_strides[3] = {a.head_dim, (int64_t)a.head_dim * p.group, row};
+    const int q_box[4] = {64, p.group, 1, x.tile_tokens};
+    if (int rc = make_map(&qm, planes, 4, q_dims, q_strides, q_box)) return rc;
+    const int64_t dims[3] = {a.head_dim, a.kv_heads, 3 * a.rows}, strides[2] = {a.head_dim, row};
+    const int box[3] = {64, 1, 128};
+    if (int rc = make_map(&km, planes + (int64_t)a.heads * a.head_dim, 3, dims, strides, box)) return rc;
+    if (int rc = make_map(&vm, planes + (int64_t)(a.heads + a.kv_heads) * a.head_dim, 3, dims, strides, box)) return rc;
+    if (int rc = cuda_status(launch_split_rows(p, a.heads, planes, flags, st), "attention rows launch")) return rc;
+    const int sms = sm_count();
+    return cuda_status(launch_attention_f32_tc(x, qm, km, vm, sms < 1024 ? sms : 1024, st), "attention launch");
+  }
   return cuda_status(launch_attention_f32(p, l.grid, before, st), "attention launch");
 }
 
@@ -378,7 +412,7 @@ int attention(const Args* a, bool paged, void* workspace, size_t workspace_bytes
   if (reinterpret_cast<uintptr_t>(workspace) % 256)
     return report_error(MTRTQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == MTRTQ_DTYPE_F32) return launch_f32(*a, paged, workspace, st);
+  if (a->dtype == MTRTQ_DTYPE_F32) return launch_f32(*a, paged, workspace, status, st);
   return launch_tc(*a, paged, workspace, status, st);
 }
 

@@ -53,6 +53,17 @@ struct F32Attention : AttentionList {
   int tile_rows;
 };
 
+// The same on the tensor cores (attention_f32_tc.cu): whole prompts, up to 64 dimensions, in
+// tiles of 128 rows. q, k and v lie as three bf16 planes.
+struct F32TcAttention : F32Attention {
+  const int* flags;  // of split_rows: whether a block of rows has infinities or NaN in v
+  unsigned* status;
+};
+constexpr int kSplitRows = 8;  // rows of a block of split_rows
+cudaError_t launch_split_rows(const F32Attention& p, int heads, __nv_bfloat16* planes, int* flags, cudaStream_t st);
+cudaError_t launch_attention_f32_tc(const F32TcAttention& p, const CUtensorMap& q, const CUtensorMap& k,
+                                    const CUtensorMap& v, int grid, cudaStream_t st);
+
 cudaError_t launch_attention_f32(const F32Attention& p, int grid, bool pdl, cudaStream_t st);
 
 cudaError_t launch_attention_tc(const TcAttention& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,

@@ -14,8 +14,7 @@
 #include <math.h>
 
 #include "../../include/mtrtq.h"
-#include "attention_sched.cuh"
-#include "q8_common.cuh"
+#include "attention_mma.cuh"
 
 namespace mtrtq {
 
@@ -39,44 +38,7 @@ struct Cfg {
   static_assert(CTAS * (BYTES + 5 * 1024) <= 228 * 1024 && FLOATS % 4 == 0, "shared memory per CTA");
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ bool broken(float x) { return !(fabsf(x) < INFINITY); }
-
-// The CTA that finishes a cut tile last joins its parts, in order: all threads.
-template <int HD, int BM>
-__device__ __forceinline__ void join_parts(const F32Attention& p, const Segment& s) {
-  const int c_first = s.c_first, c_last = s.c_last, rows = s.tokens * p.group, vecs = p.head_dim / 4;
-#pragma unroll 1
-  for (int e = threadIdx.x; e < rows * vecs; e += kThreads) {
-    const int row = e / vecs, d = e % vecs * 4, token = row / p.group, head = row - token * p.group;
-    float top = -INFINITY;
-    for (int64_t c = c_first; c <= c_last; ++c)
-      top = fmaxf(top, __ldcg(p.part_ml + (c * 2 + (c == c_first ? 1 : 0)) * BM + row).x);
-    float sum = 0.0f;
-    float4 x = make_float4(0, 0, 0, 0);
-    for (int64_t c = c_first; c <= c_last; ++c) {
-      const int64_t at = (c * 2 + (c == c_first ? 1 : 0)) * BM + row;
-      const float2 ml = __ldcg(p.part_ml + at);
-      if (ml.x == -INFINITY) continue;
-      const float w = top == INFINITY ? 1.0f : ex2(ml.x - top);
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(p.partials + at * HD + d));
-      sum += ml.y * w;
-      x.x += y.x * w;
-      x.y += y.y * w;
-      x.z += y.z * w;
-      x.w += y.w * w;
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<float4*>(p.out + (s.row0 + (int64_t)token) * p.out_row +
-                               (int64_t)(s.h * p.group + head) * p.out_head + d) =
-        make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-  }
-  if (threadIdx.x == 0) p.counters[c_first] = 0u;
-}
 
 template <int HD, int RM, bool PAGED>
 __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
@@ -335,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
       __syncthreads();
       if (tid == 0) ticket = ticket_acq_rel(p.counters + s.c_first);
       __syncthreads();
-      if (ticket == (unsigned)(s.c_last - s.c_first)) join_parts<HD, C::BM>(p, s);
+      if (ticket == (unsigned)(s.c_last - s.c_first)) join_parts_f32<HD, C::BM, kThreads>(p, s);
     }
   }
 }
@@ -538,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, Few<HD, R>::CTAS)
       __syncthreads();
       if (tid == 0) ticket = ticket_acq_rel(p.counters + s.c_first);
       __syncthreads();
-      if (ticket == (unsigned)(s.c_last - s.c_first)) join_parts<HD, R>(p, s);
+      if (ticket == (unsigned)(s.c_last - s.c_first)) join_parts_f32<HD, R, kThreads>(p, s);
     }
   }
 }
