@@ -3,7 +3,7 @@
 // An f32 number is the sum of three bf16 ones (8 bits each), x = x0 + x1 + x2, so a product
 // of two is x0 y0 + (x0 y1 + x1 y0) + (x0 y2 + x1 y1 + x2 y0) and terms below 2^-24 of it: six
 // bf16 products with fp32 accumulators, where the CUDA cores have one product per lane and
-// clock (25 heads of 64, prompts of 3076 tokens on a B200: CUDA cores 302 us, TC_US us here).
+// clock (25 heads of 64, prompts of 3076 tokens on a B200: CUDA cores 302 us, 145 us here with the split).
 // A first kernel splits q, k and v into planes; the weights are split where they are made.
 //
 // The tensor cores cut what their fp32 accumulator cannot hold (measured: toward zero, two
@@ -56,37 +56,42 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __grid_constant__
                                                          __nv_bfloat16* planes, int* flags) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int all = heads + 2 * p.kv_heads, quads = p.head_dim / 4, each = all * quads;
-  const int64_t plane = p.rows * all * p.head_dim;
+  const int64_t plane = p.rows * all * p.head_dim, r0 = (int64_t)blockIdx.x * kSplitRows;
   int odd = 0;  // of v
-  for (int e = threadIdx.x; e < kSplitRows * each; e += 256) {
-    const int64_t r = (int64_t)blockIdx.x * kSplitRows + e / each;
-    if (r >= p.rows) break;
-    const int h = e % each / quads, d = e % quads * 4;
-    const float* src = h < heads                ? p.q + r * p.q_row + h * p.q_head
-                       : h < heads + p.kv_heads ? p.k + r * p.k_row + (h - heads) * p.k_head
-                                                : p.v + r * p.v_row + (h - heads - p.kv_heads) * p.v_head;
-    const float4 u = *reinterpret_cast<const float4*>(src + d);
-    float x[4] = {u.x, u.y, u.z, u.w};
+  for (int e = threadIdx.x; e < each; e += 256) {
+    const int h = e / quads, d = (e - h * quads) * 4;
     const bool is_v = h >= heads + p.kv_heads;
+    const float* src = (h < heads ? p.q + h * p.q_head : is_v ? p.v + (h - heads - p.kv_heads) * p.v_head
+                                                              : p.k + (h - heads) * p.k_head) + d;
+    const int64_t stride = h < heads ? p.q_row : is_v ? p.v_row : p.k_row;
+    float4 u[kSplitRows];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      if (fabsf(x[y]) < INFINITY) continue;
-      odd |= is_v;
-      x[y] = is_v ? 0.0f : NAN;
-    }
-    __nv_bfloat16* dst = planes + (r * all + h) * p.head_dim + d;
+    for (int r = 0; r < kSplitRows; ++r)
+      if (r0 + r < p.rows) u[r] = *reinterpret_cast<const float4*>(src + (r0 + r) * stride);
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      float z[4];
+    for (int r = 0; r < kSplitRows; ++r) {
+      if (r0 + r >= p.rows) break;
+      float x[4] = {u[r].x, u[r].y, u[r].z, u[r].w};
 #pragma unroll
-      for (int y = 0; y < 4; ++y)  // (nothing rounds up to infinity)
-        z[y] = i == 0 && fabsf(x[y]) > 3.3895314e38f ? copysignf(3.3895314e38f, x[y]) : x[y];
-      const uint32_t lo = pack_bf16(z[0], z[1]), hi = pack_bf16(z[2], z[3]);
-      *reinterpret_cast<uint2*>(dst + i * plane) = make_uint2(lo, hi);
-      const float b[4] = {__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u), __uint_as_float(hi << 16),
-                          __uint_as_float(hi & 0xffff0000u)};
+      for (int y = 0; y < 4; ++y) {
+        if (fabsf(x[y]) < INFINITY) continue;
+        odd |= is_v;
+        x[y] = is_v ? 0.0f : NAN;
+      }
+      __nv_bfloat16* dst = planes + ((r0 + r) * all + h) * p.head_dim + d;
 #pragma unroll
-      for (int y = 0; y < 4; ++y) x[y] = b[y] == b[y] ? x[y] - b[y] : 0.0f;
+      for (int i = 0; i < 3; ++i) {
+        float z[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y)  // (nothing rounds up to infinity)
+          z[y] = i == 0 && fabsf(x[y]) > 3.3895314e38f ? copysignf(3.3895314e38f, x[y]) : x[y];
+        const uint32_t lo = pack_bf16(z[0], z[1]), hi = pack_bf16(z[2], z[3]);
+        *reinterpret_cast<uint2*>(dst + i * plane) = make_uint2(lo, hi);
+        const float b[4] = {__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u), __uint_as_float(hi << 16),
+                            __uint_as_float(hi & 0xffff0000u)};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[y] = b[y] == b[y] ? x[y] - b[y] : 0.0f;
+      }
     }
   }
   const int any = __syncthreads_or(odd);
@@ -203,11 +208,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto add_block = [&]() {
         if (!warp_wait(o_full, n_o++ & 1)) return false;
         tc_fence_after();
-        float pv[32];
-        tmem_ld32(quad + kColO + d0, pv);
-        tmem_wait_ld();
 #pragma unroll
-        for (int y = 0; y < 32; ++y) o[y] += pv[y];
+        for (int i = 0; i < 32; i += 16) {
+          uint32_t pv[16];
+          tmem_ld_32x32b_x16(quad + kColO + d0 + i, pv);
+          tmem_wait_ld();
+#pragma unroll
+          for (int y = 0; y < 16; ++y) o[i + y] += __uint_as_float(pv[y]);
+        }
         return true;
       };
 #pragma unroll 1
@@ -250,30 +258,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         l = l * keep + (sum.x + sum.y);
         m = m1;
-        // The last block's product has to be in before its weights' place is used again.
-        if (x > 0) ok = add_block();
+        // The weights' planes, while the last block's product is still being formed.
+        uint32_t w[3][32];
 #pragma unroll
-        for (int y = 0; y < 32; ++y) o[y] *= keep;
+        for (int plane = 0; plane < 3; ++plane)
+#pragma unroll
+          for (int y = 0; y < 32; ++y) {
+            w[plane][y] = pack_bf16(v[2 * y], v[2 * y + 1]);
+            if (plane < 2) {
+              v[2 * y] -= __uint_as_float(w[plane][y] << 16);
+              v[2 * y + 1] -= __uint_as_float(w[plane][y] & 0xffff0000u);
+            }
+          }
+        // That product has to be in before its place and its weights' are used again.
+        if (x > 0) ok = add_block();
         // (Leaving alone is safe: the other warp's next wait fails, and so does its swap.)
         if (!ok) *pair_failed = 1;
 #pragma unroll
-        for (int i = 0; i < 64; i += 32) {
-#pragma unroll
-          for (int plane = 0; plane < 3; ++plane) {
-            uint32_t w[16];
-#pragma unroll
-            for (int y = 0; y < 16; ++y) {
-              w[y] = pack_bf16(v[i + 2 * y], v[i + 2 * y + 1]);
-              v[i + 2 * y] -= __uint_as_float(w[y] << 16);
-              v[i + 2 * y + 1] -= __uint_as_float(w[y] & 0xffff0000u);
-            }
-            tmem_st16(quad + kColP + plane * 64 + half * 32 + (i >> 1), w);
-          }
+        for (int plane = 0; plane < 3; ++plane) {
+          tmem_st16(quad + kColP + plane * 64 + half * 32, reinterpret_cast<const uint32_t(&)[16]>(w[plane][0]));
+          tmem_st16(quad + kColP + plane * 64 + half * 32 + 16, reinterpret_cast<const uint32_t(&)[16]>(w[plane][16]));
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full);
+#pragma unroll
+        for (int y = 0; y < 32; ++y) o[y] *= keep;
       }
       if (ok) ok = add_block();
       tc_fence_before();
