@@ -519,8 +519,10 @@ int mtrtq_decode_next(unsigned long long* best, int64_t rows, int32_t* tok, int3
  * a row that sees no key gives zeros. Keys outside a row's view have no effect on it,
  * whatever they hold (infinities and NaN included).
  *
- * Element types: x_dtype of q, k and v; dtype of the cache and of out. Both f32: every
- * product and sum in fp32. dtype bf16 (x_dtype f32 or bf16): k and v are rounded to
+ * Element types: x_dtype of q, k and v; dtype of the cache and of out. Both f32: fp32
+ * throughout (long prompts of up to 64 dimensions form each product from three bf16 parts
+ * of either factor, to fp32's precision, on the tensor cores; there an infinite q or k
+ * counts as NaN). dtype bf16 (x_dtype f32 or bf16): k and v are rounded to
  * bf16 as they are stored, q and the weights p are rounded to bf16 for the tensor
  * cores' products, the maximum, the sum and the output are held in fp32 and out is
  * rounded once. x_dtype bf16 with dtype f32 is refused.

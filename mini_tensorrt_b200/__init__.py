@@ -10,6 +10,8 @@ Hand-written sm_100a kernels behind a C ABI (include/mtrtq.h, libmtrtq.so):
     bf16 and fed to tcgen05.mma with fp32 accumulators in TMEM, scale and bias
     in the epilogue;
   * fp32 mode above M = 32: a CUDA-core split-K GEMV.
+Serving many requests together (serving.py, paged.py): attention of packed prompts and of
+new tokens over a paged key/value cache, a beam search step and the cache's reordering.
 The Python layer here is plumbing (device memory, streams, the registry mirror);
 the library raises if libmtrtq.so is missing -- there is no CPU fallback.
 """
@@ -17,6 +19,7 @@ from ._lib import MtrtqError, lib  # noqa: F401
 from .matmulq import (PackedWeight, Workspace, matmul_q8, packed_bytes, plan_info,  # noqa: F401
                       prepack_host, quantize_per_channel, read_device_status, set_option,
                       workspace_bytes)
+from .serving import beam_reorder, beam_select, paged_attention, prompt_attention  # noqa: F401
 from .registry import (DType, GraphError, KernelRegistry, Node, OpContext,  # noqa: F401
                        register_cuda_kernels, run_kernel)
 
