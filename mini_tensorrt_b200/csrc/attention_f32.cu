@@ -6,8 +6,9 @@
 // (ty, tx) the rows ty RM .. and the keys 4 tx .. of the scores, then the same rows and
 // dimensions 4 tx .. of the output. Q and K lie transposed in shared memory, so that one
 // dimension's step is RM + 4 values read for 4 RM products (packed two at a time), and P
-// transposed for the same reason. Bound by the fp32 units for tiles of many rows: one
-// product of each score and output element per lane and clock.
+// transposed for the same reason. Bound by these reads of shared
+// memory (65 to 70 % of its rate with tiles of 128 rows; four chunks of 1 to 128 tokens, 25
+// heads of 64, over up to 1000: 67 us, 44 %); 32 x 8 threads instead of 16 x 16 were slower.
 //
 // V rows past the request's keys are read as zeros; where a block not seen whole by every
 // row holds an infinity or a NaN, its products are formed only for the rows that see them.
@@ -309,7 +310,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
 // dimensions) share a key, eight dimensions each, with the rows of q in registers: four
 // keys' K and V are loaded together and used straight from the registers, without shared
 // memory or barriers. Every such group of lanes keeps its own maximum, sum and output; they
-// are joined when the CTA's run of the tile ends.
+// are joined when the CTA's run of the tile ends. 32 requests of 1500 tokens, 12 heads of 64,
+// take 61 us on a B200: 4.9 TB/s.
 template <int HD, int R>
 struct Few {
   static constexpr int LANES = HD / 8;             // of a key

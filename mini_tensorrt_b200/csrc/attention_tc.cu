@@ -24,6 +24,11 @@
 // the lengths in device memory. A tile cut between CTAs leaves partial (m, l, O) in the
 // workspace, and the CTA that finishes last joins them in order.
 //
+// Bound by a row's chain of exponentials, not by the products or the memory: on a B200 a
+// prompt of 8192 tokens, 32 heads over 8 of 128 dimensions, takes 580 to 667 us with the clock
+// (tensor pipe 41 % of cycles); 64 requests of 100 to 8192 tokens decoding with the same heads
+// 160 us, 3.8 TB/s of keys and values.
+//
 // One CTA = 20 warps: 0..7 and 8..15 the slots' softmax (two threads per row, of 64 keys
 // each, also the epilogue), 16 TMA loads, 17 and 18 issue the slots' products, 19 looks over
 // the V blocks that not every row sees whole: rows past the request's keys are zeroed (a
