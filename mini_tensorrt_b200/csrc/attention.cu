@@ -341,12 +341,27 @@ F32Layout f32_layout(const Args& a, int sm_count) {
   return l;
 }
 
+// Calls with a bf16 cache that go that way too: tiles of a row or two, for which the tensor
+// cores' 128 are mostly empty. On a B200, there and here: 16 requests of 20 to 1024 tokens, 12
+// heads of 64, 34 us and 26; 64 of 2000 146 and 101; 16 of 700, 16 heads of 128, 63 and 38, 16
+// over 8 44 and 29, 64 of 2000 152 and 148. Groups of four and more gain or lose with the
+// lengths, which the host does not know (4 requests of 300, 32 heads over 8, 29 and 20; 64 of 100
+// to 8192 157 and 262), and stay.
+bool few_rows16(const Args& a) {
+  if (a.dtype == MTRTQ_DTYPE_F32 || !a.k_pages) return false;
+  const F32Layout l = f32_layout(a, sm_count());
+  return l.tile_rows <= 2;
+}
+
 int launch_f32(const Args& a, bool paged, void* workspace, unsigned* status, cudaStream_t st) {
   const F32Layout l = f32_layout(a, sm_count());
+  const bool pages16 = a.dtype != MTRTQ_DTYPE_F32, q16 = a.x_dtype != MTRTQ_DTYPE_F32;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const bool before = paged && a.k;
   if (before) {
-    append_kernel<float, float><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, nullptr);
+    if (!pages16) append_kernel<float, float><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, nullptr);
+    else if (!q16) append_kernel<float, __nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, nullptr);
+    else append_kernel<__nv_bfloat16, __nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, nullptr);
     if (int rc = cuda_status(cudaGetLastError(), "attention rows launch")) return rc;
   }
   F32Attention p = {};
@@ -355,6 +370,8 @@ int launch_f32(const Args& a, bool paged, void* workspace, unsigned* status, cud
   p.tile_tokens = l.tile_rows / p.group;
   p.min_steps = 2;
   p.pair_cost = l.tile_rows == 128;  // (every f32 tile is of that kind)
+  p.pages16 = pages16;
+  p.q16 = q16;
   p.scale = a.scale;
   p.q = static_cast<const float*>(a.q);
   p.k = static_cast<const float*>(paged ? a.k_pages : a.k);
@@ -414,7 +431,7 @@ int attention(const Args* a, bool paged, void* workspace, size_t workspace_bytes
   if (reinterpret_cast<uintptr_t>(workspace) % 256)
     return report_error(MTRTQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == MTRTQ_DTYPE_F32) return launch_f32(*a, paged, workspace, status, st);
+  if (a->dtype == MTRTQ_DTYPE_F32 || few_rows16(*a)) return launch_f32(*a, paged, workspace, status, st);
   return launch_tc(*a, paged, workspace, status, st);
 }
 
@@ -427,7 +444,7 @@ extern "C" {
 
 int64_t mtrtq_attention_workspace_bytes(const mtrtq_attention_args* a) {
   if (check_args(a, a && a->k_pages)) return -1;
-  return (int64_t)(a->dtype == MTRTQ_DTYPE_F32 ? f32_layout(*a, sm_count()).total : tc_layout(*a, sm_count()).total);
+  return (int64_t)(a->dtype == MTRTQ_DTYPE_F32 || few_rows16(*a) ? f32_layout(*a, sm_count()).total : tc_layout(*a, sm_count()).total);
 }
 
 int mtrtq_prompt_attention(const mtrtq_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {

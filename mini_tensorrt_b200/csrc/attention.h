@@ -39,9 +39,10 @@ struct TcAttention : AttentionList {
 };
 
 // fp32 throughout, on the CUDA cores (attention_f32.cu): tiles of 1, 2, 4, 8, 16, 64 or
-// 128 rows.
+// 128 rows; those of 1 and 2 also with pages and out (pages16) and q (q16) in bf16.
 struct F32Attention : AttentionList {
   float scale;
+  bool pages16, q16;
   const float *q, *k, *v;  // paged: k and v are the pages, k_row and v_row the page stride
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   float* out;

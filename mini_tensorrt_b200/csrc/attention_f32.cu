@@ -1,5 +1,5 @@
 // Attention with every product and sum in fp32, on the CUDA cores: packed prompts and new
-// tokens over a paged cache whose rows and pages are f32.
+// tokens over a paged cache whose rows and pages are f32 (for a row or two, bf16 too).
 //
 // The same online softmax as on the tensor cores (attention_tc.cu), over blocks of 64 keys:
 // a CTA of 256 threads holds a tile of 16 RM rows (tokens times the group's heads), thread
@@ -308,22 +308,52 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
 // A tile of up to R rows (one token's group of heads, as a rule) needs 2 R products for each
 // element of K and V, so the time is that of reading them. Eight lanes (16 for 128
 // dimensions) share a key, eight dimensions each, with the rows of q in registers: four
-// keys' K and V are loaded together and used straight from the registers, without shared
-// memory or barriers. Every such group of lanes keeps its own maximum, sum and output; they
+// keys' K and V (eight of bf16) are loaded together and used straight from the registers,
+// without shared memory or barriers. Every such group of lanes keeps its own maximum, sum and output; they
 // are joined when the CTA's run of the tile ends. 32 requests of 1500 tokens, 12 heads of 64,
-// take 61 us on a B200: 4.9 TB/s.
-template <int HD, int R>
+// take 61 us on a B200: 4.9 TB/s. With a bf16 cache, where q and the weights stay in fp32, the
+// instructions for each element weigh twice as much: 64 requests of 2000 tokens take 101 us,
+// 3.9 TB/s; with four keys of bf16 together 109.
+template <typename T>
+struct Eight {  // dimensions of a row, as they are read
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (uint4& x : u) x = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void load(const T* src) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(src)[i];
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        x[4 * i] = __uint_as_float(u[i].x), x[4 * i + 1] = __uint_as_float(u[i].y);
+        x[4 * i + 2] = __uint_as_float(u[i].z), x[4 * i + 3] = __uint_as_float(u[i].w);
+      }
+    } else {
+      const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+
+template <int HD, int R, typename T>
 struct Few {
   static constexpr int LANES = HD / 8;             // of a key
-  static constexpr int KEYS = 4;                   // of a lane, loaded together
+  static constexpr int KEYS = sizeof(T) == 4 ? 4 : 8;  // of a lane, loaded together (as many bytes)
   static constexpr int BLOCK = kThreads / LANES * KEYS;
   static constexpr int CTAS = R <= 2 ? 2 : 1;
 };
 
-template <int HD, int R, bool PAGED>
-__global__ void __launch_bounds__(kThreads, Few<HD, R>::CTAS)
-    attention_f32_few_kernel(const __grid_constant__ F32Attention p) {
-  using F = Few<HD, R>;
+// T: of k, v and out; TQ: of q.
+template <int HD, int R, bool PAGED, typename T, typename TQ>
+__global__ void __launch_bounds__(kThreads, Few<HD, R, T>::CTAS)
+    attention_few_kernel(const __grid_constant__ F32Attention p) {
+  using F = Few<HD, R, T>;
   constexpr int LANES = F::LANES, KEYS = F::KEYS;
   extern __shared__ float4 raw4[];
   float* joined = reinterpret_cast<float*>(raw4);  // [8 warps][R][HD], then their (m, l)
@@ -357,14 +387,11 @@ __global__ void __launch_bounds__(kThreads, Few<HD, R>::CTAS)
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int token = r / p.group, head = r - token * p.group;
-      float4 x = make_float4(0, 0, 0, 0), y = x;
-      if (r < rows && in0) {
-        const float* src = p.q + (s.row0 + (int64_t)token) * p.q_row + (int64_t)(s.h * p.group + head) * p.q_head + d0;
-        x = *reinterpret_cast<const float4*>(src);
-        y = *reinterpret_cast<const float4*>(src + 4);
-      }
-      q[r][0] = x.x, q[r][1] = x.y, q[r][2] = x.z, q[r][3] = x.w;
-      q[r][4] = y.x, q[r][5] = y.y, q[r][6] = y.z, q[r][7] = y.w;
+      Eight<TQ> x;
+      x.zero();
+      if (r < rows && in0)
+        x.load(reinterpret_cast<const TQ*>(p.q) + (s.row0 + (int64_t)token) * p.q_row + (int64_t)(s.h * p.group + head) * p.q_head + d0);
+      x.get(q[r]);
       sees[r] = r < rows ? max(0, min(s.see0 + token, keys)) : 0;
       m[r] = -INFINITY;
       l[r] = 0.0f;
@@ -373,70 +400,72 @@ __global__ void __launch_bounds__(kThreads, Few<HD, R>::CTAS)
     }
     const int k1 = s.k0 + s.n;
     for (int j = s.k0; j < k1; ++j) {
-      float4 k[KEYS][2], v[KEYS][2];
+      Eight<T> k[KEYS], v[KEYS];
 #pragma unroll
       for (int c = 0; c < KEYS; ++c) {
         const int key = j * F::BLOCK + c * (kThreads / LANES) + mine;
-        k[c][0] = k[c][1] = v[c][0] = v[c][1] = make_float4(0, 0, 0, 0);
+        k[c].zero();
+        v[c].zero();
         if (key < keys && in0) {
-          const float *ks, *vs;
+          const T *ks = reinterpret_cast<const T*>(p.k), *vs = reinterpret_cast<const T*>(p.v);
           bool there = true;
           if (PAGED) {
             const int64_t page = p.table[s.b * p.table_ld + key / p.page_size];
             there = page >= 0 && page < p.num_pages;  // else the token reads as zeros
             const int64_t at = ((int64_t)s.h * p.page_size + key % p.page_size) * p.head_dim + d0;
-            ks = p.k + page * p.k_row + at;
-            vs = p.v + page * p.v_row + at;
+            ks += page * p.k_row + at;
+            vs += page * p.v_row + at;
           } else {
-            ks = p.k + (r0 + key) * p.k_row + s.h * p.k_head + d0;
-            vs = p.v + (r0 + key) * p.v_row + s.h * p.v_head + d0;
+            ks += (r0 + key) * p.k_row + s.h * p.k_head + d0;
+            vs += (r0 + key) * p.v_row + s.h * p.v_head + d0;
           }
           if (there) {
-            k[c][0] = *reinterpret_cast<const float4*>(ks);
-            k[c][1] = *reinterpret_cast<const float4*>(ks + 4);
-            v[c][0] = *reinterpret_cast<const float4*>(vs);
-            v[c][1] = *reinterpret_cast<const float4*>(vs + 4);
+            k[c].load(ks);
+            v[c].load(vs);
           }
         }
       }
+      float e[R][KEYS];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float e[KEYS], top = m[r];
+      for (int c = 0; c < KEYS; ++c) {
+        float y[8];
+        k[c].get(y);
 #pragma unroll
-        for (int c = 0; c < KEYS; ++c) {
-          float x = q[r][0] * k[c][0].x;
-          x = fmaf(q[r][1], k[c][0].y, x);
-          x = fmaf(q[r][2], k[c][0].z, x);
-          x = fmaf(q[r][3], k[c][0].w, x);
-          x = fmaf(q[r][4], k[c][1].x, x);
-          x = fmaf(q[r][5], k[c][1].y, x);
-          x = fmaf(q[r][6], k[c][1].z, x);
-          x = fmaf(q[r][7], k[c][1].w, x);
+        for (int r = 0; r < R; ++r) {
+          float x = q[r][0] * y[0];
+#pragma unroll
+          for (int d = 1; d < 8; ++d) x = fmaf(q[r][d], y[d], x);
 #pragma unroll
           for (int w = LANES / 2; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-          e[c] = j * F::BLOCK + c * (kThreads / LANES) + mine < sees[r] ? x : -INFINITY;
-          top = fmaxf(top, e[c] * c2);
+          e[r][c] = x;
         }
-        const float base = top == -INFINITY ? 0.0f : top;
-        const float keep = m[r] == -INFINITY ? 1.0f : ex2(m[r] - base);
+      }
+      float base[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int c = 0; c < KEYS; ++c)
+          if (j * F::BLOCK + c * (kThreads / LANES) + mine < sees[r]) top = fmaxf(top, e[r][c] * c2);
+        base[r] = top == -INFINITY ? 0.0f : top;
+        const float keep = m[r] == -INFINITY ? 1.0f : ex2(m[r] - base[r]);
         m[r] = top;
         l[r] *= keep;
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[r][d] *= keep;
+      }
 #pragma unroll
-        for (int c = 0; c < KEYS; ++c) {
+      for (int c = 0; c < KEYS; ++c) {
+        float y[8];
+        v[c].get(y);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
           // a key that the row does not see adds nothing, whatever its v
           if (j * F::BLOCK + c * (kThreads / LANES) + mine >= sees[r]) continue;
-          const float w = ex2(fmaf(e[c], c2, -base));
+          const float w = ex2(fmaf(e[r][c], c2, -base[r]));
           l[r] += w;
-          o[r][0] = fmaf(w, v[c][0].x, o[r][0]);
-          o[r][1] = fmaf(w, v[c][0].y, o[r][1]);
-          o[r][2] = fmaf(w, v[c][0].z, o[r][2]);
-          o[r][3] = fmaf(w, v[c][0].w, o[r][3]);
-          o[r][4] = fmaf(w, v[c][1].x, o[r][4]);
-          o[r][5] = fmaf(w, v[c][1].y, o[r][5]);
-          o[r][6] = fmaf(w, v[c][1].z, o[r][6]);
-          o[r][7] = fmaf(w, v[c][1].w, o[r][7]);
+#pragma unroll
+          for (int d = 0; d < 8; ++d) o[r][d] = fmaf(w, y[d], o[r][d]);
         }
       }
     }
@@ -490,9 +519,9 @@ __global__ void __launch_bounds__(kThreads, Few<HD, R>::CTAS)
       if (whole) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         if (d < p.head_dim)
-          *reinterpret_cast<float4*>(p.out + (s.row0 + (int64_t)token) * p.out_row +
-                                     (int64_t)(s.h * p.group + head) * p.out_head + d) =
-              make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+          put4(reinterpret_cast<T*>(p.out) + (s.row0 + (int64_t)token) * p.out_row +
+                   (int64_t)(s.h * p.group + head) * p.out_head + d,
+               make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
       } else {
         __stcg(reinterpret_cast<float4*>(p.partials + (part * R + row) * HD + d), x);
         if (d == 0) __stcg(p.part_ml + part * R + row, make_float2(top, sum));
@@ -502,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, Few<HD, R>::CTAS)
       __syncthreads();
       if (tid == 0) ticket = ticket_acq_rel(p.counters + s.c_first);
       __syncthreads();
-      if (ticket == (unsigned)(s.c_last - s.c_first)) join_parts_f32<HD, R, kThreads>(p, s);
+      if (ticket == (unsigned)(s.c_last - s.c_first)) join_parts_f32<HD, R, kThreads, T>(p, s);
     }
   }
 }
@@ -535,7 +564,13 @@ cudaError_t launch_tile(const F32Attention& p, int grid, bool pdl, cudaStream_t 
 template <int HD, int R, bool PAGED>
 cudaError_t launch_few(const F32Attention& p, int grid, bool pdl, cudaStream_t st) {
   const int bytes = 8 * R * (HD * 4 + 8), prefix = (MTRTQ_MAX_BATCH + 2) / 2 * 16;
-  return launch(attention_f32_few_kernel<HD, R, PAGED>, p, bytes > prefix ? bytes : prefix, grid, pdl, st);
+  const int all = bytes > prefix ? bytes : prefix;
+  if constexpr (PAGED && R <= 2) {
+    using bf16 = __nv_bfloat16;
+    if (p.pages16 && p.q16) return launch(attention_few_kernel<HD, R, true, bf16, bf16>, p, all, grid, pdl, st);
+    if (p.pages16) return launch(attention_few_kernel<HD, R, true, bf16, float>, p, all, grid, pdl, st);
+  }
+  return launch(attention_few_kernel<HD, R, PAGED, float, float>, p, all, grid, pdl, st);
 }
 
 template <int HD, bool PAGED>

@@ -159,9 +159,17 @@ __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
   while (!mbar_try_wait(bar, parity) && clock64() - t0 < kSpinLimitCycles) {}
 }
 
+// Four elements of a row of out, as its type.
+__device__ __forceinline__ void put4(float* dst, float4 x) { *reinterpret_cast<float4*>(dst) = x; }
+__device__ __forceinline__ void put4(__nv_bfloat16* dst, float4 x) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(x.x, x.y), hi = __floats2bfloat162_rn(x.z, x.w);
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(reinterpret_cast<const uint32_t&>(lo), reinterpret_cast<const uint32_t&>(hi));
+}
+
 // The CTA that finishes a cut tile last joins its parts, in order: THREADS threads,
 // from the first on.
-template <int HD, int BM, int THREADS>
+template <int HD, int BM, int THREADS, typename T = float>
 __device__ __forceinline__ void join_parts_f32(const F32Attention& p, const Segment& s) {
   const int c_first = s.c_first, c_last = s.c_last, rows = s.tokens * p.group, vecs = p.head_dim / 4;
 #pragma unroll 1
@@ -185,9 +193,9 @@ __device__ __forceinline__ void join_parts_f32(const F32Attention& p, const Segm
       x.w += y.w * w;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<float4*>(p.out + (s.row0 + (int64_t)token) * p.out_row +
-                               (int64_t)(s.h * p.group + head) * p.out_head + d) =
-        make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    put4(reinterpret_cast<T*>(p.out) + (s.row0 + (int64_t)token) * p.out_row +
+             (int64_t)(s.h * p.group + head) * p.out_head + d,
+         make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
   }
   if (threadIdx.x == 0) p.counters[c_first] = 0u;
 }

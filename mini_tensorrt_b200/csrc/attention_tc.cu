@@ -16,8 +16,8 @@
 // the end -- which is what a single token over a long cache needs.
 //
 // Roundings: the weights to bf16 (their sum is that of the unrounded ones), and f32 rows of q
-// to bf16 (16 requests decoding, f32 rows: error against 64 bits 2.9e-3). A second plane of q
-// is no way out: its zeros times an infinite k would be NaN where the score is -inf.
+// to bf16. A second plane of q is no way out: its zeros times an infinite k would be NaN where
+// the score is -inf. (A row or two of a request go to attention_f32.cu, which rounds neither.)
 //
 // Work: a step is one block for each slot. The steps of all tiles of all requests form
 // one list, cut into equal runs over one CTA per SM; every CTA finds its own run from

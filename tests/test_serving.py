@@ -248,6 +248,34 @@ def test_decode(cuda_device, kind, heads, page):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("heads", [(4, 2, 64), (8, 4, 128), (6, 3, 40)], ids=str)
+@pytest.mark.parametrize("new,lens", [([1] * 6, [1, 2, 255, 256, 257, 900]), ([1], [3000]),
+                                      ([4, 0, 0, 0, 0, 1], [610, 9, 0, 5, 33, 2])], ids=str)
+def test_decode_pairs_of_heads(cuda_device, kind, heads, new, lens):
+    """Tiles of two rows, also where one request has more tokens than the others together."""
+    H, KV, D = heads
+    s = Paged(new, lens, H, KV, D, 32, kind, seed=len(new))
+    s.verify(s.run())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("heads", [(2, 2, 64), (4, 2, 128), (8, 2, 128)], ids=str)
+def test_decode_key_of_minus_infinity_has_no_weight(cuda_device, kind, heads):
+    """An infinite element of a key makes a score of -infinity where q is negative there: the
+    token counts for nothing, as if it were not there."""
+    H, KV, D = heads
+    x = Paged([1, 1], [200, 70], H, KV, D, 16, kind, seed=8)
+    x.q[..., 5] = -x.q[..., 5].abs() - 0.1
+    at = [x.table[b, 2].item() for b in range(2)]
+    for page in at:
+        x.kp[page, :, 7, 5] = INF
+    got = x.run()
+    for b, n in enumerate(x.lens):
+        keep = torch.arange(n, device="cuda") != 39
+        near(got[b:b + 1], *reference(x.q[b:b + 1], x.keys[b][keep], x.values[b][keep], [n - 1], D ** -0.5), kind, D, [n - 1])
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("heads", [(12, 12, 64), (8, 2, 128), (6, 2, 80), (5, 1, 64)], ids=str)
 @pytest.mark.parametrize("page", [32, 64])
 def test_chunks(cuda_device, kind, heads, page):
