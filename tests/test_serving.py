@@ -6,10 +6,11 @@ as the root of their number, and six standard deviations are allowed.
 * f32 (unit roundoff u = 2^-24): a score of D products is off by about u sqrt(D) S, a
   weight by as much of itself, the sums over n keys by u sqrt(n):
   |error| <= u V (6 sqrt(D) S + 6 sqrt(n) + 16).
-* bf16 (u = 2^-9): a weight is rounded once (u of itself), the output once, and f32 rows
-  round q (u S / sqrt(3) standard deviation on a score, as much of itself on a weight):
-  |error| <= u (|ref| + V (2 + 4 S)), 4 = 6 / sqrt(3) rounded up, without the S term for
-  bf16 rows; and over a whole output the errors' norm is at most 2^-8 of the result's
+* bf16 (a rounding is off by up to 2 u of the value, u = 2^-9, and by less than u in the
+  mean): the output is rounded once, up to 2 u |ref| <= u (|ref| + V); the weights once each,
+  which leaves u V for their sum; and f32 rows round q (u S / sqrt(3) standard deviation on a
+  score, as much of itself on a weight): |error| <= u (|ref| + V (2 + 4 S)), 4 = 6 / sqrt(3)
+  rounded up, without the S term for bf16 rows; and over a whole output the errors' norm is at most 2^-8 of the result's
   (2^-7 with f32 rows).
 """
 import math
