@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = swap(ok, l, other);
       if (!ok) break;
       l = half ? other + l : l + other;
+      if (m == -INFINITY && l != l) m = 0.0f;  // every score it saw was NaN: the join must not pass it over
       if (__any_sync(0xffffffffu, flagged) && live) {
 #pragma unroll 1
         for (int key = s.k0 * kBlock; key < min(keys, (s.k0 + n) * kBlock); ++key) {
