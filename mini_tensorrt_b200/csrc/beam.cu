@@ -27,7 +27,8 @@ __device__ __forceinline__ float key_score(unsigned long long key) {
 }
 __device__ __forceinline__ uint32_t key_index(unsigned long long key) { return ~(uint32_t)key; }
 
-__device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY; }
+// A logit or score as it counts: NaN as -infinity.
+__device__ __forceinline__ float number(float x) { return x == x ? x : -INFINITY; }
 
 constexpr int kThreads = 256;
 // Logits of one row that a block looks at: 16 per thread, 32 where that still leaves every
@@ -162,8 +163,7 @@ __device__ void block_top(int want, Shared& sh, Each each) {
 
 // Candidate (w, t)'s score, with what its row's logits are worth in all.
 __device__ __forceinline__ float row_score(float base, float x, float lse) {
-  const float s = base + (x - lse);
-  return s == s ? s : -INFINITY;
+  return number(base + (x - lse));
 }
 
 // One block per (chunk, row). It reads its logits once: their maximum and the sum of
@@ -362,8 +362,8 @@ __global__ void __launch_bounds__(kThreads, 5) beam_kernel(const __grid_constant
         const bool ended = p.done[r] != 0;
         const int t1 = min(p.vocab, (c + 1) * p.chunk - skip);
         for (int t = max(0, c * p.chunk - skip) + tid; t < t1; t += kThreads) {
-          const float s = ended ? (t == p.eos ? p.scores[r] : -INFINITY)
-                          : p.scores[r] > -INFINITY ? row_score(p.scores[r], logit(y[t]), sh.lse[w])
+          const float s = ended ? (t == p.eos ? number(p.scores[r]) : -INFINITY)
+                          : p.scores[r] > -INFINITY ? row_score(p.scores[r], number(y[t]), sh.lse[w])
                                                     : -INFINITY;
           const unsigned long long key = candidate_key(s, (uint32_t)w * p.vocab + t);
           k = key < below && key > k ? key : k;

@@ -1,11 +1,11 @@
-"""What NaN and infinities in q and k do to the serving operators' results: the rows that
-meet them, and only those. Expected values follow from the formulas (a sum with a NaN is
-NaN), so they are compared exactly."""
+"""What NaN and infinities in q, k and the scores do to the serving operators' results: the
+rows and beams that meet them, and only those. Expected values follow from the formulas (a
+sum with a NaN is NaN, a NaN score counts as -infinity), so they are compared exactly."""
 import pytest
 import torch
 
 from mini_tensorrt_b200 import matmulq, serving
-from tests.test_serving import INF, NAN, TYPES, Paged, i32, make_gen, offsets, rows
+from tests.test_serving import INF, NAN, TYPES, Paged, i32, make_gen, offsets, randn, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,22 @@ def test_paged_rows_of_broken_q(cuda_device, kind, heads, new, lens):
     got = s.run()
     assert got[hit].isnan().all()
     assert torch.equal(got[1:-1], want[1:-1])
+
+
+@pytest.mark.parametrize("W,V", [(2, 50257), (4, 7), (8, 9000)])
+@pytest.mark.parametrize("nan", [NAN, -NAN])
+def test_beam_that_is_done_with_a_nan_score(cuda_device, W, V, nan):
+    """Its one candidate has a NaN score, which counts as -infinity: it comes after every
+    candidate with a score, and at its index among those without."""
+    logits = randn(make_gen(24), W, V)
+    scores = torch.full((1, W), -INF, device="cuda")
+    scores[0, 0], scores[0, 1] = -1.0, nan
+    done = torch.zeros((1, W), dtype=torch.uint8, device="cuda")
+    done[0, 1] = 1
+    keep = torch.zeros(V, dtype=torch.bool, device="cuda")
+    keep[5] = True
+    logits[0] = torch.where(keep, logits[0], torch.full_like(logits[0], -INF))  # one candidate in all
+    out_scores, parent, token, _ = serving.beam_select(logits, scores, done, 3)
+    at = (parent.long() * V + token)[0].tolist()
+    assert at == [5, *[t for t in range(W + 1) if t != 5][: W - 1]]
+    assert out_scores[0, 0] == -1.0 and (out_scores[0, 1:] == -INF).all()
