@@ -553,7 +553,7 @@ typedef struct mtrtq_attention_args {
   int x_dtype, dtype; /* MTRTQ_DTYPE_* */
   float scale;
   const int32_t* cu_rows; /* device [batch + 1] */
-  /* paged only */
+  /* paged only; k_pages, v_pages, table and kv_len are NULL for whole prompts (else MTRTQ_ERR_INVALID_ARG) */
   void *k_pages, *v_pages;
   int64_t page_stride, num_pages;
   int page_size;

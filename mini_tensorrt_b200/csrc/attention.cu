@@ -144,7 +144,12 @@ int check_args(const Args* a, bool paged) {
   if (!on16(a->q, a->q_row, a->q_head, xs) || (a->k && !on16(a->k, a->k_row, a->k_head, xs)) ||
       (a->v && !on16(a->v, a->v_row, a->v_head, xs)) || !on16(a->out, a->out_row, a->out_head, cs))
     return report_error(MTRTQ_ERR_ALIGNMENT, "q, k, v and out must be 16-byte aligned with strides of whole 16 bytes");
-  if (!paged) return MTRTQ_OK;
+  if (!paged) {
+    // (the layouts and the workspace query tell the calls apart by k_pages)
+    if (a->k_pages || a->v_pages || a->table || a->kv_len)
+      return report_error(MTRTQ_ERR_INVALID_ARG, "k_pages, v_pages, table and kv_len are for paged calls: NULL here");
+    return MTRTQ_OK;
+  }
   if (!a->k_pages || !a->v_pages || !a->table || !a->kv_len) return report_error(MTRTQ_ERR_INVALID_ARG, "null pointer");
   if (a->page_size != 16 && a->page_size != 32 && a->page_size != 64 && a->page_size != 128)
     return report_error(MTRTQ_ERR_INVALID_ARG, "page_size (%d) is 16, 32, 64 or 128", a->page_size);

@@ -1,0 +1,25 @@
+"""More of the serving calls' argument checks, through the C ABI without a GPU (every check
+comes before the device is looked for)."""
+import ctypes
+
+import pytest
+
+from mini_tensorrt_b200 import _lib
+from tests.test_serving_host import A, paged, prompt
+
+
+@pytest.mark.parametrize("field", ["k_pages", "v_pages", "table", "kv_len"])
+def test_prompt_call_with_paged_arguments_refused(field):
+    """The sizes of a call with pages are not those of a prompt's, so a struct kept for both
+    would have the rows written past the workspace."""
+    a = prompt(**{field: A})
+    assert _lib.lib().mtrtq_prompt_attention(ctypes.byref(a), None, 0, None) == _lib.ERR_INVALID_ARG
+    assert "NULL" in _lib.last_error()
+
+
+@pytest.mark.parametrize("over", [{}, {"dtype": _lib.DTYPE_BF16}, {"x_dtype": _lib.DTYPE_BF16, "dtype": _lib.DTYPE_BF16}])
+def test_prompt_call_with_a_whole_cache_refused(over):
+    a = paged(**over)
+    assert _lib.lib().mtrtq_attention_workspace_bytes(ctypes.byref(a)) > 0  # of the paged call
+    assert _lib.lib().mtrtq_prompt_attention(ctypes.byref(a), A, 1 << 40, None) == _lib.ERR_INVALID_ARG
+    assert "NULL" in _lib.last_error()
