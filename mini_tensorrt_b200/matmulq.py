@@ -112,17 +112,23 @@ class PackedWeight:
 
 
 class Workspace:
-    """Zero-filled device scratch grown on demand (only when a call needs more)."""
+    """Zero-filled device scratch grown on demand (only when a call needs more). Calls that
+    share one must be ordered."""
 
     def __init__(self, device="cuda"):
         self.device = torch.device(device)
         self.buf: torch.Tensor | None = None
 
-    def get(self, nbytes: int) -> torch.Tensor | None:
+    def get(self, nbytes: int, stream: torch.cuda.Stream | None = None) -> torch.Tensor | None:
+        """stream: that of the call that needs it, if not the current one. A new buffer is
+        made and zero-filled there, and the old one not given out again before the work there."""
         if nbytes <= 0:
             return None
         if self.buf is None or self.buf.numel() < nbytes:
-            self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+            with torch.cuda.stream(stream):
+                if self.buf is not None:
+                    self.buf.record_stream(torch.cuda.current_stream(self.device))
+                self.buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
         return self.buf
 
 

@@ -43,17 +43,25 @@ def _call(where: str, index: int, *args) -> None:
             check(fn(*args), where)
 
 
-def _workspace(workspace, device, stream_ptr: int, nbytes: int):
-    """(address, bytes) of the caller's workspace (a Workspace, or a tensor), or of one
-    kept for each stream: calls that share a workspace must be ordered."""
+def _other_stream(stream, stream_ptr: int, index: int):
+    """The call's stream as torch's, None if it is the current one."""
+    if stream_ptr == torch._C._cuda_getCurrentRawStream(index):
+        return None
+    return stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream_ptr, device=index)
+
+
+def _workspace(workspace, device, stream_ptr: int, other, nbytes: int) -> torch.Tensor:
+    """The caller's workspace (a Workspace, or a tensor), or one kept for each stream: calls
+    that share a workspace must be ordered. What is made here is made and zero-filled on the
+    call's stream (other, or the current one)."""
     if workspace is None:
         key = (device.index, stream_ptr)
         workspace = _workspaces.get(key)
         if workspace is None:
             workspace = _workspaces[key] = Workspace(device)
     if isinstance(workspace, Workspace):
-        workspace = workspace.get(nbytes)
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        workspace = workspace.get(nbytes, other)
+    return workspace
 
 
 def _rows(name: str, x: torch.Tensor, shape, dtype, device):
@@ -108,9 +116,11 @@ def _attend(where, q, k, v, out, out_dtype, kv_heads, cu_rows, scale, workspace,
               cu_rows.data_ptr(), *pages)
     sp = _stream_ptr(stream, index)
     need = lib().mtrtq_attention_workspace_bytes(a)
-    # arguments that the query refuses are refused by the call, with the reason
-    ws, nbytes = _workspace(workspace, device, sp, need) if need > 0 else (None, 0)
-    _call(where, index, a, ws, nbytes, sp)
+    if need > 0:
+        ws = _workspace(workspace, device, sp, _other_stream(stream, sp, index), need)
+        _call(where, index, a, ws.data_ptr(), ws.numel() * ws.element_size(), sp)
+    else:  # refused by the call too, with the reason
+        _call(where, index, a, None, 0, sp)
     return out
 
 
@@ -196,9 +206,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor, 
     V = logits.shape[1]
     sp = _stream_ptr(stream, dev.index)
     need = lib().mtrtq_beam_workspace_bytes(B, W, V)
-    ws, nbytes = _workspace(workspace, dev, sp, need) if need > 0 else (None, 0)
+    ws = _workspace(workspace, dev, sp, _other_stream(stream, sp, dev.index), need) if need > 0 else None
     _call("mtrtq_beam_select", dev.index, logits.data_ptr(), logits.stride(0) if B * W > 1 else V, scores.data_ptr(), done.data_ptr(), eos,
-          B, W, V, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(), ws, nbytes, sp)
+          B, W, V, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
+          None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel() * ws.element_size(), sp)
     return out
 
 

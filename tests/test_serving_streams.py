@@ -1,0 +1,144 @@
+"""The serving calls on a stream that is not the current one, while the current one is busy
+with work that the call must not wait for: what the calls make for themselves (scratch that
+starts as zeros, results) belongs to the call's stream."""
+import contextlib
+
+import pytest
+import torch
+
+from mini_tensorrt_b200 import matmulq, serving
+from tests.test_serving import BF16, F32, Paged, check_select, make_gen, randn
+
+gpu = pytest.mark.gpu
+
+
+def busy(seconds=0.2):
+    """Work of about that long on the current stream (8192^3 products of some 0.8 ms)."""
+    a = torch.zeros((8192, 8192), dtype=BF16, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(int(seconds / 0.0008)):
+        a @ a
+
+
+def other_stream(raw):
+    s = torch.cuda.Stream()
+    return s, (s.cuda_stream if raw else s)
+
+
+@pytest.fixture
+def fresh(cuda_device):
+    """No kept workspaces, and memory whose next owner finds ones, not zeros."""
+    kept = dict(serving._workspaces)
+    serving._workspaces.clear()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.full((1 << 28,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    yield
+    torch.cuda.synchronize()
+    serving._workspaces.clear()
+    serving._workspaces.update(kept)
+
+
+@gpu
+@pytest.mark.parametrize("raw", [False, True], ids=["stream", "address"])
+@pytest.mark.parametrize("own", [False, True], ids=["kept", "handed_in"])
+@pytest.mark.parametrize("kind", ["f32", "mixed"])
+def test_attention_workspace_is_zeroed_on_the_calls_stream(fresh, raw, own, kind):
+    """A first call and one that needs more, both with cut tiles, which are joined by tickets
+    that have to start at zero."""
+    calls = [Paged([1, 1], [3000, 800], 4, 2, 64, 32, kind, seed=1), Paged([200, 1], [3000, 900], 8, 2, 128, 32, kind, seed=2)]
+    side, stream = other_stream(raw)
+    ws = matmulq.Workspace("cuda") if own else None
+    for s in calls:  # kernels are loaded by their first call
+        s.run(workspace=torch.zeros(1 << 26, dtype=torch.uint8, device="cuda"))
+    for s in calls:
+        out = torch.full(s.q.shape, 9.0, dtype=s.kp.dtype, device="cuda")
+        torch.full((1 << 26,), 255, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        busy()
+        s.run(out=out, workspace=ws, stream=stream)
+        side.synchronize()
+        assert not torch.cuda.current_stream().query(), "the current stream was to be busy for longer"
+        got = out.cpu()  # (waits for the current stream)
+        torch.cuda.synchronize()
+        s.verify(got.cuda())
+
+
+@gpu
+def test_beam_workspace_is_zeroed_on_the_calls_stream(fresh):
+    logits, scores = randn(make_gen(3), 12, 20000), -torch.rand((3, 4), device="cuda")
+    done = torch.zeros((3, 4), dtype=torch.uint8, device="cuda")
+    out = (torch.zeros_like(scores), *(torch.zeros((3, 4), dtype=torch.int32, device="cuda") for _ in range(2)),
+           torch.zeros_like(done))
+    side, stream = other_stream(False)
+    serving.beam_select(logits, scores, done, 7, workspace=torch.zeros(1 << 22, dtype=torch.uint8, device="cuda"))
+    torch.full((1 << 26,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    busy()
+    serving.beam_select(logits, scores, done, 7, out=out, stream=stream)
+    side.synchronize()
+    assert not torch.cuda.current_stream().query()
+    torch.cuda.synchronize()
+    check_select(logits, scores, done, 7, out)
+
+
+@pytest.fixture
+def fake_streams(monkeypatch):
+    """Stream 7 is the current one; notes where each buffer is made, on the CPU."""
+    made, now = [], [7]
+
+    @contextlib.contextmanager
+    def on(stream):
+        before = now[0]
+        now[0] = before if stream is None else stream[1]
+        yield
+        now[0] = before
+
+    class Buffer:
+        def __init__(self, n):
+            self.n, self.recorded = n, []
+
+        def numel(self):
+            return self.n
+
+        def record_stream(self, s):
+            self.recorded.append(s)
+
+    def zeros(n, dtype, device):
+        made.append((now[0], Buffer(n)))
+        return made[-1][1]
+
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: now[0])
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda ptr, device: ("external", ptr))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: now[0], raising=False)
+    monkeypatch.setattr(torch, "zeros", zeros)
+    monkeypatch.setattr(serving, "_workspaces", {})
+    return made
+
+
+def scratch(ptr, nbytes, workspace=None):
+    device = torch.device("cuda", 0)
+    return serving._workspace(workspace, device, ptr, serving._other_stream(ptr, ptr, 0), nbytes)
+
+
+def test_where_kept_workspaces_are_made(fake_streams):
+    made = fake_streams
+    a = scratch(9, 100)
+    assert [at for at, _ in made] == [9]
+    assert scratch(9, 100) is a and scratch(7, 50) is not a and len(made) == 2
+    assert [at for at, _ in made] == [9, 7]
+    b = scratch(9, 200)
+    assert b is not a and [at for at, _ in made] == [9, 7, 9]
+    assert a.recorded == [9]  # not given out again before stream 9 is done with it
+
+
+def test_where_a_workspace_handed_in_grows(fake_streams):
+    made, ws = fake_streams, matmulq.Workspace("cuda")
+    a = scratch(7, 100, ws)
+    assert scratch(9, 100, ws) is a
+    b = scratch(9, 101, ws)
+    assert b is not a and [at for at, _ in made] == [7, 9] and a.recorded == [9]
+    mine = object()
+    assert scratch(9, 10 ** 6, mine) is mine
