@@ -5,6 +5,10 @@ libmtrtq's C ABI (include/mtrtq.h, which defines the formulas).
 The reference decodes one sequence over contiguous caches (KVDecoder,
 tools/run_gpt2.cpp:88-191). Lengths, page numbers and scores are read on the device, so
 every call can be captured in a CUDA graph (with `out` and `workspace` given).
+
+`stream` (a torch stream or a raw stream's address; by default the current one) is where a
+call runs; results and scratch that the call makes come from that stream's memory. That stream
+must have waited for the inputs, and who reads the result elsewhere waits for that stream.
 """
 from __future__ import annotations
 
@@ -48,6 +52,18 @@ def _other_stream(stream, stream_ptr: int, index: int):
     if stream_ptr == torch._C._cuda_getCurrentRawStream(index):
         return None
     return stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream_ptr, device=index)
+
+
+def _made_there(other, device, make):
+    """What make() allocates, from the memory of the call's stream (other, or the current one),
+    and kept from being given out again before the current stream's work with it is done."""
+    if other is None:
+        return make()
+    with torch.cuda.stream(other):
+        made = make()
+    for x in made:
+        x.record_stream(torch.cuda.current_stream(device))
+    return made
 
 
 def _workspace(workspace, device, stream_ptr: int, other, nbytes: int) -> torch.Tensor:
@@ -100,11 +116,12 @@ def _attend(where, q, k, v, out, out_dtype, kv_heads, cu_rows, scale, workspace,
         kp, vp = k.data_ptr(), v.data_ptr()
     else:
         ks, vs, kp, vp = (0, 0), (0, 0), 0, 0
+    sp = _stream_ptr(stream, index)
+    other = _other_stream(stream, sp, index)
     if out is None:
-        out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
+        out, = _made_there(other, device, lambda: (torch.empty_like(
+            q, dtype=out_dtype, memory_format=torch.contiguous_format),))
         os = (H * D, D)
-        if isinstance(stream, torch.cuda.Stream):
-            out.record_stream(stream)
     else:
         os = _rows("out", out, shape, out_dtype, device)
     if cu_rows.dim() != 1:
@@ -114,10 +131,9 @@ def _attend(where, q, k, v, out, out_dtype, kv_heads, cu_rows, scale, workspace,
     a = _pack(q.data_ptr(), kp, vp, out.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], T, batch, H,
               kv_heads, D, _DTYPES[dtype], _DTYPES[out_dtype], D ** -0.5 if scale is None else scale,
               cu_rows.data_ptr(), *pages)
-    sp = _stream_ptr(stream, index)
     need = lib().mtrtq_attention_workspace_bytes(a)
     if need > 0:
-        ws = _workspace(workspace, device, sp, _other_stream(stream, sp, index), need)
+        ws = _workspace(workspace, device, sp, other, need)
         _call(where, index, a, ws.data_ptr(), ws.numel() * ws.element_size(), sp)
     else:  # refused by the call too, with the reason
         _call(where, index, a, None, 0, sp)
@@ -193,20 +209,19 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor, 
     if logits.dim() != 2 or logits.dtype != torch.float32 or logits.shape[0] != B * W or logits.device != dev \
             or logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("logits must be float32 [requests * beams, vocab] with unit stride along vocab")
+    sp = _stream_ptr(stream, dev.index)
+    other = _other_stream(stream, sp, dev.index)
     if out is None:
-        out = (torch.empty_like(scores), torch.empty_like(scores, dtype=torch.int32),
-               torch.empty_like(scores, dtype=torch.int32), torch.empty_like(done))
-        if isinstance(stream, torch.cuda.Stream):
-            for x in out:
-                x.record_stream(stream)
+        out = _made_there(other, dev, lambda: (
+            torch.empty_like(scores), torch.empty_like(scores, dtype=torch.int32),
+            torch.empty_like(scores, dtype=torch.int32), torch.empty_like(done)))
     else:
         for x, t in zip(out, (torch.float32, torch.int32, torch.int32, torch.uint8), strict=True):
             if x.shape != scores.shape or x.dtype != t or x.device != dev or not x.is_contiguous():
                 raise ValueError("out is (float32, int32, int32, uint8), each contiguous [requests, beams]")
     V = logits.shape[1]
-    sp = _stream_ptr(stream, dev.index)
     need = lib().mtrtq_beam_workspace_bytes(B, W, V)
-    ws = _workspace(workspace, dev, sp, _other_stream(stream, sp, dev.index), need) if need > 0 else None
+    ws = _workspace(workspace, dev, sp, other, need) if need > 0 else None
     _call("mtrtq_beam_select", dev.index, logits.data_ptr(), logits.stride(0) if B * W > 1 else V, scores.data_ptr(), done.data_ptr(), eos,
           B, W, V, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
           None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel() * ws.element_size(), sp)

@@ -83,6 +83,68 @@ def test_beam_workspace_is_zeroed_on_the_calls_stream(fresh):
     check_select(logits, scores, done, 7, out)
 
 
+@gpu
+@pytest.mark.parametrize("raw", [False, True], ids=["stream", "address"])
+def test_results_belong_to_the_calls_stream(cuda_device, raw):
+    """Memory that the current stream has been given back, but not yet written for the last
+    time, is not where another stream's result goes."""
+    s = Paged([1] * 4, [300, 40, 2, 77], 8, 2, 64, 32, "f32", seed=4)
+    logits, scores = randn(make_gen(5), 4, 3000), -torch.rand((1, 4), device="cuda")
+    done = torch.zeros((1, 4), dtype=torch.uint8, device="cuda")
+    side, stream = other_stream(raw)
+    s.run(stream=stream), serving.beam_select(logits, scores, done, 7, stream=stream)  # workspaces
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    busy()
+    late = [torch.empty(s.q.shape, dtype=F32, device="cuda"), torch.empty((1, 4), device="cuda"),
+            torch.empty((1, 4), dtype=torch.int32, device="cuda"), torch.empty((1, 4), dtype=torch.int32, device="cuda"),
+            torch.empty((1, 4), dtype=torch.uint8, device="cuda")]
+    for x in late:
+        x.fill_(7)
+    late.clear()
+    del x
+    out = s.run(stream=stream)
+    picked = serving.beam_select(logits, scores, done, 7, stream=stream)
+    side.synchronize()
+    assert not torch.cuda.current_stream().query()
+    torch.cuda.synchronize()
+    s.verify(out)
+    check_select(logits, scores, done, 7, picked)
+
+
+@gpu
+def test_results_outlive_their_readers_on_the_current_stream(cuda_device):
+    """A result that the current stream still has to read is not handed out again by the
+    other stream's memory when its last name goes."""
+    s = Paged([1] * 4, [300, 40, 2, 77], 8, 2, 64, 32, "f32", seed=6)
+    side = torch.cuda.Stream()
+    s.run(stream=side)
+    torch.cuda.synchronize()
+    out = s.run(stream=side)
+    want = out.clone()
+    side.synchronize()
+    torch.cuda.synchronize()
+    busy()
+    read = out.clone()
+    del out
+    with torch.cuda.stream(side):
+        again = [torch.full(s.q.shape, 5.0, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(read, want) and len(again) == 4
+
+
+@gpu
+def test_address_of_the_default_stream(cuda_device):
+    """stream=0 is the default stream, also where another is current."""
+    s = Paged([1] * 4, [300, 40, 2, 77], 8, 2, 64, 32, "f32", seed=7)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = s.run(stream=0)
+    torch.cuda.synchronize()
+    s.verify(out)
+
+
 @pytest.fixture
 def fake_streams(monkeypatch):
     """Stream 7 is the current one; notes where each buffer is made, on the CPU."""
