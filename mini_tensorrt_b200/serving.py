@@ -69,15 +69,20 @@ def _made_there(other, device, make):
 def _workspace(workspace, device, stream_ptr: int, other, nbytes: int) -> torch.Tensor:
     """The caller's workspace (a Workspace, or a tensor), or one kept for each stream: calls
     that share a workspace must be ordered. What is made here is made and zero-filled on the
-    call's stream (other, or the current one)."""
+    call's stream (other, or the current one); while that is being captured it is the graph's
+    (filled by its replays alone), so it is not kept for other calls."""
     if workspace is None:
         key = (device.index, stream_ptr)
         workspace = _workspaces.get(key)
         if workspace is None:
             workspace = _workspaces[key] = Workspace(device)
-    if isinstance(workspace, Workspace):
-        workspace = workspace.get(nbytes, other)
-    return workspace
+    if not isinstance(workspace, Workspace):
+        return workspace
+    if workspace.buf is None or workspace.buf.numel() < nbytes:
+        with torch.cuda.stream(other):
+            if torch.cuda.is_current_stream_capturing():
+                return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return workspace.get(nbytes, other)
 
 
 def _rows(name: str, x: torch.Tensor, shape, dtype, device):

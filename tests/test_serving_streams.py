@@ -145,6 +145,31 @@ def test_address_of_the_default_stream(cuda_device):
     s.verify(out)
 
 
+@gpu
+def test_capture_without_a_workspace(fresh):
+    """A capture that finds no kept workspace, or a small one, makes none that later calls
+    would use: its memory is the graph's, and zeros are there from its first replay on."""
+    small, large = Paged([1, 1], [300, 80], 4, 2, 64, 32, "f32", seed=1), Paged([200, 1], [3000, 900], 8, 2, 128, 32, "f32", seed=2)
+    side = torch.cuda.Stream()
+    for s in (small, large):
+        s.run(workspace=torch.zeros(1 << 26, dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    small.run(stream=side)
+    side.synchronize()
+    kept = {key: ws.buf for key, ws in serving._workspaces.items()}
+    out = torch.zeros(large.q.shape, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        large.run(out=out)
+    assert {key: ws.buf for key, ws in serving._workspaces.items()} == kept
+    large.verify(large.run(stream=side))
+    for _ in range(2):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        large.verify(out)
+
+
 @pytest.fixture
 def fake_streams(monkeypatch):
     """Stream 7 is the current one; notes where each buffer is made, on the CPU."""
@@ -175,6 +200,7 @@ def fake_streams(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: now[0])
     monkeypatch.setattr(torch.cuda, "ExternalStream", lambda ptr, device: ("external", ptr))
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: now[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == 11)
     monkeypatch.setattr(torch, "zeros", zeros)
     monkeypatch.setattr(serving, "_workspaces", {})
     return made
@@ -204,3 +230,19 @@ def test_where_a_workspace_handed_in_grows(fake_streams):
     assert b is not a and [at for at, _ in made] == [7, 9] and a.recorded == [9]
     mine = object()
     assert scratch(9, 10 ** 6, mine) is mine
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_what_a_capture_needs_is_not_kept(fake_streams, own):
+    """Stream 11 is being captured."""
+    made, ws = fake_streams, matmulq.Workspace("cuda") if own else None
+    a = scratch(11, 100, ws)
+    b = scratch(11, 100, ws)
+    assert a is not b and [at for at, _ in made] == [11, 11]
+    assert all(w.buf is None for w in serving._workspaces.values()) and (ws is None or ws.buf is None)
+
+
+def test_a_capture_uses_what_is_there(fake_streams):
+    ws = matmulq.Workspace("cuda")
+    a = scratch(9, 100, ws)
+    assert scratch(11, 100, ws) is a and scratch(11, 101, ws) is not a and ws.buf is a
