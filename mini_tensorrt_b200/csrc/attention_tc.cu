@@ -433,9 +433,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (live && half == 0 && !whole) __stcg(p.part_ml + part * p.part_rows + prow, make_float2(m, l));
         // The infinities and NaN that were taken out of the last blocks' V, for the rows
-        // that see them. A slot without blocks here has not waited for the check, and
-        // sees none of it.
-        if (cnt > 0 && (s.k0 + s.n) * kBlock > s.all_see()) {
+        // that see them. A slot without such blocks has not waited for the check (and sees
+        // none of it): with a token a slot that is slot 0's case even where it has others.
+        if (cnt > 0 && (s.k0 + (pair ? cnt : s.n)) * kBlock > s.all_see()) {
           const int have = min(kBadMax, bad_count[seg % kRing]);
 #pragma unroll 1
           for (int x = 0; x < have; ++x) {
