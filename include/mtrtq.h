@@ -587,7 +587,7 @@ int mtrtq_paged_attention(const mtrtq_attention_args* a, void* workspace, size_t
  * token, out_scores, out_done [requests, beams]. NaN logits count as -infinity, so do
  * candidates whose score is NaN; a beam not in use has the score -infinity. eos may be
  * -1 (none ends; done must then be 0). outputs must not overlap inputs.
- * beams * vocab is below 2^31. The greedy step is mtrtq_argmax_rows
+ * beams * vocab is at most 2^31 - 2^14. The greedy step is mtrtq_argmax_rows
  * (tools/run_gpt2.cpp:42-47). */
 #define MTRTQ_MAX_BEAMS 32
 int64_t mtrtq_beam_workspace_bytes(int64_t requests, int64_t beams, int64_t vocab);

@@ -453,8 +453,11 @@ int check_beams(int64_t requests, int64_t beams) {
 
 int check_select(int64_t requests, int64_t beams, int64_t vocab) {
   if (int rc = check_beams(requests, beams)) return rc;
-  if (vocab < 1 || vocab * beams > 2147483647 || vocab > 2147483647)
-    return report_error(MTRTQ_ERR_INVALID_ARG, "vocab (%lld) times beams is 1 to 2^31 - 1", (long long)vocab);
+  // (32-bit places of a row, up to a block and a few past its end)
+  constexpr int64_t most = (int64_t(1) << 31) - 2 * (2 * kChunk);
+  if (vocab < 1 || vocab > most || vocab * beams > most)
+    return report_error(MTRTQ_ERR_INVALID_ARG, "vocab (%lld) times beams is 1 to %lld", (long long)vocab,
+                        (long long)most);
   return MTRTQ_OK;
 }
 

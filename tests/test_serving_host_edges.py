@@ -23,3 +23,12 @@ def test_prompt_call_with_a_whole_cache_refused(over):
     assert _lib.lib().mtrtq_attention_workspace_bytes(ctypes.byref(a)) > 0  # of the paged call
     assert _lib.lib().mtrtq_prompt_attention(ctypes.byref(a), A, 1 << 40, None) == _lib.ERR_INVALID_ARG
     assert "NULL" in _lib.last_error()
+
+
+def test_beam_vocabulary_near_2_31_refused():
+    """Places in a row are counted in 32 bits, a block's beyond its end included."""
+    lib, most = _lib.lib(), 2 ** 31 - 2 ** 14
+    for beams, vocab in ((1, most + 1), (1, 2 ** 31 - 1), (2, most // 2 + 1), (32, most // 32 + 1)):
+        assert lib.mtrtq_beam_workspace_bytes(1, beams, vocab) == -1
+        assert lib.mtrtq_beam_select(A, vocab, A, A, -1, 1, beams, vocab, A, A, A, A, A, 1 << 40, None) == _lib.ERR_INVALID_ARG
+    assert lib.mtrtq_beam_workspace_bytes(1, 1, most) > 0 and lib.mtrtq_beam_workspace_bytes(1, 32, most // 32) > 0
