@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from . import serving
-from ._lib import check, lib
+from ._lib import MAX_BATCH, MAX_BEAMS, check, lib
 from .gpt2 import GPT2Weights
 from .matmulq import PackedWeight, Workspace, matmul_q8
 
@@ -130,6 +130,12 @@ class PagedDecoder:
         lens, _, _, _, i32 = self._packed(prompts)
         if max_new < 1 or max(lens) + max_new - 1 > self.cfg.n_pos:
             raise ValueError(f"a prompt and its new tokens exceed the {self.cfg.n_pos} positions")
+        if not 1 <= beams <= MAX_BEAMS or len(prompts) * beams > MAX_BATCH:
+            raise ValueError(f"beams is 1 to {MAX_BEAMS}, and {MAX_BATCH} at most over all prompts")
+        if not -1 <= eos < self.cfg.vocab:
+            raise ValueError("eos is -1 or a token of the vocabulary")
+        if chunk is not None and chunk < 1:
+            raise ValueError("chunk is at least 1")
         cfg, B, W = self.cfg, len(prompts), beams
         table, owned, count = assign_pages(lens, W, max_new, self.page_size)
         table, owned = i32(table), i32(owned)
@@ -140,7 +146,7 @@ class PagedDecoder:
 
         # The prompts, through the first beams' tables.
         first = table[::W]
-        step = chunk or max(lens)
+        step = max(lens) if chunk is None else chunk
         for begin in range(0, max(lens), step):
             parts = [np.asarray(p, np.int64)[begin:begin + step] for p in prompts]
             ends = [min(begin + step, n) for n in lens]
