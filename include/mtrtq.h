@@ -534,7 +534,8 @@ int mtrtq_decode_next(unsigned long long* best, int64_t rows, int32_t* tok, int3
  * Strides are in elements: row r, head h, dimension d is at r * row + h * head + d.
  * head_dim is a multiple of 8 up to 128, heads / kv_heads is whole and at most 128,
  * batch is at most 1024; pointers are 16-byte aligned and strides multiples of 16
- * bytes (else MTRTQ_ERR_ALIGNMENT); scale is positive and finite.
+ * bytes (else MTRTQ_ERR_ALIGNMENT); rows and heads of out do not overlap; scale is
+ * positive and finite.
  *
  * Paged cache: page n holds page_size (16, 32, 64 or 128) tokens of every key/value
  * head, [kv_heads, page_size, head_dim] contiguous, page_stride elements after page

@@ -139,11 +139,11 @@ int check_args(const Args* a, bool paged) {
   const int64_t strides[8] = {a->q_row, a->q_head, a->k_row, a->k_head, a->v_row, a->v_head, a->out_row, a->out_head};
   for (int64_t s : strides)
     if (s < 0 || s >= (int64_t(1) << 36)) return report_error(MTRTQ_ERR_INVALID_ARG, "a stride is out of range");
-  if (a->out_row == 0 && a->rows > 1)
-    return report_error(MTRTQ_ERR_INVALID_ARG, "the rows of out must not overlap");
   if (!on16(a->q, a->q_row, a->q_head, xs) || (a->k && !on16(a->k, a->k_row, a->k_head, xs)) ||
       (a->v && !on16(a->v, a->v_row, a->v_head, xs)) || !on16(a->out, a->out_row, a->out_head, cs))
     return report_error(MTRTQ_ERR_ALIGNMENT, "q, k, v and out must be 16-byte aligned with strides of whole 16 bytes");
+  if ((a->rows > 1 && a->out_row < a->head_dim) || (a->rows > 0 && a->heads > 1 && a->out_head < a->head_dim))
+    return report_error(MTRTQ_ERR_INVALID_ARG, "the rows and heads of out must not overlap");
   if (!paged) {
     // (the layouts and the workspace query tell the calls apart by k_pages)
     if (a->k_pages || a->v_pages || a->table || a->kv_len)

@@ -32,3 +32,19 @@ def test_beam_vocabulary_near_2_31_refused():
         assert lib.mtrtq_beam_workspace_bytes(1, beams, vocab) == -1
         assert lib.mtrtq_beam_select(A, vocab, A, A, -1, 1, beams, vocab, A, A, A, A, A, 1 << 40, None) == _lib.ERR_INVALID_ARG
     assert lib.mtrtq_beam_workspace_bytes(1, 1, most) > 0 and lib.mtrtq_beam_workspace_bytes(1, 32, most // 32) > 0
+
+
+@pytest.mark.parametrize("over", [{"out_head": 0}, {"out_head": 8}, {"out_row": 8}, {"out_head": 0, "dtype": _lib.DTYPE_BF16}])
+def test_heads_or_rows_of_out_that_overlap_refused(over):
+    """Heads of 16 dimensions that start 8 apart, or at the same place, would be written by
+    several blocks in no order."""
+    for make, fn in ((prompt, _lib.lib().mtrtq_prompt_attention), (paged, _lib.lib().mtrtq_paged_attention)):
+        assert fn(ctypes.byref(make(**over)), None, 0, None) == _lib.ERR_INVALID_ARG
+        assert "overlap" in _lib.last_error()
+
+
+def test_strides_of_a_single_row_or_head_of_out_say_nothing():
+    one = {"rows": 1, "batch": 1, "heads": 1, "kv_heads": 1}
+    for over in ({"out_row": 0}, {"out_head": 0}, {"out_row": 0, "out_head": 0}):
+        a = prompt(**one, **over)
+        assert _lib.lib().mtrtq_attention_workspace_bytes(ctypes.byref(a)) > 0
