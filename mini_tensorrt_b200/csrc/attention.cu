@@ -327,19 +327,21 @@ F32Layout f32_layout(const Args& a, int sm_count) {
   F32Layout l;
   const int group = a.heads / a.kv_heads, dp = a.head_dim <= 64 ? 64 : 128;
   const int64_t each = a.rows * group / a.batch;  // rows of a request's tiles, on average
-  if (each <= 8 && group <= 8)
-    l.tile_rows = each <= 1 && group == 1 ? 1 : each <= 2 && group <= 2 ? 2 : each <= 4 && group <= 4 ? 4 : 8;
-  else
-    l.tile_rows = each <= 16 && group <= 16 ? 16 : each <= 256 && group <= 64 ? 64 : 128;
-  const int ctas = l.tile_rows <= 2 || l.tile_rows == 16 || (dp == 64 && l.tile_rows > 8) ? 2 : 1;
-  l.grid = sm_count * ctas < 1024 ? sm_count * ctas : 1024;
-  l.off_ml = 4096;
-  l.off_part = l.off_ml + round256((size_t)l.grid * 2 * l.tile_rows * sizeof(float2));
-  l.total = l.off_part + (size_t)l.grid * 2 * l.tile_rows * dp * sizeof(float);
   // Prompts from some 100 rows a request on, where the split pays (B200, 12 heads of 64: 4
   // requests of 64 tokens 23 us against 21 on the CUDA cores, of 130 27 against 38, 8 of 300
   // 52 against 97).
   l.tc = !a.k_pages && a.head_dim <= 64 && each >= 96;
+  if (l.tc)
+    l.tile_rows = 128;
+  else if (each <= 8 && group <= 8)
+    l.tile_rows = each <= 1 && group == 1 ? 1 : each <= 2 && group <= 2 ? 2 : each <= 4 && group <= 4 ? 4 : 8;
+  else
+    l.tile_rows = each <= 16 && group <= 16 ? 16 : each <= 256 && group <= 64 ? 64 : 128;
+  const int ctas = l.tc ? 1 : l.tile_rows <= 2 || l.tile_rows == 16 || (dp == 64 && l.tile_rows > 8) ? 2 : 1;
+  l.grid = sm_count * ctas < 1024 ? sm_count * ctas : 1024;
+  l.off_ml = 4096;
+  l.off_part = l.off_ml + round256((size_t)l.grid * 2 * l.tile_rows * sizeof(float2));
+  l.total = l.off_part + (size_t)l.grid * 2 * l.tile_rows * dp * sizeof(float);
   l.off_flags = round256(l.total);
   l.off_planes = l.off_flags + round256((size_t)((a.rows + kSplitRows - 1) / kSplitRows) * sizeof(int));
   if (l.tc) l.total = l.off_planes + (size_t)3 * a.rows * (a.heads + 2 * a.kv_heads) * a.head_dim * 2;
@@ -401,9 +403,6 @@ int launch_f32(const Args& a, bool paged, void* workspace, unsigned* status, cud
     int* flags = reinterpret_cast<int*>(ws + l.off_flags);
     F32TcAttention x = {};
     static_cast<F32Attention&>(x) = p;
-    x.tile_tokens = 128 / p.group;
-    x.tile_rows = 128;
-    x.min_steps = 2;
     x.pair_cost = 2;
     x.flags = flags;
     x.status = status;
@@ -418,8 +417,7 @@ int launch_f32(const Args& a, bool paged, void* workspace, unsigned* status, cud
     if (int rc = make_map(&km, planes + (int64_t)a.heads * a.head_dim, 3, dims, strides, box)) return rc;
     if (int rc = make_map(&vm, planes + (int64_t)(a.heads + a.kv_heads) * a.head_dim, 3, dims, strides, box)) return rc;
     if (int rc = cuda_status(launch_split_rows(p, a.heads, planes, flags, st), "attention rows launch")) return rc;
-    const int sms = sm_count();
-    return cuda_status(launch_attention_f32_tc(x, qm, km, vm, sms < 1024 ? sms : 1024, st), "attention launch");
+    return cuda_status(launch_attention_f32_tc(x, qm, km, vm, l.grid, st), "attention launch");
   }
   return cuda_status(launch_attention_f32(p, l.grid, before, st), "attention launch");
 }
