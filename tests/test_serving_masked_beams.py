@@ -12,7 +12,7 @@ from tests.test_serving import F32, INF, make_gen, randn
 pytestmark = pytest.mark.gpu
 
 LOWEST = torch.finfo(F32).min
-MASKS = (-INF,)
+MASKS = (-INF, LOWEST)
 SIZES = [(1, 1, 5), (1, 4, 50257), (3, 8, 50257), (2, 16, 4097), (1, 32, 33), (40, 4, 9000), (2, 32, 20000), (1, 3, 1)]
 
 
