@@ -144,22 +144,23 @@ class PagedDecoder:
         vp = torch.empty_like(kp)
         logits = torch.empty((B * W, cfg.vocab), dtype=torch.float32, device=self.dev)
 
-        # The prompts, through the first beams' tables.
-        first = table[::W]
+        # The prompts, through the first beams' tables. (A prompt that is done is left out of
+        # the pass: the attention's kernel goes by the rows that a request has on average.)
         step = max(lens) if chunk is None else chunk
         for begin in range(0, max(lens), step):
-            parts = [np.asarray(p, np.int64)[begin:begin + step] for p in prompts]
-            ends = [min(begin + step, n) for n in lens]
-            cu, kv_len = i32([0, *itertools.accumulate(len(p) for p in parts)]), i32(ends)
+            live = [b for b, n in enumerate(lens) if n > begin]
+            parts = [np.asarray(prompts[b], np.int64)[begin:begin + step] for b in live]
+            upto = list(itertools.accumulate(len(p) for p in parts))
+            cu, kv_len, first = i32([0, *upto]), i32([begin + len(p) for p in parts]), table[i32(live).long() * W]
             ids = torch.from_numpy(np.concatenate(parts)).to(self.dev)
             at = torch.from_numpy(np.concatenate([np.arange(begin, begin + len(p)) for p in parts])).to(self.dev)
             attend = lambda i, q, k, v: serving.paged_attention(q, k, v, kp[i], vp[i], first, kv_len, cu,
                                                                 workspace=self.attn_ws)
             x = self._pass(ids, at, attend)
-            done = [b for b, n in enumerate(lens) if begin < n <= begin + step]  # their last position is in x
+            done = {b: upto[i] - 1 for i, b in enumerate(live) if lens[b] <= begin + step}  # last position, a row of x
             if done:
-                last = torch.tensor([int(sum(len(q) for q in parts[:b + 1])) - 1 for b in done], device=self.dev)
-                logits[torch.tensor(done, device=self.dev) * W] = self._logits(x[last])
+                rows = torch.tensor(list(done.values()), device=self.dev)
+                logits[torch.tensor(list(done), device=self.dev) * W] = self._logits(x[rows])
 
         # The beams: only the first is in use, with a score of 0.
         scores = torch.full((B, W), float("-inf"), device=self.dev)
