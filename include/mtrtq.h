@@ -524,9 +524,12 @@ int mtrtq_decode_next(unsigned long long* best, int64_t rows, int32_t* tok, int3
  * of either factor, to fp32's precision, on the tensor cores; there an infinite q or k
  * counts as NaN). dtype bf16 (x_dtype f32 or bf16): k and v are rounded to
  * bf16 as they are stored, q and the weights p are rounded to bf16 for the tensor
- * cores' products (neither is in a paged call whose requests have a row or two for
- * a key/value head on average), the maximum, the sum and the output are held in
- * fp32 and out is rounded once. x_dtype bf16 with dtype f32 is refused.
+ * cores' products, the maximum, the sum and the output are held in
+ * fp32 and out is rounded once. Where the requests of a paged call have no more than two rows
+ * (tokens times heads / kv_heads) on average, those of up to 16 tokens are computed from
+ * unrounded q and p: the same request can so differ by these two roundings (some 2^-9 of its
+ * largest v) between calls that have other requests in them. x_dtype bf16 with dtype f32 is
+ * refused.
  *
  * The packed rows are given by cu_rows: request b owns rows cu_rows[b] ..
  * cu_rows[b+1] - 1 of q, k, v and out (non-decreasing; a request may own none; values

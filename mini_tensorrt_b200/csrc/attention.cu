@@ -1,5 +1,6 @@
 // Attention of packed rows: over whole prompts, and of new tokens over a paged
 // key/value cache (include/mtrtq.h, mtrtq_prompt_attention and mtrtq_paged_attention).
+#include <limits.h>
 #include <math.h>
 
 #include "../../include/mtrtq.h"
@@ -11,7 +12,6 @@ namespace mtrtq {
 int report_error(int code, const char* fmt, ...);
 int report_cuda_error(cudaError_t e, const char* what);
 unsigned* device_status_address(int* rc);
-bool overlap_launch_enabled();
 
 namespace {
 
@@ -240,26 +240,35 @@ void fill_list(const Args& a, bool paged, AttentionList& p) {
   p.group = a.heads / a.kv_heads;
   p.head_dim = a.head_dim;
   p.page_size = a.page_size;
+  p.least = 1;
+  p.most = INT_MAX;
   p.max_keys = a.table_width * a.page_size;
 }
 
-int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cudaStream_t st) {
-  const TcLayout l = tc_layout(a, sm_count());
+// Stores the new tokens' k and v in the pages, and writes q (whole prompts: q, k and v) in
+// bf16 to rows if not null.
+int launch_new_rows(const Args& a, bool paged, __nv_bfloat16* rows, cudaStream_t st) {
+  const unsigned grid = (unsigned)a.rows;
+  const bool x16 = a.x_dtype != MTRTQ_DTYPE_F32;
+  if (!paged) {
+    if (x16) cast_kernel<__nv_bfloat16><<<grid, kRowThreads, 0, st>>>(a, rows);
+    else cast_kernel<float><<<grid, kRowThreads, 0, st>>>(a, rows);
+  } else if (a.dtype == MTRTQ_DTYPE_F32) {
+    append_kernel<float, float><<<grid, kRowThreads, 0, st>>>(a, nullptr);
+  } else if (x16) {
+    append_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, kRowThreads, 0, st>>>(a, rows);
+  } else {
+    append_kernel<float, __nv_bfloat16><<<grid, kRowThreads, 0, st>>>(a, rows);
+  }
+  return cuda_status(cudaGetLastError(), "attention rows launch");
+}
+
+// For requests of `least` tokens and more; after: it follows another kernel of the call.
+int launch_tc(const Args& a, bool paged, const TcLayout& l, int least, bool after, void* workspace, unsigned* status,
+              cudaStream_t st) {
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   __nv_bfloat16* rows = reinterpret_cast<__nv_bfloat16*>(ws + l.off_rows);
   Args x = a;
-  const bool before = l.cast || (paged && a.k);
-  if (before) {
-    if (!paged) {
-      if (a.x_dtype == MTRTQ_DTYPE_F32) cast_kernel<float><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, rows);
-      else cast_kernel<__nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, rows);
-    } else if (a.x_dtype == MTRTQ_DTYPE_F32) {
-      append_kernel<float, __nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, l.cast ? rows : nullptr);
-    } else {
-      append_kernel<__nv_bfloat16, __nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, l.cast ? rows : nullptr);
-    }
-    if (int rc = cuda_status(cudaGetLastError(), "attention rows launch")) return rc;
-  }
   if (l.cast) {
     const int64_t row = (int64_t)(a.heads + (paged ? 0 : 2 * a.kv_heads)) * a.head_dim;
     x.q = rows;
@@ -293,6 +302,7 @@ int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cuda
   }
   TcAttention p = {};
   fill_list(a, paged, p);
+  p.least = least;
   p.slot_tokens = l.slot_tokens;
   p.tile_tokens = 2 * l.slot_tokens;
   p.min_steps = 4;
@@ -311,7 +321,7 @@ int launch_tc(const Args& a, bool paged, void* workspace, unsigned* status, cuda
   p.part_ml = reinterpret_cast<float2*>(ws + l.off_ml);
   p.part_rows = l.part_rows;
   p.status = status;
-  return cuda_status(launch_attention_tc(p, qm, km, vm, l.grid, before, st), "attention launch");
+  return cuda_status(launch_attention_tc(p, qm, km, vm, l.grid, after, st), "attention launch");
 }
 
 // The f32 path: tickets | partials of cut tiles. Tiles of up to 8 rows where requests have
@@ -323,15 +333,17 @@ struct F32Layout {
   size_t off_ml, off_part, off_flags, off_planes, total;
 };
 
-F32Layout f32_layout(const Args& a, int sm_count) {
+F32Layout f32_layout(const Args& a, int sm_count, bool many = false) {
   F32Layout l;
   const int group = a.heads / a.kv_heads, dp = a.head_dim <= 64 ? 64 : 128;
   const int64_t each = a.rows * group / a.batch;  // rows of a request's tiles, on average
   // Prompts from some 100 rows a request on, where the split pays (B200, 12 heads of 64: 4
   // requests of 64 tokens 23 us against 21 on the CUDA cores, of 130 27 against 38, 8 of 300
   // 52 against 97).
-  l.tc = !a.k_pages && a.head_dim <= 64 && each >= 96;
-  if (l.tc)
+  l.tc = !many && !a.k_pages && a.head_dim <= 64 && each >= 96;
+  if (many)
+    l.tile_rows = 64;
+  else if (l.tc)
     l.tile_rows = 128;
   else if (each <= 8 && group <= 8)
     l.tile_rows = each <= 1 && group == 1 ? 1 : each <= 2 && group <= 2 ? 2 : each <= 4 && group <= 4 ? 4 : 8;
@@ -348,31 +360,61 @@ F32Layout f32_layout(const Args& a, int sm_count) {
   return l;
 }
 
-// Calls with a bf16 cache that go that way too: tiles of a row or two, for which the tensor
-// cores' 128 are mostly empty. On a B200, there and here: 16 requests of 20 to 1024 tokens, 12
-// heads of 64, 34 us and 26; 64 of 2000 146 and 101; 16 of 700, 16 heads of 128, 63 and 38, 16
-// over 8 44 and 29, 64 of 2000 152 and 148. Groups of four and more gain or lose with the
-// lengths, which the host does not know (4 requests of 300, 32 heads over 8, 29 and 20; 64 of 100
-// to 8192 157 and 262), and stay.
-bool few_rows16(const Args& a) {
-  if (a.dtype == MTRTQ_DTYPE_F32 || !a.k_pages) return false;
-  const F32Layout l = f32_layout(a, sm_count());
-  return l.tile_rows <= 2;
+// Which kernels a call takes, and its workspace. The kernel of few rows (tiles of up to 8) is
+// chosen by the rows that requests have on average, which is all that the host knows.
+//
+// With a bf16 cache it takes tiles of a row or two, for which the tensor cores' 128 are mostly
+// empty. On a B200, there and here: 16 requests of 20 to 1024 tokens, 12 heads of 64, 32.0 us and
+// 15.7; 64 of 2000 141 and 91; 16 of 700, 16 heads of 128, 61 and 28, 16 over 8 25.5 and 22.5,
+// 64 of 2000 149 and 136. Groups of four and more gain or lose with the lengths, which the host
+// does not know (4 requests of 300, 32 heads over 8, 29 and 20; 64 of 100 to 8192 157 and 262),
+// and stay.
+//
+// Single requests may have many rows all the same (a chunk of a prompt beside tokens that are
+// decoded, or beside requests that wait), and their keys are read again for every tile. So
+// where one can have more tokens than kFewTokens, such requests go to a second kernel, the
+// tensor cores' or that of 64 rows; it takes up to 1 us (f32: 0.5) to find that there are none. On a
+// B200, 12 heads of 64, with and without it, bf16 cache (f32): 511 requests that wait and a chunk of
+// 512 over 8192 67 us and 2136 (430 and 2316), 31 and 32 over 8000 45 and 146, 63 and 64 over
+// 1000 27 and 50, 63 that decode and 64 over 1000 78 and 90, 63 and 512 (231 and 297). A few
+// tokens cost less where the others are: 31 that decode and 32 over 1000 54.7 and 52.8 (79 and
+// 61), 63 that wait and 33 (43 and 34).
+constexpr int kFewTokens16 = 16, kFewTokens32 = 64;
+struct Plan {
+  bool few, both;
+  F32Layout f32, many;
+  TcLayout tc;
+  size_t off_few;  // of the few rows' parts, beside the tensor cores'
+  size_t total;
+};
+
+Plan plan_call(const Args& a) {
+  Plan p = {};
+  const int sms = sm_count();
+  const bool f32 = a.dtype == MTRTQ_DTYPE_F32;
+  if (f32 || a.k_pages) p.f32 = f32_layout(a, sms);
+  p.few = f32 ? p.f32.tile_rows <= 8 : a.k_pages && p.f32.tile_rows <= 2;
+  p.both = p.few && a.batch > 1 && a.rows > (f32 ? kFewTokens32 : kFewTokens16);
+  if (f32) {
+    if (p.both) p.many = f32_layout(a, sms, true);
+    p.total = p.f32.total > p.many.total ? p.f32.total : p.many.total;
+    return p;
+  }
+  if (!p.few || p.both) p.tc = tc_layout(a, sms);
+  p.off_few = round256(p.tc.total);
+  p.total = p.few ? p.off_few + p.f32.total : p.tc.total;
+  return p;
 }
 
-int launch_f32(const Args& a, bool paged, void* workspace, unsigned* status, cudaStream_t st) {
-  const F32Layout l = f32_layout(a, sm_count());
+// For requests of least .. most tokens; after: it follows another kernel of the call. parts:
+// where l's offsets count from.
+int launch_f32(const Args& a, bool paged, const F32Layout& l, int least, int most, bool after, void* workspace,
+               uint8_t* parts, unsigned* status, cudaStream_t st) {
   const bool pages16 = a.dtype != MTRTQ_DTYPE_F32, q16 = a.x_dtype != MTRTQ_DTYPE_F32;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const bool before = paged && a.k;
-  if (before) {
-    if (!pages16) append_kernel<float, float><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, nullptr);
-    else if (!q16) append_kernel<float, __nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, nullptr);
-    else append_kernel<__nv_bfloat16, __nv_bfloat16><<<(unsigned)a.rows, kRowThreads, 0, st>>>(a, nullptr);
-    if (int rc = cuda_status(cudaGetLastError(), "attention rows launch")) return rc;
-  }
   F32Attention p = {};
   fill_list(a, paged, p);
+  p.least = least;
+  p.most = most;
   p.slot_tokens = 0;
   p.tile_tokens = l.tile_rows / p.group;
   p.min_steps = 2;
@@ -393,14 +435,14 @@ int launch_f32(const Args& a, bool paged, void* workspace, unsigned* status, cud
   p.out = static_cast<float*>(a.out);
   p.out_row = a.out_row;
   p.out_head = a.out_head;
-  p.counters = reinterpret_cast<unsigned*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(ws + l.off_ml);
-  p.partials = reinterpret_cast<float*>(ws + l.off_part);
+  p.counters = static_cast<unsigned*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(parts + l.off_ml);
+  p.partials = reinterpret_cast<float*>(parts + l.off_part);
   p.tile_rows = l.tile_rows;
   if (l.tc) {
     const int all = a.heads + 2 * a.kv_heads;
-    __nv_bfloat16* planes = reinterpret_cast<__nv_bfloat16*>(ws + l.off_planes);
-    int* flags = reinterpret_cast<int*>(ws + l.off_flags);
+    __nv_bfloat16* planes = reinterpret_cast<__nv_bfloat16*>(parts + l.off_planes);
+    int* flags = reinterpret_cast<int*>(parts + l.off_flags);
     F32TcAttention x = {};
     static_cast<F32Attention&>(x) = p;
     x.pair_cost = 2;
@@ -419,7 +461,7 @@ int launch_f32(const Args& a, bool paged, void* workspace, unsigned* status, cud
     if (int rc = cuda_status(launch_split_rows(p, a.heads, planes, flags, st), "attention rows launch")) return rc;
     return cuda_status(launch_attention_f32_tc(x, qm, km, vm, l.grid, st), "attention launch");
   }
-  return cuda_status(launch_attention_f32(p, l.grid, before, st), "attention launch");
+  return cuda_status(launch_attention_f32(p, l.grid, after, st), "attention launch");
 }
 
 int attention(const Args* a, bool paged, void* workspace, size_t workspace_bytes, void* stream) {
@@ -434,8 +476,23 @@ int attention(const Args* a, bool paged, void* workspace, size_t workspace_bytes
   if (reinterpret_cast<uintptr_t>(workspace) % 256)
     return report_error(MTRTQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == MTRTQ_DTYPE_F32 || few_rows16(*a)) return launch_f32(*a, paged, workspace, status, st);
-  return launch_tc(*a, paged, workspace, status, st);
+  const Plan p = plan_call(*a);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  __nv_bfloat16* rows = p.tc.cast ? reinterpret_cast<__nv_bfloat16*>(ws + p.tc.off_rows) : nullptr;
+  const bool before = rows || (paged && a->k);
+  if (before)
+    if ((rc = launch_new_rows(*a, paged, rows, st))) return rc;
+  if (a->dtype == MTRTQ_DTYPE_F32) {
+    rc = launch_f32(*a, paged, p.f32, 1, p.both ? kFewTokens32 : INT_MAX, before, ws, ws, status, st);
+    if (rc == MTRTQ_OK && p.both)
+      rc = launch_f32(*a, paged, p.many, kFewTokens32 + 1, INT_MAX, true, ws, ws, status, st);
+    return rc;
+  }
+  if (p.few) {
+    rc = launch_f32(*a, paged, p.f32, 1, p.both ? kFewTokens16 : INT_MAX, before, ws, ws + p.off_few, status, st);
+    if (rc != MTRTQ_OK || !p.both) return rc;
+  }
+  return launch_tc(*a, paged, p.tc, p.both ? kFewTokens16 + 1 : 1, before || p.both, ws, status, st);
 }
 
 }  // namespace
@@ -447,7 +504,7 @@ extern "C" {
 
 int64_t mtrtq_attention_workspace_bytes(const mtrtq_attention_args* a) {
   if (check_args(a, a && a->k_pages)) return -1;
-  return (int64_t)(a->dtype == MTRTQ_DTYPE_F32 || few_rows16(*a) ? f32_layout(*a, sm_count()).total : tc_layout(*a, sm_count()).total);
+  return (int64_t)plan_call(*a).total;
 }
 
 int mtrtq_prompt_attention(const mtrtq_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {

@@ -19,6 +19,7 @@ struct AttentionList {
   int batch, kv_heads, group, head_dim, page_size;
   int slot_tokens;    // tensor cores: 128 / group, the tokens in a slot's 128 rows
   int tile_tokens;
+  int least, most;    // tokens of the requests that this launch takes
   int64_t max_keys;   // paged: tokens the table's columns hold
   int64_t min_steps;  // fewest steps worth a CTA
   int tile_cost, pair_cost;  // steps that a tile takes besides its own, in one slot's rows or more

@@ -12,6 +12,7 @@
 //
 // V rows past the request's keys are read as zeros; where a block not seen whole by every
 // row holds an infinity or a NaN, its products are formed only for the rows that see them.
+#include <limits.h>
 #include <math.h>
 
 #include "../../include/mtrtq.h"
@@ -59,6 +60,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
   __shared__ unsigned ticket;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, lane = tid & 31, warp = tid >> 5;
 
+  if (nothing_here<kThreads>(p)) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (the stream goes on when this kernel ends)
+    return;
+  }
   Walk walk;
   make_list<kKeys, kThreads>(p, list, walk, &shared_walk);
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -370,6 +375,7 @@ __global__ void __launch_bounds__(kThreads, Few<HD, R, T>::CTAS)
   const int mine = tid / LANES;                // and its first key of a block
   const bool in0 = d0 < p.head_dim;            // (head_dim is a multiple of 8)
 
+  if (p.most != INT_MAX) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the call's second kernel
   Walk walk;
   make_list<F::BLOCK, kThreads>(p, list, walk, &shared_walk);
   asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -56,6 +56,7 @@ __device__ __forceinline__ Request load_request(const AttentionList& p, int b) {
   q.m = min(max(hi, q.r0), rows) - q.r0;
   q.ctx = p.table ? max(n, -(1 << 30)) - q.m : 0;
   q.keys = p.table ? min(max(n, 0), (int)p.max_keys) : q.m;
+  if (q.m < p.least || q.m > p.most) q.m = 0;  // another launch's
   return q;
 }
 
@@ -145,6 +146,16 @@ __device__ bool next_segment(const AttentionList& p, const StepList list, Walk& 
     return true;
   }
   return false;
+}
+
+// Whether the second kernel of a call (attention.cu) finds no request of its own, as is usual:
+// it then leaves before it sets anything up. All threads.
+template <int THREADS>
+__device__ __forceinline__ bool nothing_here(const AttentionList& p) {
+  if (p.least <= 1) return false;
+  bool any = false;
+  for (int b = threadIdx.x; b < p.batch; b += THREADS) any |= load_request(p, b).m > 0;
+  return !__syncthreads_or(any);
 }
 
 // Fills the list and this CTA's walk, which every thread gets, through `shared`. All threads.

@@ -177,6 +177,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   Segment* segments = reinterpret_cast<Segment*>(smem + C::OFF_SEG);
 
+  if (nothing_here<kThreads>(p)) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (the stream goes on when this kernel ends)
+    return;
+  }
+
   if (tid == 0) {
     for (int x = 0; x < C::STAGES; ++x) {
       mbar_init(&full[x], 1);
