@@ -523,11 +523,11 @@ int mtrtq_decode_next(unsigned long long* best, int64_t rows, int32_t* tok, int3
  * throughout (long prompts of up to 64 dimensions form each product from three bf16 parts
  * of either factor, to fp32's precision, on the tensor cores; there an infinite q or k
  * counts as NaN). dtype bf16 (x_dtype f32 or bf16): k and v are rounded to
- * bf16 as they are stored, q and the weights p are rounded to bf16 for the tensor
- * cores' products, the maximum, the sum and the output are held in
+ * bf16 as they are stored, for the tensor cores' products the weights p are rounded to bf16 and
+ * q, where it is f32, to 16 bits; the maximum, the sum and the output are held in
  * fp32 and out is rounded once. Where the requests of a paged call have no more than two rows
  * (tokens times heads / kv_heads) on average, those of up to 16 tokens are computed from
- * unrounded q and p: the same request can so differ by these two roundings (some 2^-9 of its
+ * unrounded q and p: the same request can so differ by these roundings (some 2^-9 of its
  * largest v) between calls that have other requests in them. x_dtype bf16 with dtype f32 is
  * refused.
  *

@@ -63,20 +63,43 @@ __device__ __forceinline__ void store4(__nv_bfloat16* dst, float4 x) {
       make_uint2(reinterpret_cast<const uint32_t&>(lo), reinterpret_cast<const uint32_t&>(hi));
 }
 
+// Four elements of q in the tensor cores' types: rounded to dst's type, or (f32 rows) as two
+// bf16 planes, `plane` elements apart, of 16 bits together. The first is cut toward zero and the
+// second is never zero where q is not, so that both have q's sign: their products with an
+// infinite k are then both the infinity that q's is, and a zero q times it NaN in both.
+template <typename TX>
+__device__ __forceinline__ void store_q(__nv_bfloat16* dst, int64_t plane, float4 x) {
+  if (sizeof(TX) == 2) {
+    store4(dst, x);
+    return;
+  }
+  const float v[4] = {x.x, x.y, x.z, x.w};
+  float a[4], b[4];
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    a[y] = v[y] == v[y] ? __uint_as_float(__float_as_uint(v[y]) & 0xffff0000u) : v[y];
+    b[y] = __bfloat162float(__float2bfloat16_rn(v[y] - a[y]));
+    if (!(fabsf(b[y]) >= 1.1754944e-38f) && v[y] != 0.0f) b[y] = copysignf(1.1754944e-38f, v[y]);  // (2^-126; of infinities too)
+  }
+  store4(dst, make_float4(a[0], a[1], a[2], a[3]));
+  store4(dst + plane, make_float4(b[0], b[1], b[2], b[3]));
+}
+
 // One block per new row: its k and v go to its position's page, rounded to the
-// cache's type; q_rows (if not null) gets q in that type, [rows, heads, head_dim].
+// cache's type; q_rows (if not null) gets q, [rows, heads, head_dim], see store_q.
 // 16 rows of 12 x 64 take 5.3 us on a B200 and 964 of 32 / 8 x 128 6.3: the latency of a load and
 // a store, during which the attention kernel is launched and makes its list.
 constexpr int kRowThreads = 256;
 template <typename TX, typename TC>
-__global__ void __launch_bounds__(kRowThreads) append_kernel(const __grid_constant__ Args a, TC* q_rows) {
+__global__ void __launch_bounds__(kRowThreads) append_kernel(const __grid_constant__ Args a, __nv_bfloat16* q_rows) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t r = blockIdx.x;
   const int quads = a.head_dim / 4;
   if (q_rows) {
     for (int e = threadIdx.x; e < a.heads * quads; e += kRowThreads) {
       const int h = e / quads, d = (e - h * quads) * 4;
-      store4(q_rows + (r * a.heads + h) * a.head_dim + d, load4(static_cast<const TX*>(a.q) + r * a.q_row + h * a.q_head + d));
+      store_q<TX>(q_rows + (r * a.heads + h) * a.head_dim + d, a.rows * a.heads * a.head_dim,
+                  load4(static_cast<const TX*>(a.q) + r * a.q_row + h * a.q_head + d));
     }
   }
   if (!a.k) return;
@@ -96,18 +119,24 @@ __global__ void __launch_bounds__(kRowThreads) append_kernel(const __grid_consta
   }
 }
 
-// Rows of q, k and v in bf16, [rows, heads + 2 kv_heads, head_dim]: 60 rows of 12 x 64 4.2 us.
+// q (see store_q), [rows, heads, head_dim], and k and v in bf16, [rows, 2 kv_heads, head_dim]: 60
+// rows of 12 x 64 4.2 us.
 template <typename TX>
-__global__ void __launch_bounds__(kRowThreads) cast_kernel(const __grid_constant__ Args a, __nv_bfloat16* rows) {
+__global__ void __launch_bounds__(kRowThreads)
+    cast_kernel(const __grid_constant__ Args a, __nv_bfloat16* q_rows, __nv_bfloat16* kv_rows) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t r = blockIdx.x;
-  const int hq = a.heads, hk = a.kv_heads, all = hq + 2 * hk, quads = a.head_dim / 4;
-  for (int e = threadIdx.x; e < all * quads; e += kRowThreads) {
+  const int hq = a.heads, hk = a.kv_heads, quads = a.head_dim / 4;
+  for (int e = threadIdx.x; e < (hq + 2 * hk) * quads; e += kRowThreads) {
     const int h = e / quads, d = (e - h * quads) * 4;
-    const TX* src = h < hq        ? static_cast<const TX*>(a.q) + r * a.q_row + h * a.q_head
-                    : h < hq + hk ? static_cast<const TX*>(a.k) + r * a.k_row + (h - hq) * a.k_head
-                                  : static_cast<const TX*>(a.v) + r * a.v_row + (h - hq - hk) * a.v_head;
-    store4(rows + (r * all + h) * a.head_dim + d, load4(src + d));
+    if (h < hq) {
+      store_q<TX>(q_rows + (r * hq + h) * a.head_dim + d, a.rows * hq * a.head_dim,
+                  load4(static_cast<const TX*>(a.q) + r * a.q_row + h * a.q_head + d));
+      continue;
+    }
+    const TX* src = h < hq + hk ? static_cast<const TX*>(a.k) + r * a.k_row + (h - hq) * a.k_head
+                                : static_cast<const TX*>(a.v) + r * a.v_row + (h - hq - hk) * a.v_head;
+    store4(kv_rows + (r * 2 * hk + h - hq) * a.head_dim + d, load4(src + d));
   }
 }
 
@@ -170,11 +199,12 @@ int cuda_status(cudaError_t e, const char* what) {
 
 size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-// Workspace of the tensor-core path: 4 KiB of tickets, as in every call's | cast rows | partials of cut tiles.
+// Workspace of the tensor-core path: 4 KiB of tickets, as in every call's | q's planes | whole
+// prompts' k and v, where they are cast | partials of cut tiles.
 struct TcLayout {
-  int grid, slot_tokens, part_rows;
+  int grid, slot_tokens, part_rows, planes;
   bool cast;
-  size_t off_rows, off_ml, off_part, total;
+  size_t off_q, off_kv, off_ml, off_part, total;
 };
 
 // TMA reads rows of the kernel's own type whose strides are not zero.
@@ -190,9 +220,12 @@ TcLayout tc_layout(const Args& a, int sm_count) {
   l.slot_tokens = 128 / group;
   l.part_rows = a.rows > l.slot_tokens ? 256 : (int)((a.rows * group + 31) / 32 * 32);
   l.cast = needs_cast(a);
-  const int dp = a.head_dim <= 64 ? 64 : 128, heads = a.heads + (a.k_pages ? 0 : 2 * a.kv_heads);
-  l.off_rows = 4096;
-  l.off_ml = l.off_rows + (l.cast ? round256((size_t)a.rows * heads * a.head_dim * 2) : 0);
+  l.planes = a.x_dtype == MTRTQ_DTYPE_F32 ? 2 : 1;
+  const int dp = a.head_dim <= 64 ? 64 : 128;
+  const size_t row = (size_t)a.rows * a.head_dim * 2;  // of one head
+  l.off_q = 4096;
+  l.off_kv = l.off_q + (l.cast ? round256(row * a.heads * l.planes) : 0);
+  l.off_ml = l.off_kv + (l.cast && !a.k_pages ? round256(row * 2 * a.kv_heads) : 0);
   l.off_part = l.off_ml + round256((size_t)l.grid * 2 * l.part_rows * sizeof(float2));
   l.total = l.off_part + (size_t)l.grid * 2 * l.part_rows * dp * sizeof(float);
   return l;
@@ -245,20 +278,20 @@ void fill_list(const Args& a, bool paged, AttentionList& p) {
   p.max_keys = a.table_width * a.page_size;
 }
 
-// Stores the new tokens' k and v in the pages, and writes q (whole prompts: q, k and v) in
-// bf16 to rows if not null.
-int launch_new_rows(const Args& a, bool paged, __nv_bfloat16* rows, cudaStream_t st) {
+// Stores the new tokens' k and v in the pages, and writes q (whole prompts: q, k and v) for the
+// tensor cores to q_rows (and kv_rows) if not null.
+int launch_new_rows(const Args& a, bool paged, __nv_bfloat16* q_rows, __nv_bfloat16* kv_rows, cudaStream_t st) {
   const unsigned grid = (unsigned)a.rows;
   const bool x16 = a.x_dtype != MTRTQ_DTYPE_F32;
   if (!paged) {
-    if (x16) cast_kernel<__nv_bfloat16><<<grid, kRowThreads, 0, st>>>(a, rows);
-    else cast_kernel<float><<<grid, kRowThreads, 0, st>>>(a, rows);
+    if (x16) cast_kernel<__nv_bfloat16><<<grid, kRowThreads, 0, st>>>(a, q_rows, kv_rows);
+    else cast_kernel<float><<<grid, kRowThreads, 0, st>>>(a, q_rows, kv_rows);
   } else if (a.dtype == MTRTQ_DTYPE_F32) {
     append_kernel<float, float><<<grid, kRowThreads, 0, st>>>(a, nullptr);
   } else if (x16) {
-    append_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, kRowThreads, 0, st>>>(a, rows);
+    append_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, kRowThreads, 0, st>>>(a, q_rows);
   } else {
-    append_kernel<float, __nv_bfloat16><<<grid, kRowThreads, 0, st>>>(a, rows);
+    append_kernel<float, __nv_bfloat16><<<grid, kRowThreads, 0, st>>>(a, q_rows);
   }
   return cuda_status(cudaGetLastError(), "attention rows launch");
 }
@@ -267,20 +300,20 @@ int launch_new_rows(const Args& a, bool paged, __nv_bfloat16* rows, cudaStream_t
 int launch_tc(const Args& a, bool paged, const TcLayout& l, int least, bool after, void* workspace, unsigned* status,
               cudaStream_t st) {
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  __nv_bfloat16* rows = reinterpret_cast<__nv_bfloat16*>(ws + l.off_rows);
   Args x = a;
   if (l.cast) {
-    const int64_t row = (int64_t)(a.heads + (paged ? 0 : 2 * a.kv_heads)) * a.head_dim;
-    x.q = rows;
-    x.k = rows + (int64_t)a.heads * a.head_dim;
-    x.v = rows + (int64_t)(a.heads + a.kv_heads) * a.head_dim;
-    x.q_row = x.k_row = x.v_row = row;
+    __nv_bfloat16* kv = reinterpret_cast<__nv_bfloat16*>(ws + l.off_kv);
+    x.q = ws + l.off_q;
+    x.q_row = (int64_t)a.heads * a.head_dim;
+    x.k = kv;
+    x.v = kv + (int64_t)a.kv_heads * a.head_dim;
+    x.k_row = x.v_row = (int64_t)2 * a.kv_heads * a.head_dim;
     x.q_head = x.k_head = x.v_head = a.head_dim;
   }
   const int group = a.heads / a.kv_heads;
   CUtensorMap qm, km, vm;
   {
-    const int64_t dims[4] = {a.head_dim, group, a.kv_heads, a.rows};
+    const int64_t dims[4] = {a.head_dim, group, a.kv_heads, l.planes * a.rows};
     const int64_t strides[3] = {x.q_head, x.q_head * group, x.q_row};
     const int box[4] = {64, group, 1, l.slot_tokens};
     if (int rc = make_map(&qm, x.q, 4, dims, strides, box)) return rc;
@@ -304,7 +337,9 @@ int launch_tc(const Args& a, bool paged, const TcLayout& l, int least, bool afte
   fill_list(a, paged, p);
   p.least = least;
   p.slot_tokens = l.slot_tokens;
-  p.tile_tokens = 2 * l.slot_tokens;
+  p.planes = l.planes == 2;
+  p.q_buffers = p.planes && a.head_dim > 64 ? 1 : 2;
+  p.tile_tokens = p.q_buffers * l.slot_tokens;
   p.min_steps = 4;
   p.tile_cost = 3;
   p.pair_cost = 3;
@@ -416,6 +451,7 @@ int launch_f32(const Args& a, bool paged, const F32Layout& l, int least, int mos
   p.least = least;
   p.most = most;
   p.slot_tokens = 0;
+  p.q_buffers = 1;
   p.tile_tokens = l.tile_rows / p.group;
   p.min_steps = 2;
   p.pair_cost = l.tile_rows == 128;  // (every f32 tile is of that kind)
@@ -478,10 +514,12 @@ int attention(const Args* a, bool paged, void* workspace, size_t workspace_bytes
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Plan p = plan_call(*a);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  __nv_bfloat16* rows = p.tc.cast ? reinterpret_cast<__nv_bfloat16*>(ws + p.tc.off_rows) : nullptr;
-  const bool before = rows || (paged && a->k);
-  if (before)
-    if ((rc = launch_new_rows(*a, paged, rows, st))) return rc;
+  __nv_bfloat16* q_rows = p.tc.cast ? reinterpret_cast<__nv_bfloat16*>(ws + p.tc.off_q) : nullptr;
+  const bool before = q_rows || (paged && a->k);
+  if (before) {
+    rc = launch_new_rows(*a, paged, q_rows, reinterpret_cast<__nv_bfloat16*>(ws + p.tc.off_kv), st);
+    if (rc) return rc;
+  }
   if (a->dtype == MTRTQ_DTYPE_F32) {
     rc = launch_f32(*a, paged, p.f32, 1, p.both ? kFewTokens32 : INT_MAX, before, ws, ws, status, st);
     if (rc == MTRTQ_OK && p.both)

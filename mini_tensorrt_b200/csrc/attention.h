@@ -18,6 +18,7 @@ struct AttentionList {
   int64_t rows;
   int batch, kv_heads, group, head_dim, page_size;
   int slot_tokens;    // tensor cores: 128 / group, the tokens in a slot's 128 rows
+  int q_buffers;      // and whether the next tile's Q has a place of its own (2)
   int tile_tokens;
   int least, most;    // tokens of the requests that this launch takes
   int64_t max_keys;   // paged: tokens the table's columns hold
@@ -27,6 +28,7 @@ struct AttentionList {
 
 struct TcAttention : AttentionList {
   float scale;
+  bool planes;  // q lies in two planes of `rows` rows
   __nv_bfloat16* out;
   int64_t out_row, out_head;
   bool out32;  // rows of out start on 32 bytes

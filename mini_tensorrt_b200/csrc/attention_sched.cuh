@@ -141,7 +141,7 @@ __device__ bool next_segment(const AttentionList& p, const StepList list, Walk& 
       w.buf = 0;
     } else {
       ++w.q_use[w.buf];
-      w.buf ^= 1;
+      w.buf = p.q_buffers - 1 - w.buf;
     }
     return true;
   }

@@ -15,9 +15,14 @@
 // otherwise both hold the same rows and take alternate key blocks ("halves"), joined at
 // the end -- which is what a single token over a long cache needs.
 //
-// Roundings: the weights to bf16 (their sum is that of the unrounded ones), and f32 rows of q
-// to bf16. A second plane of q is no way out: its zeros times an infinite k would be NaN where
-// the score is -inf. (A row or two of a request go to attention_f32.cu, which rounds neither.)
+// Roundings: the weights to bf16 (their sum is that of the unrounded ones). f32 rows of q are two
+// bf16 planes of 16 bits together (attention.cu, store_q) and S the sum of both products, the
+// smaller first: half as many products again, which cost prompts of 1024 + 700 + 333 + 1019 tokens, 12
+// heads of 64, 49 us in place of 46, and, as two planes of 128 dimensions leave room for one
+// tile's Q only, 8192 tokens of 32 heads over 8 of 128 928 in place of 698. One plane left errors
+// 1.7 times those of fp32 arithmetic (2.8e-3 against 1.6e-3 of the result) at scores of a few, and
+// as many times more at larger ones. (A row or two of a request go to attention_f32.cu, which
+// rounds neither.)
 //
 // Work: a step is one block for each slot. The steps of all tiles of all requests form
 // one list, cut into equal runs over one CTA per SM; every CTA finds its own run from
@@ -37,6 +42,8 @@
 // rows that see them.
 #include <math.h>
 
+#include <type_traits>
+
 #include "../../include/mtrtq.h"
 #include "attention_mma.cuh"
 
@@ -50,12 +57,15 @@ constexpr int kBadMax = 384;  // listed V rows of a tile: three blocks
 
 constexpr int kRing = 4;  // segments that the roles may lie apart
 
-template <int DP>
+// PLANES: of Q. Two of 128 dimensions leave shared memory for one tile's, so that the slots
+// always have the same rows and the next tile's Q is not loaded ahead.
+template <int DP, int PLANES>
 struct Cfg {
   static constexpr int TILE = kBlock * DP * 2;  // Q, K or V block in shared memory
   static constexpr int STAGES = DP == 128 ? 4 : 8;
+  static constexpr int Q_BUFFERS = DP == 128 && PLANES == 2 ? 1 : 2;
   static constexpr int OFF_Q = 0;
-  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int OFF_KV = Q_BUFFERS * PLANES * TILE;
   static constexpr int OFF_LIST = OFF_KV + STAGES * TILE;
   static constexpr int OFF_SEG = OFF_LIST + MTRTQ_MAX_BATCH * sizeof(Request);
   static constexpr int OFF_ML = OFF_SEG + kRing * ((sizeof(Segment) + 15) / 16 * 16);  // slot 1's (m, l)
@@ -138,11 +148,11 @@ __device__ __forceinline__ void join_parts(const TcAttention& p, int c_first, in
 
 // After a bounded wait gives up, every role's next wait fails at once and it leaves its
 // loop for the barrier at the end; there is no other barrier without a limit.
-template <int DP, bool PAGED>
+template <int DP, bool PAGED, int PLANES>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const __grid_constant__ TcAttention p) {
-  using C = Cfg<DP>;
+  using C = Cfg<DP, PLANES>;
   constexpr int NH = DP / 64;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -500,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int q_sent[2] = {0, 0};
       const int pages = PAGED ? kBlock / p.page_size : 1;
       const uint32_t box = (PAGED ? p.page_size : kBlock) * 128;
-      const uint32_t rows_bytes = (uint32_t)p.slot_tokens * p.group * 128 * NH;
+      const uint32_t rows_bytes = (uint32_t)p.slot_tokens * p.group * 128 * NH * PLANES;
       bool ok = true;
 #pragma unroll 1
       for (int seg = 0; ok; ++seg) {
@@ -530,9 +540,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++q_sent[buf];
           if (lane == 0) mbar_arrive_expect_tx(&q_full[buf], rows_bytes);
           __syncwarp();
-          if (lane < NH)
-            tma_load_4d(smem + C::OFF_Q + buf * C::TILE + lane * kBlock * 128, &qmap, lane * 64, 0, s.h,
-                        s.row0 + t * p.slot_tokens, &q_full[buf]);
+          if (lane < NH * PLANES)
+            tma_load_4d(smem + C::OFF_Q + (buf * PLANES * NH + lane) * kBlock * 128, &qmap, lane % NH * 64, 0, s.h,
+                        lane / NH * (int)p.rows + s.row0 + t * p.slot_tokens, &q_full[buf]);
         }
 #pragma unroll 1
         for (int at = 0; ok && at < 2 * n; ++at) {
@@ -598,14 +608,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto take_turn = [&]() { return wait(&turn[t], (n_turn++ & 1) ^ (t ^ 1)); };
       auto end_turn = [&]() { mbar_arrive(&turn[t ^ 1]); };
       auto landed = [&]() { return wait(&full[seq % C::STAGES], (seq / C::STAGES) & 1); };
-      // The scores of a block; the other slot may go on shortly before the end.
+      // The scores of a block, q's smaller plane first; the other slot may go on shortly
+      // before the end.
       auto scores = [&](uint32_t q, uint32_t k) {
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          if (i == DP / 32) end_turn();
-          if (i < ksteps)
-            mma_ss(s_col, q + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2,
-                   k + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2, idesc_s, i > 0);
+        for (int plane = PLANES - 1; plane >= 0; --plane) {
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i) {
+            if (plane == 0 && i == DP / 32) end_turn();
+            if (i < ksteps)
+              mma_ss(s_col, q + plane * (C::TILE >> 4) + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2,
+                     k + (i >> 2) * (kBlock * 128 >> 4) + (i & 3) * 2, idesc_s, plane < PLANES - 1 || i > 0);
+          }
         }
         umma_commit(&s_full[t]);
       };
@@ -624,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ok = ok && wait(&q_full[buf], s.q_use[buf] & 1);
           if (cnt == 0) mbar_arrive(&q_free[buf]);
-          const uint32_t q = q_desc + buf * (C::TILE >> 4), first = seq;
+          const uint32_t q = q_desc + buf * (PLANES * C::TILE >> 4), first = seq;
           // Passes over the loads of the other slot's blocks before `to`.
           auto skip = [&](uint32_t to) {
 #pragma unroll 1
@@ -781,15 +795,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int DP, bool PAGED>
+template <int DP, bool PAGED, int PLANES>
 cudaError_t launch_one(const TcAttention& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, int grid,
                        bool pdl, cudaStream_t st) {
-  auto kernel = attention_tc_kernel<DP, PAGED>;
-  if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kernel), Cfg<DP>::BYTES)) return e;
+  auto kernel = attention_tc_kernel<DP, PAGED, PLANES>;
+  if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kernel), Cfg<DP, PLANES>::BYTES)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<DP>::BYTES;
+  cfg.dynamicSmemBytes = Cfg<DP, PLANES>::BYTES;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -803,9 +817,13 @@ cudaError_t launch_one(const TcAttention& p, const CUtensorMap& q, const CUtenso
 
 cudaError_t launch_attention_tc(const TcAttention& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                                 int grid, bool pdl, cudaStream_t st) {
-  if (p.head_dim <= 64)
-    return p.table ? launch_one<64, true>(p, q, k, v, grid, pdl, st) : launch_one<64, false>(p, q, k, v, grid, pdl, st);
-  return p.table ? launch_one<128, true>(p, q, k, v, grid, pdl, st) : launch_one<128, false>(p, q, k, v, grid, pdl, st);
+  auto run = [&](auto planes) {
+    constexpr int P = decltype(planes)::value;
+    if (p.head_dim <= 64)
+      return p.table ? launch_one<64, true, P>(p, q, k, v, grid, pdl, st) : launch_one<64, false, P>(p, q, k, v, grid, pdl, st);
+    return p.table ? launch_one<128, true, P>(p, q, k, v, grid, pdl, st) : launch_one<128, false, P>(p, q, k, v, grid, pdl, st);
+  };
+  return p.planes ? run(std::integral_constant<int, 2>()) : run(std::integral_constant<int, 1>());
 }
 
 }  // namespace mtrtq
