@@ -49,16 +49,14 @@ def _call(where: str, index: int, *args) -> None:
 
 def _other_stream(stream, stream_ptr: int, index: int):
     """The call's stream as torch's, None if it is the current one."""
-    if stream_ptr == torch._C._cuda_getCurrentRawStream(index):
+    if stream is None or stream_ptr == torch._C._cuda_getCurrentRawStream(index):
         return None
     return stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(stream_ptr, device=index)
 
 
 def _made_there(other, device, make):
-    """What make() allocates, from the memory of the call's stream (other, or the current one),
-    and kept from being given out again before the current stream's work with it is done."""
-    if other is None:
-        return make()
+    """What make() allocates, from the memory of `other`, the call's stream, and kept from being
+    given out again before the current stream's work with it is done."""
     with torch.cuda.stream(other):
         made = make()
     for x in made:
@@ -78,10 +76,12 @@ def _workspace(workspace, device, stream_ptr: int, other, nbytes: int) -> torch.
             workspace = _workspaces[key] = Workspace(device)
     if not isinstance(workspace, Workspace):
         return workspace
-    if workspace.buf is None or workspace.buf.numel() < nbytes:
-        with torch.cuda.stream(other):
-            if torch.cuda.is_current_stream_capturing():
-                return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    buf = workspace.buf
+    if buf is not None and buf.numel() >= nbytes:
+        return buf
+    with torch.cuda.stream(other):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.zeros(nbytes, dtype=torch.uint8, device=device)
     return workspace.get(nbytes, other)
 
 
@@ -124,8 +124,10 @@ def _attend(where, q, k, v, out, out_dtype, kv_heads, cu_rows, scale, workspace,
     sp = _stream_ptr(stream, index)
     other = _other_stream(stream, sp, index)
     if out is None:
-        out, = _made_there(other, device, lambda: (torch.empty_like(
-            q, dtype=out_dtype, memory_format=torch.contiguous_format),))
+        if other is None:
+            out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
+        else:
+            out, = _made_there(other, device, lambda: [torch.empty(shape, dtype=out_dtype, device=device)])
         os = (H * D, D)
     else:
         os = _rows("out", out, shape, out_dtype, device)
@@ -217,9 +219,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, done: torch.Tensor, 
     sp = _stream_ptr(stream, dev.index)
     other = _other_stream(stream, sp, dev.index)
     if out is None:
-        out = _made_there(other, dev, lambda: (
-            torch.empty_like(scores), torch.empty_like(scores, dtype=torch.int32),
-            torch.empty_like(scores, dtype=torch.int32), torch.empty_like(done)))
+        make = lambda: (torch.empty_like(scores), torch.empty_like(scores, dtype=torch.int32),
+                        torch.empty_like(scores, dtype=torch.int32), torch.empty_like(done))
+        out = make() if other is None else _made_there(other, dev, make)
     else:
         for x, t in zip(out, (torch.float32, torch.int32, torch.int32, torch.uint8), strict=True):
             if x.shape != scores.shape or x.dtype != t or x.device != dev or not x.is_contiguous():
