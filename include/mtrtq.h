@@ -590,7 +590,9 @@ int mtrtq_paged_attention(const mtrtq_attention_args* a, void* workspace, size_t
  * eos), best first. logits [requests * beams, ldl] f32; scores, done (0 or 1), parent,
  * token, out_scores, out_done [requests, beams]. NaN logits count as -infinity, so do
  * candidates whose score is NaN; a beam not in use has the score -infinity. eos may be
- * -1 (none ends; done must then be 0). outputs must not overlap inputs.
+ * -1 (none ends; done must then be 0). outputs must not overlap inputs. Rows of logits are
+ * read in whole 16-byte lines, so up to 12 bytes before and behind a row (and what they hold is
+ * not used).
  * beams * vocab is at most 2^31 - 2^14. The greedy step is mtrtq_argmax_rows
  * (tools/run_gpt2.cpp:42-47). */
 #define MTRTQ_MAX_BEAMS 32

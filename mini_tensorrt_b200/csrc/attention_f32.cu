@@ -316,9 +316,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<HD, RM>::CTAS)
 // keys' K and V (eight of bf16) are loaded together and used straight from the registers,
 // without shared memory or barriers. Every such group of lanes keeps its own maximum, sum and output; they
 // are joined when the CTA's run of the tile ends. 32 requests of 1500 tokens, 12 heads of 64,
-// take 61 us on a B200: 4.9 TB/s. With a bf16 cache, where q and the weights stay in fp32, the
-// instructions for each element weigh twice as much: 64 requests of 2000 tokens take 101 us,
-// 3.9 TB/s; with four keys of bf16 together 109.
+// take 56 us on a B200: 5.2 TB/s. With a bf16 cache, where q and the weights stay in fp32, the
+// instructions for each element weigh twice as much: 64 requests of 2000 tokens take 91 us,
+// 4.3 TB/s; with four keys of bf16 together 8 % more.
 template <typename T>
 struct Eight {  // dimensions of a row, as they are read
   uint4 u[sizeof(T) / 2];
