@@ -112,3 +112,22 @@ def test_masks_cost_no_more_than_other_logits(cuda_device):
     scores[:, 1:] = -INF
     for x in masked.values():
         assert took(x) < 10 * usual
+
+
+@pytest.mark.parametrize("mask", [-INF, LOWEST], ids=["inf", "lowest"])
+@pytest.mark.parametrize("beam", [0, 17, 31])
+def test_one_beam_of_many_in_use(cuda_device, mask, beam):
+    """Its chunks come after hundreds of others', and ties start in the middle of one."""
+    W, V = 32, 50257
+    logits = randn(make_gen(beam), W, V)
+    logits[beam] = -INF
+    logits[beam, 30000:] = mask
+    logits[beam, 40000:40005] = torch.tensor([4.0, 8.0, 0.0, 2.0, 6.0], device="cuda")
+    scores = torch.full((1, W), -INF, device="cuda")
+    scores[0, beam] = -3.0
+    done = torch.zeros((1, W), dtype=torch.uint8, device="cuda")
+    got = serving.beam_select(logits, scores, done)
+    want = expected(logits, scores, done, -1)
+    assert pairs(got) == want
+    first = [(beam, 40000 + i) for i in (1, 4, 0, 3, 2)]
+    assert want[0][:5] == first and want[0][5] == ((beam, 30000) if mask == LOWEST else (0, 0))
